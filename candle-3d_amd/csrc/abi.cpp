@@ -480,6 +480,63 @@ int lux3d_gated_residual_adaln_modulate(const lux3d_tensor_t *x, const lux3d_ten
   return hip_status(launch_rows(ROW_GATE_MOD, x->dtype, p, vec, stream_of(stream)), fn);
 }
 
+int lux3d_norm_gated_residual_norm(const lux3d_tensor_t *x, const lux3d_tensor_t *h, const lux3d_tensor_t *post_w,
+                                   const lux3d_tensor_t *post_b, const lux3d_tensor_t *ls_gamma,
+                                   const lux3d_tensor_t *seg_offsets, const lux3d_tensor_t *gate,
+                                   const lux3d_tensor_t *gate_base, const lux3d_tensor_t *pre_w,
+                                   const lux3d_tensor_t *pre_b, const lux3d_tensor_t *shift,
+                                   const lux3d_tensor_t *shift_base, const lux3d_tensor_t *scale,
+                                   const lux3d_tensor_t *scale_base, int32_t rms, float eps,
+                                   const lux3d_tensor_t *x_out, const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_norm_gated_residual_norm";
+  RowView xv, hv, xov, yv{};
+  int r;
+  if ((r = row_tensor(x, fn, "x", -1, xv))) return r;
+  if ((r = row_tensor(h, fn, "h", x->dtype, hv))) return r;
+  if ((r = row_tensor(x_out, fn, "x_out", x->dtype, xov))) return r;
+  if ((r = same_rows(xv, hv, fn, "h")) || (r = same_rows(xv, xov, fn, "x_out"))) return r;
+  if (xv.d == 0) return fail(LUX3D_ERR_SHAPE, "%s: empty rows", fn);
+  if (y) {
+    if ((r = row_tensor(y, fn, "y", x->dtype, yv))) return r;
+    if ((r = same_rows(xv, yv, fn, "y"))) return r;
+    if (xv.rows > 0 && (yv.p == xv.p || yv.p == xov.p))
+      return fail(LUX3D_ERR_LAYOUT, "%s: `y` must not alias `x` or `x_out`", fn);
+  } else if (pre_w || pre_b || shift || scale) {
+    return fail(LUX3D_ERR_NULL, "%s: `y` is NULL while parameters of its norm are given", fn);
+  }
+  if (rms != 0 && rms != 1) return fail(LUX3D_ERR_VALUE, "%s: rms must be 0 (LayerNorm) or 1 (RMSNorm)", fn);
+  if (!(eps >= 0.f)) return fail(LUX3D_ERR_VALUE, "%s: eps must be >= 0", fn);
+  BlockNormParams p;
+  if ((r = param_vec(post_w, xv.d, fn, "post_w", p.post_w, p.post_w_dt)) ||
+      (r = param_vec(post_b, xv.d, fn, "post_b", p.post_b, p.post_b_dt)) ||
+      (r = param_vec(ls_gamma, xv.d, fn, "ls_gamma", p.gamma, p.gamma_dt)) ||
+      (r = param_vec(pre_w, xv.d, fn, "pre_w", p.pre_w, p.pre_w_dt)) ||
+      (r = param_vec(pre_b, xv.d, fn, "pre_b", p.pre_b, p.pre_b_dt)))
+    return r;
+  int64_t s_g = 0, s_sh = 0, s_sc = 0;
+  if ((r = mod_piece(gate, gate_base, xv.d, fn, "gate", p.gate, s_g)) ||
+      (r = mod_piece(shift, shift_base, xv.d, fn, "shift", p.shift, s_sh)) ||
+      (r = mod_piece(scale, scale_base, xv.d, fn, "scale", p.scale, s_sc)))
+    return r;
+  const int64_t nseg = gate ? s_g : shift ? s_sh : scale ? s_sc : 1;
+  if ((shift && s_sh != nseg) || (scale && s_sc != nseg))
+    return fail(LUX3D_ERR_SHAPE, "%s: gate/shift/scale have different segment counts", fn);
+  if (nseg < 1) return fail(LUX3D_ERR_SHAPE, "%s: gate/shift/scale have no segment", fn);
+  RowParams seg;
+  if ((r = segments(seg_offsets, xv.rows, nseg, fn, seg))) return r;
+  p.seg_off = seg.seg_off; p.nseg = seg.nseg; p.rows_per_seg = seg.rows_per_seg;
+  p.x = xv.p; p.x_rs = xv.rs;
+  p.h = hv.p; p.h_rs = hv.rs;
+  p.x_out = const_cast<void *>(xov.p); p.xo_rs = xov.rs;
+  if (y) p.y = const_cast<void *>(yv.p), p.y_rs = yv.rs;
+  p.rows = xv.rows; p.d = xv.d; p.eps = eps; p.rms = rms != 0;
+  const bool vec = vec_ok_rows({xv, hv, xov}) && (!y || vec_ok_rows({yv})) && param_aligned(p.post_w, p.post_w_dt) &&
+                   param_aligned(p.post_b, p.post_b_dt) && param_aligned(p.gamma, p.gamma_dt) &&
+                   param_aligned(p.pre_w, p.pre_w_dt) && param_aligned(p.pre_b, p.pre_b_dt) && vec_ok_piece(p.gate) &&
+                   vec_ok_piece(p.shift) && vec_ok_piece(p.scale);
+  return hip_status(launch_block_norm(x->dtype, p, vec, stream_of(stream)), fn);
+}
+
 // ---------------------------------------------------------------------------
 
 namespace {

@@ -43,6 +43,28 @@ struct RowParams {
 // kernels (the caller has checked alignment and d % 8 == 0).
 hipError_t launch_rows(int mode, int dt, const RowParams &p, bool vec, hipStream_t s);
 
+// ---- norms on both sides of a residual sum (block_norm.hip) --------------------
+// x_out = x + Norm(h; post_w, post_b) * gamma * gate; y = Norm(x_out; pre_w,
+// pre_b) * (scale + 1) + shift; y null: x_out alone. Absent vectors have dt < 0.
+struct BlockNormParams {
+  const void *x = nullptr; int64_t x_rs = 0;
+  const void *h = nullptr; int64_t h_rs = 0;
+  void *x_out = nullptr;   int64_t xo_rs = 0;
+  void *y = nullptr;       int64_t y_rs = 0;
+  int64_t rows = 0, d = 0;
+  float eps = 0.f;
+  bool rms = false;
+  const void *post_w = nullptr; int post_w_dt = -1;
+  const void *post_b = nullptr; int post_b_dt = -1;
+  const void *gamma = nullptr;  int gamma_dt = -1;
+  const void *pre_w = nullptr;  int pre_w_dt = -1;
+  const void *pre_b = nullptr;  int pre_b_dt = -1;
+  const int64_t *seg_off = nullptr;  // [nseg + 1] or NULL
+  int64_t nseg = 1, rows_per_seg = 1;
+  ModPiece gate, shift, scale;
+};
+hipError_t launch_block_norm(int dt, const BlockNormParams &p, bool vec, hipStream_t s);
+
 // ---- head family: per-head norm + rotary on [B, H, N, D] views ------------
 enum HeadNorm : int { HN_NONE = 0, HN_LN = 1, HN_RMS = 2, HN_L2 = 3 };
 enum HeadRot : int {

@@ -10,6 +10,7 @@ the reference's `candle_core::bail!` sites return an error.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import struct
@@ -63,6 +64,25 @@ def _stream(t: torch.Tensor) -> int:
     if t.is_cuda:  # the handle itself, without a torch.cuda.Stream around it
         return torch._C._cuda_getCurrentRawStream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _one_device(fn: str, first: torch.Tensor, *rest):
+    """Every tensor of a call lives on the first one's GPU."""
+    if not first.is_cuda:
+        raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"the tensors must be on a GPU, not on {first.device}")
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"tensors on {first.device} and {t.device} in one call")
+
+
+def _device_of(t: torch.Tensor):
+    """The launch goes to t's GPU, whichever is current (the default stream's
+    handle names the current device's)."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _keep(*ts):
@@ -140,6 +160,32 @@ def gated_residual_adaln_modulate(x: torch.Tensor, h: torch.Tensor, gate: Option
     _lib.call("lux3d_gated_residual_adaln_modulate", _d(x), _d(h), _d(seg_offsets), _d(gate),
               _d(gate_base), _d(shift), _d(shift_base), _d(scale), _d(scale_base), eps, _d(xo),
               _d(y), _stream(x))
+    return xo, y
+
+
+def norm_gated_residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,
+                             post_bias: Optional[torch.Tensor] = None, ls_gamma: Optional[torch.Tensor] = None,
+                             gate: Optional[torch.Tensor] = None, gate_base=None,
+                             pre_weight: Optional[torch.Tensor] = None, pre_bias: Optional[torch.Tensor] = None,
+                             shift: Optional[torch.Tensor] = None, shift_base=None,
+                             scale: Optional[torch.Tensor] = None, scale_base=None,
+                             seg_offsets: Optional[torch.Tensor] = None, norm: str = "rms", eps: float = 1e-6,
+                             x_out: Optional[torch.Tensor] = None, next_norm: bool = True):
+    """The residual sum of a block with a norm on both sides, in one pass:
+    `xs = xs + norm(h)*ls_gamma*gate`, `y = norm(xs)*(1 + scale) + shift`, with
+    norm "layer" or "rms" (weight and bias each optional). Returns (x_out, y);
+    x_out may be x (in-place residual update). next_norm False (the last
+    block): the residual sum alone, y is None."""
+    if norm not in ("layer", "rms"):
+        raise _lib.Lux3dError("lux3d_norm_gated_residual_norm", _lib.ERR_VALUE, f"norm must be 'layer' or 'rms', not {norm!r}")
+    _one_device("lux3d_norm_gated_residual_norm", x, h, post_weight, post_bias, ls_gamma, seg_offsets, gate, gate_base,
+                pre_weight, pre_bias, shift, shift_base, scale, scale_base, x_out)
+    with _device_of(x):
+        xo = _new(x) if x_out is None else x_out
+        y = _new(x) if next_norm else None
+        _lib.call("lux3d_norm_gated_residual_norm", _d(x), _d(h), _d(post_weight), _d(post_bias), _d(ls_gamma),
+                  _d(seg_offsets), _d(gate), _d(gate_base), _d(pre_weight), _d(pre_bias), _d(shift), _d(shift_base),
+                  _d(scale), _d(scale_base), 1 if norm == "rms" else 0, eps, _d(xo), _d(y), _stream(x))
     return xo, y
 
 

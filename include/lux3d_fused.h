@@ -172,6 +172,32 @@ int lux3d_gated_residual_adaln_modulate(const lux3d_tensor_t *x, const lux3d_ten
                                         const lux3d_tensor_t *y, lux3d_stream_t stream);
 
 /* --------------------------------------------------------------------------
+ * Norms on both sides of a block's residual sum, in one pass over the rows:
+ *   x_out = x + Norm(h; post_w, post_b)*ls_gamma*gate
+ *   y     = Norm(x_out; pre_w, pre_b)*(scale + 1) + shift
+ * Norm is LayerNorm (rms 0) or RMSNorm (rms 1: v / sqrt(mean(v^2) + eps), no
+ * mean); both norms of a call are of one kind and one eps. h is the block's
+ * (attention's or feed-forward's) raw output, y the next block's input.
+ * post_w / post_b / ls_gamma / pre_w / pre_b: [C] vectors, each may be NULL
+ * (factor 1, summand 0); gate / shift / scale (+ *_base) and seg_offsets as in
+ * lux3d_adaln_modulate, each piece may be NULL, those given share one segment
+ * count. y NULL (the last block): x_out alone, without pre_* / shift / scale.
+ * f32 arithmetic, x_out rounded once; y is computed from the stored (rounded)
+ * x_out. x_out may alias x; y must not alias x or x_out. One kernel. The
+ * reference's blocks norm on one side only: this is the form of blocks with a
+ * norm on each (its residual sum is lux3d_gated_residual's up to the norm).   */
+int lux3d_norm_gated_residual_norm(const lux3d_tensor_t *x, const lux3d_tensor_t *h,
+                                   const lux3d_tensor_t *post_w, const lux3d_tensor_t *post_b,
+                                   const lux3d_tensor_t *ls_gamma,
+                                   const lux3d_tensor_t *seg_offsets,
+                                   const lux3d_tensor_t *gate, const lux3d_tensor_t *gate_base,
+                                   const lux3d_tensor_t *pre_w, const lux3d_tensor_t *pre_b,
+                                   const lux3d_tensor_t *shift, const lux3d_tensor_t *shift_base,
+                                   const lux3d_tensor_t *scale, const lux3d_tensor_t *scale_base,
+                                   int32_t rms, float eps, const lux3d_tensor_t *x_out,
+                                   const lux3d_tensor_t *y, lux3d_stream_t stream);
+
+/* --------------------------------------------------------------------------
  * VGGT/Pi3 2D RoPE (R1) on Q and K head views, optionally after a per-head
  * affine LayerNorm (the q_norm/k_norm of the attention).
  *   q, k: [B, H, N, D] views with any outer strides (e.g. the permuted
