@@ -1040,6 +1040,114 @@ int lux3d_sdpa(const lux3d_tensor_t *q, const lux3d_tensor_t *k, const lux3d_ten
   return hip_status(launch_attention(q->dtype, p, stream_of(stream)), fn);
 }
 
+namespace {
+// [n, h, L, D] or [h, L, D] operand of the shared-prefix attention: unit inner stride, q's dtype.
+int prefix_operand(const lux3d_tensor_t *t, const char *fn, const char *name, int rank, int dt) {
+  int r = check_desc(t, fn, name);
+  if (r) return r;
+  if (t->rank != rank) return fail(LUX3D_ERR_SHAPE, "%s: `%s` must have rank %d (rank %d given)", fn, name, rank, t->rank);
+  if (t->dtype != dt) return fail(LUX3D_ERR_DTYPE, "%s: `%s` must have q's dtype", fn, name);
+  if (t->shape[rank - 1] > 1 && t->stride[rank - 1] != 1)
+    return fail(LUX3D_ERR_LAYOUT, "%s: `%s` must have a unit innermost stride", fn, name);
+  return LUX3D_OK;
+}
+bool prefix_aligned(const lux3d_tensor_t *t) {
+  if (numel(t) == 0) return true;
+  const int64_t el = 16 / elem_bytes(t->dtype);
+  if (!aligned16(t->data)) return false;
+  for (int a = 0; a < t->rank - 1; ++a)
+    if (t->shape[a] > 1 && t->stride[a] % el) return false;
+  return true;
+}
+// rows of keys do not overlap, and a block of them lies within the 32-bit offsets of one buffer descriptor
+bool prefix_block_fits(const lux3d_tensor_t *t, int64_t D) {
+  const int64_t st = t->stride[t->rank - 2], e = elem_bytes(t->dtype);
+  return t->shape[t->rank - 2] <= 1 || (st >= D && st < (int64_t(1) << 31) / (kPrefixKeys + 1) / e);
+}
+// the stride of a lone row counts for nothing: a descriptor's end must follow from it all the same
+int64_t prefix_row_stride(const lux3d_tensor_t *t, int64_t D) {
+  return t->shape[t->rank - 2] <= 1 ? D : t->stride[t->rank - 2];
+}
+}  // namespace
+
+int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t prefix,
+                                           int64_t own, int64_t head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries <= 0 || prefix < 0 || own < 0 || head_dim <= 0)
+    return 0;
+  const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own);
+  return prefix_workspace(plan, batch, heads, queries, head_dim);
+}
+
+int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *prefix_k, const lux3d_tensor_t *prefix_v,
+                             const lux3d_tensor_t *k, const lux3d_tensor_t *v, const lux3d_tensor_t *lens, int32_t causal,
+                             float scale, const lux3d_tensor_t *workspace, const lux3d_tensor_t *out,
+                             lux3d_stream_t stream) {
+  const char *fn = "lux3d_sdpa_shared_prefix";
+  int r;
+  if ((r = check_desc(q, fn, "q"))) return r;
+  if (!is_float(q->dtype)) return fail(LUX3D_ERR_DTYPE, "%s: `q` must be f32, bf16 or f16", fn);
+  const int dt = q->dtype;
+  if ((r = prefix_operand(q, fn, "q", 4, dt)) || (r = prefix_operand(prefix_k, fn, "prefix_k", 3, dt)) ||
+      (r = prefix_operand(prefix_v, fn, "prefix_v", 3, dt)) || (r = prefix_operand(k, fn, "k", 4, dt)) ||
+      (r = prefix_operand(v, fn, "v", 4, dt)) || (r = prefix_operand(out, fn, "out", 4, dt)))
+    return r;
+  PrefixParams p;
+  p.B = q->shape[0]; p.H = q->shape[1]; p.Lq = q->shape[2]; p.D = q->shape[3];
+  p.Hkv = prefix_k->shape[0]; p.P = prefix_k->shape[1]; p.Ls = k->shape[2];
+  if (p.D < 1 || p.D > 512) return fail(LUX3D_ERR_SHAPE, "%s: head dim %lld outside 1..512", fn, (long long)p.D);
+  if (p.Hkv < 1 ? p.H != 0 : p.H % p.Hkv != 0)
+    return fail(LUX3D_ERR_SHAPE, "%s: %lld query heads are no multiple of %lld key heads", fn, (long long)p.H,
+                (long long)p.Hkv);
+  if (prefix_k->shape[2] != p.D || prefix_v->shape[0] != p.Hkv || prefix_v->shape[1] != p.P || prefix_v->shape[2] != p.D)
+    return fail(LUX3D_ERR_SHAPE, "%s: prefix_k and prefix_v must be [Hkv, P, %lld]", fn, (long long)p.D);
+  for (const lux3d_tensor_t *t : {k, v})
+    if (t->shape[0] != p.B || t->shape[1] != p.Hkv || t->shape[2] != p.Ls || t->shape[3] != p.D)
+      return fail(LUX3D_ERR_SHAPE, "%s: k and v must be [%lld, %lld, Ls, %lld]", fn, (long long)p.B, (long long)p.Hkv,
+                  (long long)p.D);
+  for (int i = 0; i < 4; ++i)
+    if (out->shape[i] != q->shape[i]) return fail(LUX3D_ERR_SHAPE, "%s: out must have the shape of q", fn);
+  if (lens) {
+    if ((r = check_desc(lens, fn, "lens"))) return r;
+    if (lens->dtype != LUX3D_I32) return fail(LUX3D_ERR_DTYPE, "%s: `lens` must be int32", fn);
+    if (lens->rank != 1 || lens->shape[0] != p.B || !is_contiguous(lens))
+      return fail(LUX3D_ERR_SHAPE, "%s: `lens` must be a contiguous [%lld] vector", fn, (long long)p.B);
+    p.lens = reinterpret_cast<const int32_t *>(lens->data);
+  }
+  if (causal != 0 && causal != 1) return fail(LUX3D_ERR_VALUE, "%s: causal must be 0 or 1", fn);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(LUX3D_ERR_VALUE, "%s: scale must be finite and > 0", fn);
+  if (p.B == 0 || p.H == 0 || p.Lq == 0) return ok();
+  p.G = p.H / p.Hkv;
+  if (p.P > INT32_MAX - 256 || p.Ls > INT32_MAX - 256) return fail(LUX3D_ERR_SHAPE, "%s: more than 2^31 keys", fn);
+  if (p.Lq > INT32_MAX / p.B / p.G) return fail(LUX3D_ERR_SHAPE, "%s: more than 2^31 query rows a key head", fn);
+  p.q = q->data; p.pk = prefix_k->data; p.pv = prefix_v->data; p.k = k->data; p.v = v->data; p.o = out->data;
+  p.q_sb = q->stride[0]; p.q_sh = q->stride[1]; p.q_st = q->stride[2];
+  p.pk_sh = prefix_k->stride[0]; p.pk_st = prefix_row_stride(prefix_k, p.D);
+  p.pv_sh = prefix_v->stride[0]; p.pv_st = prefix_row_stride(prefix_v, p.D);
+  p.k_sb = k->stride[0]; p.k_sh = k->stride[1]; p.k_st = prefix_row_stride(k, p.D);
+  p.v_sb = v->stride[0]; p.v_sh = v->stride[1]; p.v_st = prefix_row_stride(v, p.D);
+  p.o_sb = out->stride[0]; p.o_sh = out->stride[1]; p.o_st = out->stride[2];
+  p.causal = causal != 0;
+  p.scale = scale;
+  p.mfma = dt != LUX3D_F32 && (p.D == 64 || p.D == 128) && prefix_aligned(q) && prefix_aligned(prefix_k) &&
+           prefix_aligned(prefix_v) && prefix_aligned(k) && prefix_aligned(v) && prefix_aligned(out) &&
+           prefix_block_fits(prefix_k, p.D) && prefix_block_fits(prefix_v, p.D) && prefix_block_fits(k, p.D) &&
+           prefix_block_fits(v, p.D);
+  if (p.mfma) {
+    p.plan = prefix_plan(p.B, p.H, p.Hkv, p.Lq, p.P, p.Ls);
+    const int64_t need = prefix_workspace(p.plan, p.B, p.H, p.Lq, p.D);
+    if (need > 0) {
+      if ((r = check_desc(workspace, fn, "workspace"))) return r;
+      if (workspace->dtype != LUX3D_F32 || !is_contiguous(workspace) || !aligned16(workspace->data))
+        return fail(LUX3D_ERR_LAYOUT, "%s: `workspace` must be contiguous f32, 16-byte aligned", fn);
+      if (numel(workspace) < need)
+        return fail(LUX3D_ERR_SHAPE, "%s: `workspace` has %lld values, %lld are needed", fn, (long long)numel(workspace),
+                    (long long)need);
+      p.ws = reinterpret_cast<float *>(workspace->data);
+    }
+  }
+  return hip_status(launch_prefix_attention(dt, p, stream_of(stream)), fn);
+}
+
 int lux3d_sdpa_heads_f32(const lux3d_tensor_t *q, const lux3d_tensor_t *k, const lux3d_tensor_t *v, float scale,
                          const lux3d_tensor_t *out, lux3d_stream_t stream) {
   const char *fn = "lux3d_sdpa_heads_f32";

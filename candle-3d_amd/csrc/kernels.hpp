@@ -7,6 +7,8 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
+#include "prefix_plan.hpp"
+
 namespace lux3d {
 
 // ---- row family: LayerNorm / residual+LayerNorm / AdaLN modulate / gate ----
@@ -202,6 +204,30 @@ struct AttnParams {
 };
 enum { QP_NONE = 0, QP_LN_R1 = 1, QP_RMS = 2, QP_L2_R2 = 3, QP_R3 = 4 };
 hipError_t launch_attention(int dt, const AttnParams &p, hipStream_t s);
+
+// Attention of a batch that shares a prefix of keys (prefix_attention.hip):
+// q, o [B, H, Lq, D]; pk, pv [Hkv, P, D]; k, v [B, Hkv, Ls, D], G = H / Hkv;
+// lens [B] (own keys of a sequence, clamped to 0 .. Ls) or null: Ls. `mfma`
+// selects the matrix-core kernels (2-byte types, D 64 or 128, every row
+// 16-byte aligned, block offsets below 2^31 bytes), which follow `plan` and
+// use ws where it has several parts; otherwise the generic kernel.
+struct PrefixParams {
+  const void *q = nullptr, *pk = nullptr, *pv = nullptr, *k = nullptr, *v = nullptr;
+  void *o = nullptr;
+  int64_t B = 0, H = 0, Hkv = 0, G = 1, Lq = 0, P = 0, Ls = 0, D = 0;
+  int64_t q_sb = 0, q_sh = 0, q_st = 0;
+  int64_t pk_sh = 0, pk_st = 0, pv_sh = 0, pv_st = 0;
+  int64_t k_sb = 0, k_sh = 0, k_st = 0;
+  int64_t v_sb = 0, v_sh = 0, v_st = 0;
+  int64_t o_sb = 0, o_sh = 0, o_st = 0;
+  const int32_t *lens = nullptr;
+  bool causal = false;
+  float scale = 0.f;
+  bool mfma = false;
+  PrefixPlan plan;
+  float *ws = nullptr;
+};
+hipError_t launch_prefix_attention(int dt, const PrefixParams &p, hipStream_t s);
 
 // TRELLIS.2 sparse voxel ops.
 // Coordinate hash (cap: a power of two >= 2n) and neighbour table nbr [n, 27].

@@ -46,7 +46,7 @@ class Tensor(ctypes.Structure):
 TP = ctypes.POINTER(Tensor)
 S = ctypes.c_void_p  # lux3d_stream_t
 
-# name -> argtypes (every entry returns int)
+# name -> argtypes (every entry returns int, but those of SIZES)
 SIGNATURES = {
     "lux3d_layer_norm": [TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_residual_layer_norm": [TP, TP, TP, TP, TP, ctypes.c_float, TP, TP, S],
@@ -71,6 +71,8 @@ SIGNATURES = {
     "lux3d_q8_0_linear_int8": [TP, TP, TP, TP, TP, TP, TP, S],
     "lux3d_q8_0_quantize": [TP, TP, TP, S],
     "lux3d_sdpa": [TP, TP, TP, ctypes.c_float, TP, S],
+    "lux3d_sdpa_shared_prefix_workspace": [ctypes.c_int64] * 7,
+    "lux3d_sdpa_shared_prefix": [TP, TP, TP, TP, TP, TP, ctypes.c_int32, ctypes.c_float, TP, TP, S],
     "lux3d_sdpa_heads_f32": [TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_sdpa_layernorm_rope2d": [TP, TP, TP, ctypes.c_float, TP, TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_sdpa_rms_norm_heads": [TP, TP, ctypes.c_float, TP, TP, ctypes.c_float, TP, S],
@@ -86,6 +88,9 @@ SIGNATURES = {
     "lux3d_index_select_rows": [TP, TP, TP, TP, S],
     "lux3d_channel_to_spatial": [TP, TP, TP, TP, TP, TP, TP, TP, TP, S],
 }
+
+# entries that return a size (int64), not a status
+SIZES = ("lux3d_sdpa_shared_prefix_workspace",)
 
 
 class Lux3dError(RuntimeError):
@@ -112,7 +117,7 @@ def _load() -> ctypes.CDLL:
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
-        fn.restype = ctypes.c_int
+        fn.restype = ctypes.c_int64 if name in SIZES else ctypes.c_int
     lib.lux3d_abi_version.restype = ctypes.c_int
     lib.lux3d_abi_version.argtypes = []
     lib.lux3d_last_error.restype = ctypes.c_char_p

@@ -509,6 +509,31 @@ def sdpa(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
     return out
 
 
+def sdpa_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                       v: torch.Tensor, scale: float, *, lens: Optional[torch.Tensor] = None, causal: bool = False,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a batch of sequences behind one shared prefix of keys: q
+    [B, H, Lq, D]; prefix_k / prefix_v [Hkv, P, D], stored and read once for
+    all; k / v [B, Hkv, Ls, D] the sequences' own, of which the first lens[b]
+    (int32 [B]; default Ls) count. causal: a sequence's last Lq own keys are
+    its queries' own, and query i sees them up to its own. A query that sees no
+    key gives zeros. The workspace is allocated here."""
+    fn = "lux3d_sdpa_shared_prefix"
+    _one_device(fn, q, prefix_k, prefix_v, k, v, lens, out)
+    if q.dim() != 4 or prefix_k.dim() != 3 or k.dim() != 4:
+        raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "q and k must be [B, H, L, D], the prefix [Hkv, P, D]")
+    with _device_of(q):
+        if out is None:
+            out = _new(q)
+        b, h, n, d = q.shape
+        hkv, p, _ = prefix_k.shape
+        size = _lib.LIB.lux3d_sdpa_shared_prefix_workspace(b, h, hkv, n, p, k.shape[2], d)
+        ws = torch.empty(size, dtype=torch.float32, device=q.device) if size else None
+        _lib.call(fn, _d(q), _d(prefix_k), _d(prefix_v), _d(k), _d(v), _d(lens), 1 if causal else 0, float(scale), _d(ws),
+                  _d(out), _stream(q))
+    return out
+
+
 def sdpa_layernorm_rope2d(q_raw: torch.Tensor, q_norm, embeddings: "RopeEmbeddings", k: torch.Tensor,
                           v: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """exact_query_chunked_sdpa(apply_layernorm_rope(q_raw, q_norm, rope), k, v,

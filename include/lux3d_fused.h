@@ -535,6 +535,39 @@ int lux3d_sdpa(const lux3d_tensor_t *q, const lux3d_tensor_t *k,
                const lux3d_tensor_t *v, float scale, const lux3d_tensor_t *out,
                lux3d_stream_t stream);
 
+/* lux3d_sdpa_shared_prefix: attention of a batch whose sequences share one long
+ * prefix of keys, which is stored and read once for all of them:
+ *   out[b, h, i] = softmax over the P prefix keys and the own keys j < n(b, i)
+ *                  of (q . key * scale), times the values
+ *   n(b, i) = len_b, or with causal = 1 len_b - Lq + i + 1 (the sequence's last
+ *   Lq own keys are the queries' own; values below 0 count as 0).
+ *   q, out: [B, H, Lq, D]; prefix_k, prefix_v: [Hkv, P, D]; k, v: [B, Hkv, Ls,
+ *   D], the sequences' own (a cache that fills from the front); H a multiple of
+ *   Hkv, query head h uses key head h / (H / Hkv). One dtype (f32, bf16 or f16);
+ *   any outer strides, unit innermost stride; P and Ls may be 0; D <= 512.
+ *   lens: int32 [B] on the device, len_b = lens[b] clamped to 0 .. Ls; NULL: Ls.
+ *   A query that sees no key gives zeros. Own keys at or past len_b are never
+ *   read.
+ *   workspace: contiguous f32, 16-byte aligned, of at least
+ *   lux3d_sdpa_shared_prefix_workspace(B, H, Hkv, Lq, P, Ls, D) values (0: may
+ *   be NULL); its contents do not matter and it holds nothing between calls, but
+ *   no two calls that may overlap share one.
+ * D = 64 or 128 of a 2-byte type with every row 16-byte aligned runs on the
+ * matrix cores (f32 scores, softmax and sums, probabilities rounded to the type,
+ * one rounding of the output, as lux3d_sdpa); other cases run a generic kernel in
+ * f32 throughout. One or two kernels. out must not overlap an input. The
+ * reference attends to one sequence a call (exact_query_chunked_sdpa,
+ * runtime/attention_math.rs:199-241, without a cache): this is the form of
+ * several samples or frames behind one context.                             */
+int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t kv_heads,
+                                           int64_t queries, int64_t prefix, int64_t own,
+                                           int64_t head_dim);
+int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *prefix_k,
+                             const lux3d_tensor_t *prefix_v, const lux3d_tensor_t *k,
+                             const lux3d_tensor_t *v, const lux3d_tensor_t *lens, int32_t causal,
+                             float scale, const lux3d_tensor_t *workspace,
+                             const lux3d_tensor_t *out, lux3d_stream_t stream);
+
 /* lux3d_sdpa_heads_f32: exact_sdpa_heads (attention_math.rs:244-259), which
  * widens q, k and v to f32, computes scores, softmax and P v in f32 and
  * narrows the result to the input dtype. Arguments as lux3d_sdpa, except that
