@@ -901,9 +901,10 @@ int lux3d_q8_0_repack(const lux3d_tensor_t *blocks, int64_t n, int64_t k, const 
                     fn);
 }
 
-int lux3d_q8_0_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *qs, const lux3d_tensor_t *scales,
-                      const lux3d_tensor_t *bias, const lux3d_tensor_t *y, lux3d_stream_t stream) {
-  const char *fn = "lux3d_q8_0_linear";
+namespace {
+// The arguments of a Q8_0 linear, checked, in p.
+int q8_linear_params(const char *fn, const lux3d_tensor_t *x, const lux3d_tensor_t *qs, const lux3d_tensor_t *scales,
+                     const lux3d_tensor_t *bias, const lux3d_tensor_t *y, Q8GemmParams &p) {
   int r;
   RowView xv, yv;
   if ((r = row_tensor(x, fn, "x", -1, xv))) return r;
@@ -934,13 +935,89 @@ int lux3d_q8_0_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *qs, const l
     return fail(LUX3D_ERR_LAYOUT, "%s: x rows and qs must be 16-byte aligned", fn);
   if (xf32 && (xv.rs > (int64_t(1) << 20) || k > (int64_t(1) << 22)))
     return fail(LUX3D_ERR_SHAPE, "%s: f32 x rows of more than 2^20 elements are not supported", fn);
-  Q8GemmParams p;
   p.x = xv.p; p.ldx = xv.rs; p.x_f32 = xf32;
   p.qs = reinterpret_cast<const int8_t *>(qs->data);
   p.scales = reinterpret_cast<const float *>(scales->data);
   p.bias = bp;
   p.y = const_cast<void *>(yv.p); p.ldy = yv.rs;
   p.M = xv.rows; p.N = n; p.K = k;
+  return LUX3D_OK;
+}
+}  // namespace
+
+int lux3d_q8_0_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *qs, const lux3d_tensor_t *scales,
+                      const lux3d_tensor_t *bias, const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_q8_0_linear";
+  Q8GemmParams p;
+  if (int r = q8_linear_params(fn, x, qs, scales, bias, y, p)) return r;
+  return hip_status(launch_q8_0_gemm(y->dtype, p, stream_of(stream)), fn);
+}
+
+int lux3d_q8_0_linear_adapters(const lux3d_tensor_t *x, const lux3d_tensor_t *qs, const lux3d_tensor_t *scales,
+                               const lux3d_tensor_t *bias, const lux3d_tensor_t *a, const lux3d_tensor_t *b,
+                               const lux3d_tensor_t *alphas, const lux3d_tensor_t *adapter_ids,
+                               const lux3d_tensor_t *seg_offsets, const lux3d_tensor_t *t, const lux3d_tensor_t *bad_ids,
+                               const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_q8_0_linear_adapters";
+  Q8GemmParams p;
+  int r;
+  if ((r = q8_linear_params(fn, x, qs, scales, bias, y, p))) return r;
+  if ((r = check_desc(a, fn, "a")) || (r = check_desc(b, fn, "b")) || (r = check_desc(adapter_ids, fn, "adapter_ids")) ||
+      (r = check_desc(t, fn, "t")))
+    return r;
+  if (a->dtype != x->dtype || b->dtype != x->dtype || t->dtype != x->dtype)
+    return fail(LUX3D_ERR_DTYPE, "%s: `a`, `b` and `t` must have x's dtype", fn);
+  if (a->rank != 3 || a->shape[2] != p.K || a->shape[0] < 1 || a->shape[1] < 1)
+    return fail(LUX3D_ERR_SHAPE, "%s: `a` must be [adapters, rank, %lld], with one adapter and a rank of 1 at least", fn,
+                (long long)p.K);
+  const int64_t na = a->shape[0], rank = a->shape[1];
+  if (na > INT32_MAX || rank > 1024) return fail(LUX3D_ERR_SHAPE, "%s: rank %lld above 1024, or too many adapters", fn, (long long)rank);
+  if (b->rank != 3 || b->shape[0] != na || b->shape[1] != p.N || b->shape[2] != rank)
+    return fail(LUX3D_ERR_SHAPE, "%s: `b` must be [%lld, %lld, %lld]", fn, (long long)na, (long long)p.N, (long long)rank);
+  if (!is_contiguous(a) || !is_contiguous(b) || !is_contiguous(t) || !aligned16(a->data) || !aligned16(t->data))
+    return fail(LUX3D_ERR_LAYOUT, "%s: `a`, `b` and `t` must be contiguous, `a` and `t` 16-byte aligned", fn);
+  AdapterParams &d = p.ad;
+  d.tp = (int)((rank + 15) / 16 * 16);
+  if (numel(t) / d.tp < p.M)
+    return fail(LUX3D_ERR_SHAPE, "%s: `t` has %lld values, rows times the rank rounded up to 16 are needed: %lld", fn,
+                (long long)numel(t), (long long)(p.M * d.tp));
+  if (adapter_ids->dtype != LUX3D_I32) return fail(LUX3D_ERR_DTYPE, "%s: `adapter_ids` must be int32", fn);
+  if (adapter_ids->rank != 1 || adapter_ids->shape[0] < 1 || !is_contiguous(adapter_ids))
+    return fail(LUX3D_ERR_SHAPE, "%s: `adapter_ids` must be a contiguous [S] vector, S >= 1", fn);
+  if (alphas) {
+    if ((r = check_desc(alphas, fn, "alphas"))) return r;
+    if (alphas->dtype != LUX3D_F32) return fail(LUX3D_ERR_DTYPE, "%s: `alphas` must be f32", fn);
+    if (alphas->rank != 1 || alphas->shape[0] != na || !is_contiguous(alphas))
+      return fail(LUX3D_ERR_SHAPE, "%s: `alphas` must be a contiguous [%lld] vector", fn, (long long)na);
+    d.alpha = reinterpret_cast<const float *>(alphas->data);
+  }
+  AdapterDownParams dp;
+  if (bad_ids) {
+    if ((r = check_desc(bad_ids, fn, "bad_ids"))) return r;
+    if (bad_ids->dtype != LUX3D_I32 || numel(bad_ids) != 1)
+      return fail(LUX3D_ERR_SHAPE, "%s: `bad_ids` must be one int32", fn);
+    dp.bad = reinterpret_cast<int32_t *>(bad_ids->data);
+  }
+  d.nseg = adapter_ids->shape[0];
+  if (seg_offsets) {
+    if ((r = check_desc(seg_offsets, fn, "seg_offsets"))) return r;
+    if (seg_offsets->dtype != LUX3D_I64) return fail(LUX3D_ERR_DTYPE, "%s: `seg_offsets` must be int64", fn);
+    if (seg_offsets->rank != 1 || seg_offsets->shape[0] != d.nseg + 1 || !is_contiguous(seg_offsets))
+      return fail(LUX3D_ERR_SHAPE, "%s: `seg_offsets` must be a contiguous [%lld] vector", fn, (long long)(d.nseg + 1));
+    d.seg_off = reinterpret_cast<const int64_t *>(seg_offsets->data);
+  } else if (p.M % d.nseg) {
+    return fail(LUX3D_ERR_SHAPE, "%s: %lld rows do not split into %lld equal segments (pass seg_offsets)", fn,
+                (long long)p.M, (long long)d.nseg);
+  }
+  d.rows_per_seg = p.M / d.nseg > 0 ? p.M / d.nseg : 1;
+  d.a = a->data; d.b = b->data; d.t = t->data;
+  d.ids = reinterpret_cast<const int32_t *>(adapter_ids->data);
+  d.n = (int)na; d.r = (int)rank;
+  d.b_vec = aligned16(b->data) && rank * elem_bytes(b->dtype) % 16 == 0;
+  dp.ad = d;
+  dp.x = p.x; dp.ldx = p.ldx; dp.M = p.M; dp.K = p.K;
+  if (p.M == 0 || p.N == 0) return ok();
+  if (hipError_t e = launch_adapter_down(dp, p.x_f32, stream_of(stream))) return hip_status(e, fn);
   return hip_status(launch_q8_0_gemm(y->dtype, p, stream_of(stream)), fn);
 }
 

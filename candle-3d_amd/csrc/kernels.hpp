@@ -127,6 +127,28 @@ hipError_t launch_timestep(const float *t, int64_t n, const float *freqs, int64_
 hipError_t launch_dequant_q8_0(const uint8_t *blocks, int64_t nblocks, int out_dt, void *y,
                                bool vec, hipStream_t s);
 
+// ---- low-rank adapters beside a linear (adapters.hip, adapters.hpp) -------------
+// Rows of segment s take adapter ids[s] (none outside 0 .. n - 1): y += t B^T, t
+// = alpha x A^T, in x's type. a [n, r, K], b [n, N, r], t [M, tp], tp = r
+// rounded up to 16; b_vec: B's rows are 16-byte aligned.
+struct AdapterParams {
+  const void *a = nullptr, *b = nullptr;
+  const float *alpha = nullptr;      // [n] or null
+  const int32_t *ids = nullptr;      // [nseg]
+  const int64_t *seg_off = nullptr;  // [nseg + 1] or null: equal segments
+  int64_t nseg = 0, rows_per_seg = 1;
+  int n = 0, r = 0, tp = 0;
+  bool b_vec = false;
+  void *t = nullptr;
+};
+struct AdapterDownParams {
+  AdapterParams ad;
+  const void *x = nullptr; int64_t ldx = 0;
+  int64_t M = 0, K = 0;
+  int32_t *bad = nullptr;            // [1] or null: segments with an id that is no adapter's and not -1
+};
+hipError_t launch_adapter_down(const AdapterDownParams &p, bool x_f32, hipStream_t s);
+
 // ---- Q8_0 quantized linear ---------------------------------------------------
 // y[m, n] = sum_k x[m, k] * bf16(q[n, k] * scale[n, k / 32]) (+ bias[n]).
 struct Q8GemmParams {
@@ -137,6 +159,7 @@ struct Q8GemmParams {
   const float *bias = nullptr;                // [N] or null
   void *y = nullptr; int64_t ldy = 0;         // [M, N] rows
   int64_t M = 0, N = 0, K = 0;
+  AdapterParams ad;                           // ad.n > 0: adapters, their t already formed
 };
 hipError_t launch_q8_0_repack(const uint8_t *blocks, int64_t nblocks, int8_t *qs, float *scales, hipStream_t s);
 hipError_t launch_q8_0_gemm(int out_dt, const Q8GemmParams &p, hipStream_t s);

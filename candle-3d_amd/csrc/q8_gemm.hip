@@ -31,6 +31,7 @@
 // Within a k-step the kernels assign k to MFMA sub-steps differently, so
 // their outputs can differ in the last bit of the f32 sum; each is
 // deterministic.
+#include "adapters.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
 #include "q8_tiles.hpp"
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(256) void q8_0_repack_kernel(const uint8_t *blocks,
 // wavefronts form a 2 x 2 grid, each owning (BM/2) x (BN/2) = TM x TN MFMA
 // tiles of 32 x 32. MINW is the minimum number of wavefronts per SIMD the
 // register allocation must allow.
-template <typename OUT, int BM, int BN, int BK, int MINW>
+template <typename OUT, int BM, int BN, int BK, int MINW, bool AD>
 __global__ __launch_bounds__(kGemmThreads, MINW) void q8_0_gemm_kernel(Q8GemmParams p) {
   constexpr int TM = BM / 64, TN = BN / 64;
   constexpr int LDS_ROW = BK + 8;                    // bf16 per LDS row (odd multiple of 16 bytes)
@@ -176,6 +177,8 @@ __global__ __launch_bounds__(kGemmThreads, MINW) void q8_0_gemm_kernel(Q8GemmPar
     lds_barrier();
   }
 
+  if constexpr (AD) adapter_add<false, TM, TN>(p.ad, p.M, p.N, m0 + wm * (BM / 2), n0 + wn * (BN / 2), acc);
+
   // epilogue: lane holds C[8*(e/4) + 4*(lane/32) + e%4][lane%32] of each tile
   char *ybase = reinterpret_cast<char *>(p.y);
 #pragma unroll
@@ -252,7 +255,7 @@ __device__ __forceinline__ bf16x8_t dequant8(uint32_t lo, uint32_t hi, float d) 
 // XCDs; they are renumbered so that each XCD takes a contiguous range, walked
 // in groups of GM row tiles (columns fastest within a group), so the tiles
 // running on one XCD share x rows and weight columns in its L2.
-template <typename OUT, int GM, int BM, int NW = 8>
+template <typename OUT, int GM, int BM, int NW, bool AD>
 __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams p, int tiles_m, int tiles_n) {
   // NW wavefronts, each owning 32 columns: BN = 32 NW (256 or 128); BM a multiple of 32 up to 256
   constexpr int BN = 32 * NW, BK = 64, TM = BM / 32, NS = kRingStages;
@@ -328,12 +331,12 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
 #pragma unroll
     for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const bf16x8_t *>(st + fbase[s] + i * 4096);
   };
-  f32x16_t acc[TM];
+  f32x16_t acc[TM][1];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) acc[i] = f32x16_t{};
+  for (int i = 0; i < TM; ++i) acc[i][0] = f32x16_t{};
   auto mfmas = [&](const bf16x8_t (&a)[TM], bf16x8_t b) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b, acc[i], 0, 0, 0);
+    for (int i = 0; i < TM; ++i) acc[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b, acc[i][0], 0, 0, 0);
   };
 
   // Prologue: stages 0 .. NS-2. The loop body is branch-free: past the last
@@ -378,6 +381,7 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
     __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads and reads
+  if constexpr (AD) adapter_add<false, TM, 1>(p.ad, p.M, p.N, m0, c0 + wave * 32, acc);
 
   char *ybase = reinterpret_cast<char *>(p.y);
   const float bias = (p.bias && ncol < p.N) ? p.bias[ncol] : 0.f;
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int r = ii * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-          const float v = acc[pass * (RP / 32) + ii][e] + bias;
+          const float v = acc[pass * (RP / 32) + ii][0][e] + bias;
           if constexpr (EB == 4) *reinterpret_cast<float *>(reg + r * LROW + lrow * 4) = v;
           else if constexpr (OUT::code == LUX3D_BF16)
             *reinterpret_cast<uint16_t *>(reg + r * LROW + lrow * 2) = (uint16_t)(pack_bf16x2(v, 0.f) & 0xFFFFu);
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
       for (int e = 0; e < 16; ++e) {
         const int64_t row = m0 + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
         if (row >= p.M) continue;
-        store1<OUT>(ybase, row * p.ldy + ncol, acc[i][e] + bias);
+        store1<OUT>(ybase, row * p.ldy + ncol, acc[i][0][e] + bias);
       }
   }
 }
@@ -486,7 +490,7 @@ struct X3Tile {
   static_assert(BM % (8 * NW) == 0 && BN % (32 * NW) == 0, "whole segments per wavefront");
 };
 
-template <typename OUT, int GM, int WM, int WN, int TI, int TJ, int KG>
+template <typename OUT, int GM, int WM, int WN, int TI, int TJ, int KG, bool AD>
 __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8GemmParams p, int tiles_m, int tiles_n) {
   using T = X3Tile<WM, WN, TI, TJ>;
   constexpr int BM = T::BM, BN = T::BN, BK = 32, NS = kX3Stages;
@@ -666,6 +670,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8Ge
     __syncthreads();
     if (kg > 0) return;
   }
+  if constexpr (AD) adapter_add<true, TI, TJ>(p.ad, p.M, p.N, m0 + wm * TI * 32, c0 + wn * TJ * 32, acc);
 
   // epilogue: each wavefront's 32 TI x 32 TJ block through LDS, bias added, one
   // rounding, 16-byte row pieces
@@ -752,7 +757,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8Ge
 // does. Before / after, us: M 2, K 1536 -> N 9216 16.9 / 8.0 in bf16 (16 MB of
 // weights: 3.1 us at the copy rate) and 71 / 10.8 in f32; M 64, K 8192 -> N
 // 2048 68 / 38 and 363 / 69.
-template <typename OUT, bool XF32, int NW, int MT>
+template <typename OUT, bool XF32, int NW, int MT, bool AD>
 __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_kernel(Q8GemmParams p) {
   typedef float f32x4_t __attribute__((ext_vector_type(4)));
   constexpr int U = MT == 1 ? (XF32 ? 4 : 8) : 2;  // chunks per turn
@@ -855,42 +860,43 @@ __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_kernel(Q8GemmParams p) 
     float v = part[0][o];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += part[w][o];
+    if constexpr (AD) v += adapter_dot<XF32>(p.ad, p.N, row, col);
     store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
   }
 }
 
-template <typename OUT, bool XF32, int MT>
+template <typename OUT, bool XF32, int MT, bool AD>
 hipError_t launch_few_rows(const Q8GemmParams &p, hipStream_t s) {
   // 2048 wavefronts (two per SIMD), or as many as k has chunk pairs
   const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * MT - 1) / (16 * MT);
   if (tn > INT32_MAX || tm > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tn, (unsigned)tm);
   if (tn * tm * 4 >= 2048 || p.K <= 512)
-    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 4, MT>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 4, MT, AD>), grid, dim3(256), 0, s, p);
   else if (tn * tm * 8 >= 2048 || p.K <= 1024)
-    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 8, MT>), grid, dim3(512), 0, s, p);
+    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 8, MT, AD>), grid, dim3(512), 0, s, p);
   else
-    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 16, MT>), grid, dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, 16, MT, AD>), grid, dim3(1024), 0, s, p);
   return hipGetLastError();
 }
 
-template <typename OUT, int WM, int WN, int TI, int TJ, int KG>
+template <typename OUT, bool AD, int WM, int WN, int TI, int TJ, int KG>
 hipError_t launch_x3(const Q8GemmParams &p, hipStream_t s) {
   using T = X3Tile<WM, WN, TI, TJ>;
   const int64_t tiles_m = (p.M + T::BM - 1) / T::BM, tiles_n = (p.N + T::BN - 1) / T::BN;
   if (tiles_m * tiles_n > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((q8_0_gemm_x3_kernel<OUT, 8, WM, WN, TI, TJ, KG>), dim3((unsigned)(tiles_m * tiles_n)),
+  hipLaunchKernelGGL((q8_0_gemm_x3_kernel<OUT, 8, WM, WN, TI, TJ, KG, AD>), dim3((unsigned)(tiles_m * tiles_n)),
                      dim3(64 * T::NW * KG), 0, s, p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
-template <typename OUT>
+template <typename OUT, bool AD>
 hipError_t launch_f32(const Q8GemmParams &p, hipStream_t s) {
   const Q8Tile tile = q8_tile_f32(p.M, p.N, p.K);
-  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, true, 1>(p, s) : launch_few_rows<OUT, true, 4>(p, s);
-  if (tile.rows == 128) return launch_x3<OUT, 2, 4, 2, 2, 1>(p, s);
-  if (tile.rows == 32) return launch_x3<OUT, 1, 4, 1, 1, 3>(p, s);
-  return tile.groups == 1 ? launch_x3<OUT, 2, 2, 1, 2, 1>(p, s) : launch_x3<OUT, 2, 2, 1, 2, 2>(p, s);
+  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, true, 1, AD>(p, s) : launch_few_rows<OUT, true, 4, AD>(p, s);
+  if (tile.rows == 128) return launch_x3<OUT, AD, 2, 4, 2, 2, 1>(p, s);
+  if (tile.rows == 32) return launch_x3<OUT, AD, 1, 4, 1, 1, 3>(p, s);
+  return tile.groups == 1 ? launch_x3<OUT, AD, 2, 2, 1, 2, 1>(p, s) : launch_x3<OUT, AD, 2, 2, 1, 2, 2>(p, s);
 }
 
 // The ring kernel's buffer descriptors span one tile (at most 256 rows of x,
@@ -902,35 +908,35 @@ bool ring_fits(const Q8GemmParams &p) {
          (p.M + 127) / 128 * ((p.N + 255) / 256) <= INT32_MAX;
 }
 
-template <typename OUT, int BM, int NW>
+template <typename OUT, bool AD, int BM, int NW>
 hipError_t launch_ring(const Q8GemmParams &p, hipStream_t s) {
   const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + 32 * NW - 1) / (32 * NW);
   if (tiles_m * tiles_n > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((q8_0_gemm_ring_kernel<OUT, 8, BM, NW>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * NW), 0, s,
+  hipLaunchKernelGGL((q8_0_gemm_ring_kernel<OUT, 8, BM, NW, AD>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * NW), 0, s,
                      p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
-template <typename OUT>
+template <typename OUT, bool AD>
 hipError_t launch_bf16(const Q8GemmParams &p, hipStream_t s) {
   const Q8Tile tile = q8_tile_bf16(p.M, p.N, p.K);
-  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, false, 1>(p, s) : launch_few_rows<OUT, false, 4>(p, s);
-  if (tile.cols == 256) return tile.rows == 256 ? launch_ring<OUT, 256, 8>(p, s) : launch_ring<OUT, 128, 8>(p, s);
+  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, false, 1, AD>(p, s) : launch_few_rows<OUT, false, 4, AD>(p, s);
+  if (tile.cols == 256) return tile.rows == 256 ? launch_ring<OUT, AD, 256, 8>(p, s) : launch_ring<OUT, AD, 128, 8>(p, s);
   switch (tile.rows) {
-    case 32: return launch_ring<OUT, 32, 4>(p, s);
-    case 64: return launch_ring<OUT, 64, 4>(p, s);
-    case 128: return launch_ring<OUT, 128, 4>(p, s);
+    case 32: return launch_ring<OUT, AD, 32, 4>(p, s);
+    case 64: return launch_ring<OUT, AD, 64, 4>(p, s);
+    case 128: return launch_ring<OUT, AD, 128, 4>(p, s);
   }
-  return launch_ring<OUT, 160, 4>(p, s);
+  return launch_ring<OUT, AD, 160, 4>(p, s);
 }
 
-template <typename OUT>
+template <typename OUT, bool AD>
 hipError_t launch_tiles(const Q8GemmParams &p, hipStream_t s) {
-  if (p.x_f32) return launch_f32<OUT>(p, s);  // K % 64 == 0, checked by the caller
-  if (ring_fits(p)) return launch_bf16<OUT>(p, s);
+  if (p.x_f32) return launch_f32<OUT, AD>(p, s);  // K % 64 == 0, checked by the caller
+  if (ring_fits(p)) return launch_bf16<OUT, AD>(p, s);
   // K % 64 == 32, or rows too far apart for the ring's offsets
   const dim3 grid((unsigned)((p.N + 127) / 128), (unsigned)((p.M + 127) / 128));
-  hipLaunchKernelGGL((q8_0_gemm_kernel<OUT, 128, 128, 32, 1>), grid, dim3(kGemmThreads), 0, s, p);
+  hipLaunchKernelGGL((q8_0_gemm_kernel<OUT, 128, 128, 32, 1, AD>), grid, dim3(kGemmThreads), 0, s, p);
   return hipGetLastError();
 }
 
@@ -1110,9 +1116,9 @@ hipError_t launch_q8_0_gemm(int out_dt, const Q8GemmParams &p, hipStream_t s) {
     return hipErrorInvalidValue;
   if ((p.N + 127) / 128 > INT32_MAX || (p.M + 127) / 128 > 65535) return hipErrorInvalidValue;
   switch (out_dt) {
-    case LUX3D_BF16: return launch_tiles<BF16>(p, s);
-    case LUX3D_F16: return launch_tiles<F16>(p, s);
-    case LUX3D_F32: return launch_tiles<F32>(p, s);
+    case LUX3D_BF16: return p.ad.n > 0 ? launch_tiles<BF16, true>(p, s) : launch_tiles<BF16, false>(p, s);
+    case LUX3D_F16: return p.ad.n > 0 ? launch_tiles<F16, true>(p, s) : launch_tiles<F16, false>(p, s);
+    case LUX3D_F32: return p.ad.n > 0 ? launch_tiles<F32, true>(p, s) : launch_tiles<F32, false>(p, s);
   }
   return hipErrorInvalidValue;
 }

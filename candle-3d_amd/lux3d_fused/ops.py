@@ -447,6 +447,27 @@ def q8_0_linear(x: torch.Tensor, qs: torch.Tensor, scales: torch.Tensor, bias: O
     return y
 
 
+def q8_0_linear_adapters(x: torch.Tensor, qs: torch.Tensor, scales: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                         adapter_ids: torch.Tensor, *, alphas: Optional[torch.Tensor] = None,
+                         seg_offsets: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                         out_dtype=torch.bfloat16, bad_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q8_0_linear with low-rank adapters of many requests beside the shared
+    weight: rows of segment s (seg_offsets int64 [S + 1], or S equal segments)
+    add alphas[e] * (x @ a[e]^T) @ b[e]^T, e = adapter_ids[s] (int32 [S], -1:
+    none); a [adapters, rank, k], b [adapters, n, rank] in x's dtype. `bad_ids`
+    (int32 [1]) receives the number of segments with any other id."""
+    fn = "lux3d_q8_0_linear_adapters"
+    _one_device(fn, x, qs, scales, a, b, adapter_ids, alphas, seg_offsets, bias, bad_ids)
+    if a.dim() != 3 or x.dim() < 1 or x.shape[-1] == 0:
+        raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "a must be [adapters, rank, k], x [..., k]")
+    with _device_of(x):
+        y = torch.empty(tuple(x.shape[:-1]) + (qs.shape[0],), dtype=out_dtype, device=x.device)
+        t = torch.empty((x.numel() // x.shape[-1], (a.shape[1] + 15) // 16 * 16), dtype=x.dtype, device=x.device)
+        _lib.call(fn, _d(x), _d(qs), _d(scales), _d(bias), _d(a), _d(b), _d(alphas), _d(adapter_ids), _d(seg_offsets),
+                  _d(t), _d(bad_ids), _d(y), _stream(x))
+    return y
+
+
 def q8_0_quantize(x: torch.Tensor):
     """BlockQ8_0::from_float of f32 x [..., k] rows (candle-core
     k_quants.rs, the first step of candle's CPU QMatMul): -> (xq int8
@@ -495,6 +516,10 @@ class QMatMul:
 
     def forward(self, xs: torch.Tensor, bias: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16):
         return q8_0_linear(xs, self.qs, self.scales, bias, out_dtype)
+
+    def forward_adapters(self, xs: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor, **kw):
+        """forward with low-rank adapters beside the weight (q8_0_linear_adapters)."""
+        return q8_0_linear_adapters(xs, self.qs, self.scales, a, b, adapter_ids, **kw)
 
 
 def sdpa(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,

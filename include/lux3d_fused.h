@@ -376,6 +376,35 @@ int lux3d_q8_0_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *qs,
                       const lux3d_tensor_t *scales, const lux3d_tensor_t *bias,
                       const lux3d_tensor_t *y, lux3d_stream_t stream);
 
+/* lux3d_q8_0_linear_adapters: the same linear with low-rank adapters of many
+ * requests beside the shared weight: row m of segment s, whose adapter is e =
+ * adapter_ids[s],
+ *   y[m] = x[m] W^T (+ bias) + alphas[e] * (x[m] A_e^T) B_e^T
+ *   x, qs, scales, bias, y: as lux3d_q8_0_linear;
+ *   a: [adapters, rank, k], b: [adapters, n, rank], x's dtype, contiguous, a
+ *      16-byte aligned; rank 1 to 1024 (adapters of lower rank are padded with
+ *      zero rows of A); alphas: f32 [adapters] or NULL (1);
+ *   adapter_ids: int32 [S] on the device; -1: the weight alone. Any other id
+ *      outside 0 .. adapters - 1 counts as -1 and into bad_ids (int32 [1] or
+ *      NULL: set to the number of such segments);
+ *   seg_offsets: int64 [S + 1], ascending, or NULL: S equal segments, as in
+ *      lux3d_adaln_modulate (rows before the first offset are segment 0's, rows
+ *      from the last one on segment S - 1's; segments may be empty);
+ *   t: a workspace of x's dtype, contiguous and 16-byte aligned, of at least rows *
+ *      (rank rounded up to 16) values; it holds nothing between calls, and no
+ *      two calls that may overlap share one.
+ * alphas[e] * (x A^T) is summed in f32 and rounded once to x's dtype (f32: not
+ * rounded further); its product with B^T joins the linear's f32 sum, and y is
+ * rounded once. Two kernels. The reference merges no adapters: this is the form
+ * of one quantized model that serves several fine-tunes at once.             */
+int lux3d_q8_0_linear_adapters(const lux3d_tensor_t *x, const lux3d_tensor_t *qs,
+                               const lux3d_tensor_t *scales, const lux3d_tensor_t *bias,
+                               const lux3d_tensor_t *a, const lux3d_tensor_t *b,
+                               const lux3d_tensor_t *alphas, const lux3d_tensor_t *adapter_ids,
+                               const lux3d_tensor_t *seg_offsets, const lux3d_tensor_t *t,
+                               const lux3d_tensor_t *bad_ids, const lux3d_tensor_t *y,
+                               lux3d_stream_t stream);
+
 /* lux3d_q8_0_linear_int8: the same Linear::forward Quant branch with
  * candle's CPU arithmetic (QMatMul::forward on the CPU: the QTensor custom
  * op over upstream candle-core's k_quants::matmul), bit for bit: each f32 x
