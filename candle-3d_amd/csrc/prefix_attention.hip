@@ -46,14 +46,30 @@ struct PrefixItem {
   int64_t part;
 };
 
-__device__ __forceinline__ PrefixItem prefix_item(const PrefixParams &p, int64_t lid, int tile) {
+// `first`: joint items and prefix items, else own items (lid counts each kind from 0)
+__device__ __forceinline__ PrefixItem prefix_item(const PrefixParams &p, int64_t lid, bool first) {
   const PrefixPlan &s = p.plan;
-  const int64_t R = p.Lq * p.G, run = s.run * kPrefixKeys;
+  const int64_t R = p.Lq * p.G;
+  uint32_t x = (uint32_t)lid;
   PrefixItem w;
-  w.p0 = w.p1 = w.o0 = w.o1 = 0;
+  w.p0 = w.p1 = w.o0 = w.o1 = w.b = 0;
+  int tile = s.tile;
+  if (first && !s.joint) {
+    // tiles innermost: those that share keys run side by side
+    const uint32_t tiles = (uint32_t)s.prefix_tiles, runs = (uint32_t)s.prefix_runs;
+    const uint32_t t = x % tiles;
+    x /= tiles;
+    w.part = x % runs;
+    w.kv = x / runs;
+    w.r0 = (int64_t)t * tile;
+    w.rlim = p.B * R;
+    const int64_t run = s.prefix_run * kPrefixKeys;
+    w.p0 = w.part * run;
+    w.p1 = w.p0 + run < p.P ? w.p0 + run : p.P;
+    return w;
+  }
   if (s.joint) {
     // key heads outermost: the tiles of one XCD share a key head's prefix in its L2
-    uint32_t x = (uint32_t)lid;
     const uint32_t tiles = (uint32_t)s.own_tiles, B = (uint32_t)p.B, runs = (uint32_t)s.own_runs;
     const uint32_t t = x % tiles;
     x /= tiles;
@@ -62,31 +78,15 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixParams &p, int64_t
     w.part = x % runs;
     w.kv = x / runs;
     w.r0 = w.b * R + (int64_t)t * tile;
-    w.rlim = (w.b + 1) * R;
     // blocks of the prefix, then of the own keys, in runs
     const int64_t pb = (p.P + kPrefixKeys - 1) / kPrefixKeys;
-    const int64_t j0 = w.part * s.run, j1 = j0 + s.run;
+    const int64_t j0 = w.part * s.own_run, j1 = j0 + s.own_run;
     w.p0 = j0 * kPrefixKeys;
     w.p1 = j1 * kPrefixKeys < p.P ? j1 * kPrefixKeys : p.P;
     w.o0 = j0 > pb ? (j0 - pb) * kPrefixKeys : 0;
     w.o1 = j1 > pb ? (j1 - pb) * kPrefixKeys : 0;
   } else {
-    const uint32_t np = (uint32_t)(p.Hkv * s.prefix_tiles * s.prefix_runs);
-    uint32_t x = (uint32_t)lid;
-    if (x < np) {
-      const uint32_t tiles = (uint32_t)s.prefix_tiles, runs = (uint32_t)s.prefix_runs;
-      const uint32_t t = x % tiles;
-      x /= tiles;
-      w.part = x % runs;
-      w.kv = x / runs;
-      w.r0 = (int64_t)t * tile;
-      w.rlim = p.B * R;
-      w.b = 0;
-      w.p0 = w.part * run;
-      w.p1 = w.p0 + run < p.P ? w.p0 + run : p.P;
-      return w;
-    }
-    x -= np;
+    tile = s.own_tile;
     const uint32_t tiles = (uint32_t)s.own_tiles, runs = (uint32_t)s.own_runs, hkv = (uint32_t)p.Hkv;
     const uint32_t t = x % tiles;
     x /= tiles;
@@ -96,10 +96,10 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixParams &p, int64_t
     w.b = x / hkv;
     w.part = s.prefix_runs + pr;
     w.r0 = w.b * R + (int64_t)t * tile;
-    w.rlim = (w.b + 1) * R;
-    w.o0 = pr * run;
-    w.o1 = w.o0 + run;
+    w.o0 = pr * s.own_run * kPrefixKeys;
+    w.o1 = w.o0 + s.own_run * kPrefixKeys;
   }
+  w.rlim = (w.b + 1) * R;
   if (w.o1 > w.o0) {  // up to what the tile's last query sees
     const int64_t last = (w.r0 + tile < w.rlim ? w.r0 + tile : w.rlim) - 1;
     const int64_t seen = own_seen(p, own_len(p, w.b), (last - w.b * R) / p.G);
@@ -124,25 +124,27 @@ __device__ __forceinline__ PrefixRow prefix_row(const PrefixParams &p, int64_t k
 // Matrix-core kernel of the 2-byte types. Four wavefronts: 4 / KS row groups of 32 rows, the KS wavefronts of a group
 // taking every block's 64 / KS keys. S^T = K Q^T, O^T += V^T P^T as attn_mfma_kernel does it: each lane holds one row's
 // scores of 16 keys, K and V blocks come by direct global -> LDS loads, two blocks deep.
-template <typename T, int D, int KS, int MINW>
-__global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, int64_t nwg) {
+template <typename T, int D, int KS> struct PrefixLds {
+  // the ring of two K and two V blocks; at the end the key groups' partial results
+  static constexpr int PW = KS > 1 ? (D / 32 * 16 + 2) * 64 : 0;  // floats of a wavefront
+  static constexpr int bytes = 4 * kPrefixKeys * D * 2 > 4 * PW * 4 ? 4 * kPrefixKeys * D * 2 : 4 * PW * 4;
+};
+template <typename T, int D, int KS>
+__device__ __forceinline__ void prefix_attend(const PrefixParams &p, const PrefixItem &w, uint16_t *smem) {
   using M = Mma<T>;
   using op_t = typename M::op_t;
-  constexpr int BKV = kPrefixKeys, NKT = BKV / 32 / KS, NDT = D / 32, TILE = 128 / KS;
+  constexpr int BKV = kPrefixKeys, NKT = BKV / 32 / KS, NDT = D / 32;
   constexpr int KCH = BKV * D / 8 / 256;   // 16-byte chunks of K (and V) per thread and block
   constexpr int BUF = BKV * D;             // 2-byte elements of a block
   constexpr bool VEARLY = D == 128 && KS == 2;  // 128 rows leave no registers for it
-  // the ring of two K and two V blocks; at the end the key groups' partial results
-  constexpr int PW = KS > 1 ? (NDT * 16 + 2) * 64 : 0;  // floats of a wavefront
-  constexpr int LDS = 4 * BUF * 2 > 4 * PW * 4 ? 4 * BUF * 2 : 4 * PW * 4;
-  __shared__ __align__(16) uint16_t smem[LDS / 2];
+  constexpr int PW = PrefixLds<T, D, KS>::PW;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   const int qg = wave / KS, kg = wave % KS, kt0 = kg * NKT;
 
-  const PrefixItem w = prefix_item(p, xcd_logical_id(blockIdx.x, nwg), TILE);
   const int64_t g = w.r0 + qg * 32 + l32;          // this lane's row
   const bool live = g < w.rlim;
+  const bool rows = w.r0 + qg * 32 < w.rlim;       // this wavefront's row group has rows (uniform)
   const int np = (int)((w.p1 - w.p0 + BKV - 1) / BKV), no = (int)((w.o1 - w.o0 + BKV - 1) / BKV), nblk = np + no;
 
   op_t qf[D / 16];
@@ -200,6 +202,11 @@ __global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, 
     constexpr bool MASK = decltype(mask_c)::value;
     const int buf = j & 1;
     if (j + 1 < nblk) issue(j + 1, buf ^ 1);
+    if (!rows) {  // a row group past the tile's last row only loads
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      lds_barrier();
+      return;
+    }
     const uint16_t *Ks = smem + buf * BUF, *Vs = smem + 2 * BUF + buf * BUF;
     f32x16_t s[NKT];
 #pragma unroll
@@ -342,6 +349,7 @@ __global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, 
     const int64_t rows = p.B * p.Lq * p.G * p.Hkv, r = (w.part * p.Hkv + w.kv) * (p.B * p.Lq * p.G) + g;
     float *po = p.ws + r * D;
     if (kg == 0 && hh == 0) *reinterpret_cast<float2 *>(p.ws + p.plan.parts * rows * D + r * 2) = make_float2(m, total);
+    if (m == -INFINITY) return;  // no key seen: the merge does not take this part's O
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
       if (KS > 1 && dt % KS != kg) continue;
@@ -366,31 +374,429 @@ __global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, 
   }
 }
 
-// Merges a row's partial results in their order: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). D / 4
-// lanes a row, 16 bytes each. A part that saw no key (m = -inf) is not read.
-template <typename T, int D>
+// ---- pipelined form: 128 QT rows a workgroup -------------------------------------
+//
+// attn_pipe_kernel's pipeline over the blocks of two key ranges: keys go by 32, two steps to a pair, and step j is one
+// straight line of MFMAs (scores of block j + 2, O += P V of block j) with the exponentials, the maximum and the LDS reads
+// in the gaps between them. Each of the 4 wavefronts keeps QT tiles of 32 rows. A block lies in one range: the prefix's
+// last one ends where the prefix ends, and the next begins the own keys. K and V arrive by direct global -> LDS loads in
+// two stages of 64 keys, of which wavefronts 0 and 1 load the first block and 2 and 3 the second, so that each builds the
+// descriptor of its block's range; what lies past the range reads as zeros.
+// The running maximum starts at -3e38 rather than -inf: a row that has seen nothing yet forms exp2(-inf) = 0.
+template <typename T, int D, int QT>
+__device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const PrefixItem &w, char *ring, int *seen_lds) {
+  using M = Mma<T>;
+  using op_t = typename M::op_t;
+  constexpr int BK = 32, NC = D / 16, NDT = D / 32;
+  constexpr int KB = BK * D * 2, STAGE = 4 * KB;          // bytes of a block; a stage: V, V, K, K
+  constexpr int SEGW = 2 * KB / 1024 / 4;                 // direct loads per wavefront for two blocks
+  constexpr int RS = 512 / D;                             // rows of a load
+  static_assert(SEGW * RS == 16, "two wavefronts load a block");
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  int *const seen = seen_lds + wave * (QT * 32) + l32;  // own keys from o0 on that the lane's rows see: read for a mask only
+  const int np = (int)((w.p1 - w.p0 + BK - 1) / BK), no = (int)((w.o1 - w.o0 + BK - 1) / BK), nkv = np + no;
+
+  op_t qf[QT][NC];
+  int all_seen;  // own keys from o0 on that every row of the tile sees
+  {
+    const int64_t len = own_len(p, w.b);
+    all_seen = __builtin_amdgcn_readfirstlane((int)(own_seen(p, len, (w.r0 - w.b * p.Lq * p.G) / p.G) - w.o0));
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int64_t g = w.r0 + wave * (QT * 32) + qt * 32 + l32;
+      const PrefixRow row = prefix_row(p, w.kv, g < w.rlim ? g : w.rlim - 1);
+      seen[qt * 32] = (int)(own_seen(p, len, row.i) - w.o0);
+      const char *q = reinterpret_cast<const char *>(p.q) + (row.b * p.q_sb + row.h * p.q_sh + row.i * p.q_st) * 2;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) qf[qt][c] = *reinterpret_cast<const op_t *>(q + (c * 16 + 8 * hh) * 2);
+    }
+  }
+
+  // the lane's part of a load: row r0 + RS i of its wavefront's block, the chunk that its slot holds
+  uint32_t ln = (uint32_t)lane;  // opaque in each load: its parts are formed again there, not kept
+  auto row_of = [&]() { return (uint32_t)(wave & 1) * 16 + ln / (D / 8); };
+  const char *ok = reinterpret_cast<const char *>(p.k) + (w.b * p.k_sb + w.kv * p.k_sh + w.o0 * p.k_st) * 2;
+  const char *ov = reinterpret_cast<const char *>(p.v) + (w.b * p.v_sb + w.kv * p.v_sh + w.o0 * p.v_st) * 2;
+  const int pn = (int)(w.p1 - w.p0), own_end = np * BK + (int)(w.o1 - w.o0);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)ring;
+  // The wavefront's blocks of K (of V): the descriptor of block `blk` of the item's, its keys of the range and zeros beyond.
+  // A stage's descriptors are formed while the stage before it is worked on, without branches: at the head of a stage, or
+  // with a branch for the range, their scalar instructions cost 8 to 15% of the kernel.
+  struct Source {
+    const char *pre, *own;
+    uint32_t pst2, ost2, st2;  // bytes from key to key: of the prefix, of the own keys, of this block
+    int blk;
+    i32x4_t rs;
+  };
+  auto describe = [&](Source &s) {
+    const bool own = s.blk >= np;
+    const int at = s.blk * BK, left = (own ? own_end : pn) - at, rows = left < BK ? left : BK;
+    s.st2 = own ? s.ost2 : s.pst2;
+    const uint64_t a = (uint64_t)(own ? s.own : s.pre) + (uint64_t)(uint32_t)at * s.st2;
+    const int bytes = rows > 0 ? (rows - 1) * (int)s.st2 + 2 * D : 0;
+    s.rs = i32x4_t{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)),
+                   __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+  };
+  auto source = [&](int blk, const void *pre, int64_t sh, int64_t pst, const char *own, int64_t ost) {
+    Source s;
+    s.pre = reinterpret_cast<const char *>(pre) + (w.kv * sh + w.p0 * pst) * 2;
+    s.own = own - (int64_t)(np * BK) * ost * 2;  // as if its blocks had been counted from the item's first
+    s.pst2 = (uint32_t)pst * 2;
+    s.ost2 = (uint32_t)ost * 2;
+    s.blk = blk + (wave >> 1);
+    describe(s);
+    return s;
+  };
+  Source sk = source(0, p.pk, p.pk_sh, p.pk_st, ok, p.k_st), sv = source(0, p.pv, p.pv_sh, p.pv_st, ov, p.v_st);
+  auto load_k = [&](const Source &s, uint32_t lds) {
+    asm volatile("" : "+v"(ln));
+    const uint32_t r = row_of(), off = r * s.st2, ch = ((ln % (D / 8)) ^ (uint32_t)k_swz<D>((int)r)) * 16;
+#pragma unroll
+    for (int i = 0; i < SEGW; ++i)
+      lds_load16(s.rs, off + (uint32_t)(i * RS) * s.st2 + (ch ^ (k_swz<D>(i * RS) * 16)), 0,
+                 __builtin_amdgcn_readfirstlane(lds + (wave * SEGW + i) * 1024));
+  };
+  auto load_v = [&](const Source &s, uint32_t lds) {
+    asm volatile("" : "+v"(ln));
+    const uint32_t r = row_of(), off = r * s.st2 + ((ln % (D / 8)) ^ (uint32_t)v_swz<D>((int)r)) * 16;
+#pragma unroll
+    for (int i = 0; i < SEGW; ++i)
+      lds_load16(s.rs, off + (uint32_t)(i * RS) * s.st2, 0, __builtin_amdgcn_readfirstlane(lds + (wave * SEGW + i) * 1024));
+  };
+  int slot = 0;  // stage g: V's blocks 2 g, 2 g + 1, K's 2 g + 3, 2 g + 4
+  auto load_stage = [&](int to) {
+    load_v(sv, lds0 + to * STAGE);
+    load_k(sk, lds0 + to * STAGE + 2 * KB);
+  };
+  int kfo = 2 * KB + l32 * 2 * D + ((hh ^ k_swz<D>(l32)) << 4);
+  auto kfrag = [&](int at, int c) { return *reinterpret_cast<const op_t *>(ring + at + (kfo ^ (c << 5))); };
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+  const int vr0 = 4 * hh + ((lane & 15) >> 2), vc0 = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  int vfo = vr0 * 2 * D + (((vc0 >> 3) ^ v_swz<D>(vr0)) << 4) + (vc0 & 7) * 2;
+  auto vhalf = [&](int at, int dt, int jj, int h) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4_t *)(ring + at + (vfo ^ (dt << 6)) + (16 * jj + 8 * h) * 2 * D));
+  };
+
+  f32x16_t o[QT][NDT], sa[QT], sb[QT];
+  float m[QT], l[QT], ls[QT], alpha[QT], mx[QT];
+  op_t kf[NC], pf[QT][2];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m[qt] = -3e38f;
+    l[qt] = ls[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x16_t{};
+  }
+  const float c2 = p.scale * kLog2e;
+
+  // block j's keys that a row does not see (past the prefix's end, the sequence's, or by causality) score -inf
+  auto mask = [&](int j, f32x16_t (&s)[QT]) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int lim = (j < np ? pn - j * BK : j < nkv ? seen[qt * 32] - (j - np) * BK : 0) - 4 * hh;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= lim) s[qt][i] = -INFINITY;
+    }
+  };
+  // blocks that need a mask: the prefix's last where it is not whole, and from own_first on
+  const int cut = pn % BK ? np - 1 : -1, all = all_seen > 0 ? all_seen / BK : 0, own_first = np + (all < no ? all : no);
+  auto partial = [&](int j) { return (j == cut) | (j >= own_first); };
+  auto max_step = [&](const f32x16_t (&s)[QT], int qt, int i, bool first) {
+    if (first && i == 0) mx[qt] = fmaxf(s[qt][0], s[qt][1]);
+    else mx[qt] = fmaxf(fmaxf(mx[qt], s[qt][2 * i]), s[qt][2 * i + 1]);
+  };
+  auto max_done = [&](int qt) {
+    const float cand = half_swap_max(mx[qt]) * c2;
+    float mn = m[qt];
+    if (cand > mn + 8.f) mn = cand;
+    alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mn);
+    m[qt] = mn;
+  };
+  auto sum_pair = [&](int qt) { l[qt] = __builtin_fmaf(l[qt], alpha[qt], ls[qt]); };
+
+  if (nkv > 0) {
+    // prologue: K's blocks 0, 1 and 2, 3 into the slot of stage 1, stage 0; the scores of the first pair, its maximum
+    load_k(sk, lds0 + STAGE + 2 * KB);
+    sk.blk += 2;
+    describe(sk);
+    load_k(sk, lds0 + STAGE);
+    sk.blk += 1;
+    describe(sk);
+    load_stage(0);
+    sk.blk += 2;
+    sv.blk += 2;
+    describe(sk);
+    describe(sv);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * SEGW));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    auto scores = [&](f32x16_t (&s)[QT]) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[qt] = M::run(kf[c], qf[qt][c], c == 0 ? f32x16_t{} : s[qt]);
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kf[c] = kfrag(STAGE, c);
+    scores(sa);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kf[c] = kfrag(STAGE + KB, c);
+    scores(sb);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kf[c] = kfrag(STAGE - 2 * KB, c);
+    mask(0, sa);
+    mask(1, sb);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) max_step(sa, qt, i, true);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) max_step(sb, qt, i, false);
+      max_done(qt);
+    }
+
+    // One step on block j, of parity PAR, whose scores are in s. NEXT: there is a next pair, and the scores of block
+    // j + 2 replace them. The mask is a branch inside the step: a second form of the step beside it, chosen by the block,
+    // spills 157 registers.
+    auto step = [&](int j, f32x16_t (&s)[QT], auto par_c, auto next_c) {
+      constexpr int PAR = decltype(par_c)::value;
+      constexpr bool NEXT = decltype(next_c)::value;
+      // MFMAs: the scores but for their last chunk, one half of P v, the scores' last chunk, the other half
+      constexpr int NA = NEXT ? QT * (NC - 1) : 0, NL = NEXT ? QT : 0, NB = QT * 2 * NDT, NM = NA + NB + NL;
+      constexpr int LAST = NA + NB / 2;  // the scores' last chunk
+      constexpr int at = PAR * KB;
+      if constexpr (PAR == 0) {
+        // the stage landed, and every wavefront is done with the one before
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        load_stage(slot ^ 1);
+        bool any = false;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) any = any || alpha[qt] != 1.f;
+        if (__builtin_amdgcn_ballot_w64(any)) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha[qt];
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) ls[qt] = 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      s16x4_t vh[NDT][2][2];
+      f32x16_t sn[QT];
+      // exponentials, two pairs of scores at a time: 4 FMAs, 4 exponentials, 2 packs, 2 sums
+      auto exp_op = [&](int n) {
+        const int g = n / 12, r = n % 12, qt = g / 4, e0 = 4 * (g % 4);
+        if (r < 4) {
+          s[qt][e0 + r] = __builtin_fmaf(s[qt][e0 + r], c2, -m[qt]);
+        } else if (r < 8) {
+          s[qt][e0 + r - 4] = __builtin_amdgcn_exp2f(s[qt][e0 + r - 4]);
+        } else {
+          const int h = r & 1, pe = e0 / 2 + h;  // packed pair pe of the tile: element pe % 4 of fragment pe / 4
+          u32x4_t pk4 = __builtin_bit_cast(u32x4_t, pf[qt][pe / 4]);
+          if (r < 10) pk4[pe % 4] = M::pack(s[qt][e0 + 2 * h], s[qt][e0 + 2 * h + 1]);
+          else ls[qt] = M::sum2(pk4[pe % 4], ls[qt]);
+          pf[qt][pe / 4] = __builtin_bit_cast(op_t, pk4);
+        }
+      };
+      // VALU items: 4 groups of 12 per tile; 8 steps of the maximum per tile and the pair's end
+      constexpr int NEXP = 48 * QT, NMT = PAR == 1 ? 9 : 8, NMAX = NEXT ? NMT * QT : 0, REST = NB / 2;
+      if constexpr (!NEXT) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vh[dt][jj][h] = vhalf(at, dt, jj, h);
+#pragma unroll
+        for (int n = 0; n < NEXP; ++n) exp_op(n);
+      }
+#pragma unroll
+      for (int u = 0; u < NM; ++u) {
+        if (u < NA) {
+          const int c = u / QT, qt = u % QT;
+          sn[qt] = M::run(kf[c], qf[qt][c], c == 0 ? f32x16_t{} : sn[qt]);
+          // V's 4 NDT fragment halves, spread over these MFMAs
+#pragma unroll
+          for (int x = 0; x < 4 * NDT; ++x)
+            if (x >= u * 4 * NDT / (NA ? NA : 1) && x < (u + 1) * 4 * NDT / (NA ? NA : 1))
+              vh[x / 4][x / 2 % 2][x % 2] = vhalf(at, x / 4, x / 2 % 2, x % 2);
+        } else if (u >= LAST && u < LAST + NL) {
+          const int qt = u - LAST;
+          s[qt] = M::run(kf[NC - 1], qf[qt][NC - 1], sn[qt]);
+          keep(sn[qt]);  // the product goes to s's registers, not to sn's and a copy
+        } else {
+          const int b = u < LAST ? u - NA : u - NA - NL, qt = b / (2 * NDT), jj = b / NDT % 2, dt = b % NDT;
+          const op_t a = __builtin_bit_cast(op_t, __builtin_shufflevector(vh[dt][jj][0], vh[dt][jj][1], 0, 1, 2, 3, 4, 5, 6, 7));
+          o[qt][dt] = M::run(a, pf[qt][jj], o[qt][dt]);
+          if (NEXT && b % QT == 0 && b / QT < NC) kf[b / QT] = kfrag(at, b / QT);
+        }
+        if constexpr (NEXT) {
+#pragma unroll
+          for (int n = 0; n < NEXP; ++n)
+            if (n >= u * NEXP / LAST && n < (u + 1) * NEXP / LAST) exp_op(n);
+          if (PAR == 1 && u == LAST - 1) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) sum_pair(qt);
+          }
+          if (u == LAST + NL - 1) {
+            // formed by here: the compiler would move what is used behind the branch there, away from the MFMAs before it
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int jj = 0; jj < 2; ++jj) asm volatile("" ::"v"(pf[qt][jj]), "v"(ls[qt]), "v"(l[qt]));
+#pragma unroll
+            for (int x = 0; x < 4 * NDT; ++x) asm volatile("" ::"v"(vh[x / 4][x / 2 % 2][x % 2]));
+            if (partial(j + 2)) mask(j + 2, s);
+          }
+          // the next stage's descriptors
+          if (PAR == 1 && (u == 1 || u == 3)) {
+            Source &src = u == 1 ? sv : sk;
+            src.blk += 2;
+            describe(src);
+          }
+          const int r = u - LAST - NL;
+#pragma unroll
+          for (int n = 0; n < NMAX; ++n)
+            if (r >= 0 && n >= r * NMAX / REST && n < (r + 1) * NMAX / REST) {
+              if (n % NMT < 8) max_step(s, n / NMT, n % NMT, PAR == 0);
+              else max_done(n / NMT);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (PAR == 1) {
+        slot ^= 1;
+        kfo ^= STAGE;
+        vfo ^= STAGE;
+      }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    constexpr std::true_type yes{};
+    constexpr std::false_type no_{};
+    int j = 0;
+    for (; j + 2 < nkv; j += 2) {
+      step(j, sa, even, yes);
+      step(j + 1, sb, odd, yes);
+    }
+    step(j, sa, even, no_);
+    if (j + 2 == nkv) step(j + 1, sb, odd, no_);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) sum_pair(qt);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads
+  }
+
+  // lane holds dims dt * 32 + 8 g4 + 4 hh + {0..3}, g4 = 0..3
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int64_t g = w.r0 + wave * (QT * 32) + qt * 32 + l32;
+    const float total = half_swap_sum(l[qt]);
+    if (g >= w.rlim) continue;
+    if (p.plan.parts > 1) {
+      const int64_t per = p.B * p.Lq * p.G, rows = per * p.Hkv, r = w.part * rows + w.kv * per + g;
+      const bool none = total == 0.f;
+      if (hh == 0) *reinterpret_cast<float2 *>(p.ws + p.plan.parts * rows * D + r * 2) = make_float2(none ? -INFINITY : m[qt], total);
+      if (none) continue;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+          *reinterpret_cast<float4 *>(p.ws + r * D + dt * 32 + 8 * g4 + 4 * hh) =
+              make_float4(o[qt][dt][4 * g4], o[qt][dt][4 * g4 + 1], o[qt][dt][4 * g4 + 2], o[qt][dt][4 * g4 + 3]);
+      continue;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const PrefixRow row = prefix_row(p, w.kv, g);
+    char *orow = reinterpret_cast<char *>(p.o) + (row.b * p.o_sb + row.h * p.o_sh + row.i * p.o_st) * 2;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<uint2 *>(orow + (dt * 32 + 8 * g4 + 4 * hh) * 2) =
+            make_uint2(M::pack(o[qt][dt][4 * g4] * inv, o[qt][dt][4 * g4 + 1] * inv),
+                       M::pack(o[qt][dt][4 * g4 + 2] * inv, o[qt][dt][4 * g4 + 3] * inv));
+  }
+}
+
+// JOINT: every workgroup 128 / KS rows (KS 1: pipelined, 128 QT rows) of one sequence through prefix and own keys. Else
+// pipelined prefix items of 128 rows, and own items whose few rows split each block's keys between two wavefronts.
+template <typename T, int D, bool JOINT, int KS, int QT, int MINW>
+__global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, int64_t nwg) {
+  constexpr int RING = 8 * 32 * D * 2, LDS = JOINT && KS == 1 ? RING : PrefixLds<T, D, 2>::bytes;
+  static_assert(LDS >= RING, "both item kinds fit");
+  __shared__ __align__(16) uint16_t smem[LDS / 2];
+  __shared__ int seen[JOINT && KS > 1 ? 1 : 128 * QT];
+  if constexpr (JOINT && KS > 1) {
+    prefix_attend<T, D, KS>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), smem);
+  } else if constexpr (JOINT) {
+    prefix_attend_pipe<T, D, QT>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), reinterpret_cast<char *>(smem), seen);
+  } else {
+    const int64_t np = p.Hkv * p.plan.prefix_tiles * p.plan.prefix_runs;
+    if ((int64_t)blockIdx.x < np)
+      prefix_attend_pipe<T, D, QT>(p, prefix_item(p, xcd_logical_id(blockIdx.x, np), true), reinterpret_cast<char *>(smem), seen);
+    else
+      prefix_attend<T, D, 2>(p, prefix_item(p, (int64_t)blockIdx.x - np, false), smem);
+  }
+}
+
+// Merges a row's partial results: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). D / 4 lanes hold a row, 16
+// bytes each; GP groups of them take every GP th part, four loads in flight, and their results are added in group order
+// through LDS. A part that saw no key (m = -inf) has left no O: its weight is zero and what was read for it is dropped.
+template <typename T, int D, int GP>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixParams p) {
-  constexpr int LPR = D / 4, RPB = 256 / LPR;
+  constexpr int LPR = D / 4, RPB = 256 / (LPR * GP), U = 4;
+  __shared__ float4 so[GP > 1 ? 256 : 1];
+  __shared__ float2 sml[GP > 1 ? 256 : 1];
   const int64_t per = p.B * p.Lq * p.G, rows = per * p.Hkv;
-  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-  if (r >= rows) return;
-  const int d = (int)(threadIdx.x % LPR) * 4;
+  const int t = threadIdx.x, grp = t / LPR % GP;
+  int64_t r = (int64_t)blockIdx.x * RPB + t / (LPR * GP);
+  const bool live = r < rows;
+  r = live ? r : rows - 1;
+  const int d = (t % LPR) * 4;
   const float2 *ml = reinterpret_cast<const float2 *>(p.ws + p.plan.parts * rows * D);
+  const int parts = (int)p.plan.parts;
   float m = -INFINITY, l = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t s = 0; s < p.plan.parts; ++s) {
-    const float2 v = ml[s * rows + r];
-    if (v.x == -INFINITY) continue;
-    const float4 x = *reinterpret_cast<const float4 *>(p.ws + (s * rows + r) * D + d);
-    const float mn = fmaxf(m, v.x);
-    const float a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(v.x - mn);
+  auto add = [&](float mp, float lp, const float4 &x) {
+    const float mn = fmaxf(m, mp), mb = mn == -INFINITY ? 0.f : mn;
+    const float a = __builtin_amdgcn_exp2f(m - mb), b = __builtin_amdgcn_exp2f(mp - mb);
+    const bool none = mp == -INFINITY;
     m = mn;
-    l = l * a + v.y * b;
-    acc[0] = acc[0] * a + x.x * b;
-    acc[1] = acc[1] * a + x.y * b;
-    acc[2] = acc[2] * a + x.z * b;
-    acc[3] = acc[3] * a + x.w * b;
+    l = l * a + lp * b;
+    acc[0] = acc[0] * a + (none ? 0.f : x.x * b);
+    acc[1] = acc[1] * a + (none ? 0.f : x.y * b);
+    acc[2] = acc[2] * a + (none ? 0.f : x.z * b);
+    acc[3] = acc[3] * a + (none ? 0.f : x.w * b);
+  };
+  for (int s0 = grp; s0 < parts; s0 += GP * U) {
+    float2 v[U];
+    float4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * GP < parts ? s0 + u * GP : s0;
+      v[u] = ml[s * rows + r];
+      x[u] = *reinterpret_cast<const float4 *>(p.ws + (s * rows + r) * D + d);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * GP < parts) add(v[u].x, v[u].y, x[u]);
   }
+  if constexpr (GP > 1) {
+    so[t] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    sml[t] = make_float2(m, l);
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int g = 1; g < GP; ++g) add(sml[t + g * LPR].x, sml[t + g * LPR].y, so[t + g * LPR]);
+  }
+  if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t kv = r / per;
   const PrefixRow row = prefix_row(p, kv, r - kv * per);
@@ -493,12 +899,16 @@ hipError_t launch_prefix_mfma(const PrefixParams &p, hipStream_t s) {
   if (nwg > INT32_MAX || p.B * p.Lq * p.G > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)nwg), block(256);
   constexpr int MINW = D == 64 ? 3 : 2;
-  if (p.plan.ks == 1) hipLaunchKernelGGL((prefix_attn_kernel<T, D, 1, MINW>), grid, block, 0, s, p, nwg);
-  else hipLaunchKernelGGL((prefix_attn_kernel<T, D, 2, MINW>), grid, block, 0, s, p, nwg);
+  if (!p.plan.joint) hipLaunchKernelGGL((prefix_attn_kernel<T, D, false, 1, 1, MINW>), grid, block, 0, s, p, nwg);
+  else if (p.plan.ks == 2) hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 2, 1, MINW>), grid, block, 0, s, p, nwg);
+  else hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 1, 1, MINW>), grid, block, 0, s, p, nwg);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.plan.parts > 1) {
-    const int64_t rows = p.B * p.H * p.Lq, per = 256 / (D / 4);
-    hipLaunchKernelGGL((prefix_merge_kernel<T, D>), dim3((unsigned)((rows + per - 1) / per)), block, 0, s, p);
+    const int64_t rows = p.B * p.H * p.Lq;
+    constexpr int LPR = D / 4;
+    auto grid_of = [&](int gp) { return dim3((unsigned)((rows * LPR * gp + 255) / 256)); };
+    if (p.plan.parts <= 4) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1>), grid_of(1), block, 0, s, p);
+    else hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4>), grid_of(4), block, 0, s, p);
   }
   return hipGetLastError();
 }
