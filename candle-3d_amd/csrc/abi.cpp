@@ -1151,7 +1151,7 @@ int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t
                                            int64_t own, int64_t head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries <= 0 || prefix < 0 || own < 0 || head_dim <= 0)
     return 0;
-  const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own);
+  const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own, head_dim);
   return prefix_workspace(plan, batch, heads, queries, head_dim);
 }
 
@@ -1210,7 +1210,7 @@ int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *pref
            prefix_block_fits(prefix_k, p.D) && prefix_block_fits(prefix_v, p.D) && prefix_block_fits(k, p.D) &&
            prefix_block_fits(v, p.D);
   if (p.mfma) {
-    p.plan = prefix_plan(p.B, p.H, p.Hkv, p.Lq, p.P, p.Ls);
+    p.plan = prefix_plan(p.B, p.H, p.Hkv, p.Lq, p.P, p.Ls, p.D);
     const int64_t need = prefix_workspace(p.plan, p.B, p.H, p.Lq, p.D);
     if (need > 0) {
       if ((r = check_desc(workspace, fn, "workspace"))) return r;

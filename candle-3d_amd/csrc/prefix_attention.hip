@@ -907,7 +907,8 @@ hipError_t launch_prefix_mfma(const PrefixParams &p, hipStream_t s) {
     const int64_t rows = p.B * p.H * p.Lq;
     constexpr int LPR = D / 4;
     auto grid_of = [&](int gp) { return dim3((unsigned)((rows * LPR * gp + 255) / 256)); };
-    if (p.plan.parts <= 4) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1>), grid_of(1), block, 0, s, p);
+    if (p.plan.parts > 32) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 256 / LPR>), grid_of(256 / LPR), block, 0, s, p);
+    else if (p.plan.parts <= 4) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1>), grid_of(1), block, 0, s, p);
     else hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4>), grid_of(4), block, 0, s, p);
   }
   return hipGetLastError();

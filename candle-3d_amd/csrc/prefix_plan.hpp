@@ -24,21 +24,42 @@ struct PrefixPlan {
 
 inline int64_t prefix_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t P, int64_t Ls) {
+// Joint: into how many runs the keys of `tiles` tiles of 128 rows are cut, by the time that follows: the busiest CU's
+// blocks (us a block with 1, 2 or 3 workgroups on the CU: D 64 0.83, 1.25, 1.85, D 128 1.07, 1.9), and for more than one
+// run the merge, 4 us and the partial results' bytes at 4 TB/s. us, one run / the one so chosen / the best of 1 to 16: 2 x
+// 16 heads x 300 on 1029 + 300 24.7 / 20.6 / 20.6, 16 x 1374 on 10992 + 1374 165 / 98.9 / 98.9, 16 x 130 on 16000 + 130
+// 211 / 31.3 / 31.3 (D 64); 3 x 12 / 4 x 333 on 4001 + 707 85.1 / 51.0 / 51.0, 12 x 1029 on 4000 + 1029 90.4 / 58.2 / 52.3,
+// 4 x 12 x 200 on 1029 + 200 28.3 / 26.9 / 26.9, 2 x 12 x 2000 on 4000 + 2000 167 / 167 / 163 (D 128).
+inline int64_t prefix_joint_runs(int64_t tiles, int64_t blocks, int64_t rows, int64_t D) {
+  const double t64[4] = {0, 0.83, 1.25, 1.85}, t128[3] = {0, 1.07, 1.9};
+  const int per_cu = D <= 64 ? 3 : 2;
+  const double *t = D <= 64 ? t64 : t128;
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t runs = 1; runs <= 16 && (runs == 1 || runs <= blocks / 2); ++runs) {
+    const int64_t m = prefix_ceil(tiles * runs, 256);
+    double us = (double)prefix_ceil(blocks, runs) * ((double)(m / per_cu) * t[per_cu] + t[m % per_cu]);
+    if (runs > 1) us += 4 + (double)rows * (double)runs * (double)D * 8 / 4e6;
+    if (runs == 1 || us < least) least = us, best = runs;
+  }
+  return best;
+}
+
+inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t P, int64_t Ls, int64_t D) {
   PrefixPlan s;
   const int64_t rows = Lq * (H / Hkv);                                    // of one sequence and key head
   const int64_t pb = prefix_ceil(P, kPrefixKeys), ob = prefix_ceil(Ls, kPrefixKeys);
-  const int64_t slots = 512;                                              // two workgroups on each of 256 CUs
+  auto run_of = [](int64_t blocks, int64_t runs) { return blocks <= 0 ? 1 : runs > 1 ? prefix_ceil(blocks, runs) : blocks; };
   s.joint = rows >= 128 || B == 1;
   if (s.joint) {
     s.ks = rows > 64 ? 1 : 2;
     s.tile = 128 / s.ks;
     s.own_tiles = prefix_ceil(rows, s.tile);
     const int64_t tiles = B * Hkv * s.own_tiles, blocks = pb + ob;
-    // too few tiles for the chip: runs of the keys that fill it once, four blocks or more each
-    int64_t runs = slots / tiles;
-    if (runs > blocks / 4) runs = blocks / 4;
-    s.own_run = runs > 1 ? prefix_ceil(blocks, runs) : blocks > 0 ? blocks : 1;
+    // few rows, bound by the keys' bytes: runs that fill the chip twice, two blocks or more each
+    int64_t runs = s.ks == 1 ? prefix_joint_runs(tiles, blocks, B * H * Lq, D) : 512 / tiles;
+    if (runs > blocks / 2) runs = blocks / 2;
+    s.own_run = run_of(blocks, runs);
     s.own_runs = blocks > 0 ? prefix_ceil(blocks, s.own_run) : 1;
     s.parts = s.own_runs;
     s.wgs = tiles * s.own_runs;
@@ -46,14 +67,16 @@ inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int
   }
   s.prefix_tiles = prefix_ceil(B * rows, s.tile);
   s.own_tiles = prefix_ceil(rows, s.own_tile);
-  // the prefix fills the chip once, beside the own keys' workgroups
+  // The prefix's workgroups take half of the CUs, or all where there are few own keys: with more of them the own keys'
+  // workgroups, which wait for memory, start late. us with 64 / 128 / 256 of them: 64 x 32 / 8 heads on 16384 + 1000 (D
+  // 128) 80.7 / 50.5 / 59.6, 4 x 16 on 16384 + 2000 (D 64) 62.7 / 36.4 / 23.8, 64 x 16 on 4096 + 100 21.9 / 21.5 / 21.4.
   const int64_t tiles = Hkv * s.prefix_tiles, own = Hkv * B * s.own_tiles;
-  int64_t runs = prefix_ceil(slots / 2, tiles);
+  int64_t runs = prefix_ceil(2 * own * ob <= tiles * pb ? 256 : 128, tiles);
   if (runs > pb / 2) runs = pb / 2;
-  s.prefix_run = runs > 1 ? prefix_ceil(pb, runs) : pb > 0 ? pb : 1;
-  runs = prefix_ceil(slots, own);
+  s.prefix_run = run_of(pb, runs);
+  runs = prefix_ceil(512, own);
   if (runs > ob / 4) runs = ob / 4;
-  s.own_run = runs > 1 ? prefix_ceil(ob, runs) : ob > 0 ? ob : 1;
+  s.own_run = run_of(ob, runs);
   s.prefix_runs = prefix_ceil(pb, s.prefix_run);
   s.own_runs = prefix_ceil(ob, s.own_run);
   s.parts = s.prefix_runs + s.own_runs;
