@@ -1151,8 +1151,14 @@ int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t
                                            int64_t own, int64_t head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries <= 0 || prefix < 0 || own < 0 || head_dim <= 0)
     return 0;
-  const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own, head_dim);
-  return prefix_workspace(plan, batch, heads, queries, head_dim);
+  // the larger of the two element sizes' plans
+  int64_t most = 0;
+  for (bool f32 : {false, true}) {
+    const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own, head_dim, f32);
+    const int64_t n = prefix_workspace(plan, batch, heads, queries, head_dim);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *prefix_k, const lux3d_tensor_t *prefix_v,
@@ -1205,12 +1211,15 @@ int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *pref
   p.o_sb = out->stride[0]; p.o_sh = out->stride[1]; p.o_st = out->stride[2];
   p.causal = causal != 0;
   p.scale = scale;
-  p.mfma = dt != LUX3D_F32 && (p.D == 64 || p.D == 128) && prefix_aligned(q) && prefix_aligned(prefix_k) &&
+  // no keys: an address that exists in place of an empty tensor's, for descriptors of no bytes
+  if (p.P == 0) p.pk = p.pv = p.q, p.pk_sh = p.pv_sh = 0, p.pk_st = p.pv_st = p.D;
+  if (p.Ls == 0) p.k = p.v = p.q, p.k_sb = p.v_sb = p.k_sh = p.v_sh = 0, p.k_st = p.v_st = p.D;
+  p.mfma = (p.D == 64 || p.D == 128) && prefix_aligned(q) && prefix_aligned(prefix_k) &&
            prefix_aligned(prefix_v) && prefix_aligned(k) && prefix_aligned(v) && prefix_aligned(out) &&
            prefix_block_fits(prefix_k, p.D) && prefix_block_fits(prefix_v, p.D) && prefix_block_fits(k, p.D) &&
            prefix_block_fits(v, p.D);
   if (p.mfma) {
-    p.plan = prefix_plan(p.B, p.H, p.Hkv, p.Lq, p.P, p.Ls, p.D);
+    p.plan = prefix_plan(p.B, p.H, p.Hkv, p.Lq, p.P, p.Ls, p.D, dt == LUX3D_F32);
     const int64_t need = prefix_workspace(p.plan, p.B, p.H, p.Lq, p.D);
     if (need > 0) {
       if ((r = check_desc(workspace, fn, "workspace"))) return r;

@@ -15,7 +15,8 @@
 //
 // Masks. Keys past a sequence's length are never read: the buffer loads end at the last visible key and return zeros, so
 // that a probability of zero meets a finite value. Inside a tile, keys that causality hides from some of its rows are
-// read for the others; scores there become -inf whatever K holds, and V there is handled as described at `poison`.
+// read for the others: their scores become -inf whatever K holds, and their V, times a probability of zero, has to be
+// finite.
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -746,12 +747,202 @@ __global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, 
   }
 }
 
+// ---- f32 on the bf16 matrix cores ------------------------------------------------
+//
+// attn_f32x3_kernel's arithmetic over two key ranges: q, k, v and the probabilities as three exact bf16 terms each, six
+// significant products an MFMA step, scores, probabilities and sums in f32. 128 rows a workgroup, 32 a wavefront; blocks of
+// 32 keys are loaded as f32 (zeros past the range), split in registers and stored as three bf16 planes each of K and V,
+// double-buffered. A wavefront without rows only stages.
+template <int D, bool JOINT, int MINW>
+__global__ __launch_bounds__(256, MINW) void prefix_f32_kernel(PrefixParams p, int64_t nwg) {
+  using op_t = bf16x8_t;
+  using M = Mma<BF16>;
+  constexpr int BK = 32, NC = D / 16, NDT = D / 32;
+  constexpr int KROW = D + 8;              // bf16 per plane row
+  constexpr int PL = BK * KROW;            // one plane of one block
+  constexpr int KCH = BK * D / 4 / 256;    // 16-byte f32 chunks of K (and of V) per thread and block
+  __shared__ __align__(16) uint16_t smem[2 * 6 * PL];  // [buffer][K planes 0..2, V planes 0..2]
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int64_t npi = JOINT ? nwg : p.Hkv * p.plan.prefix_tiles * p.plan.prefix_runs;
+  const bool first = JOINT || (int64_t)blockIdx.x < npi;
+  const PrefixItem w = prefix_item(p, first ? xcd_logical_id(blockIdx.x, npi) : (int64_t)blockIdx.x - npi, first);
+  const int64_t g = w.r0 + wave * 32 + l32;
+  const bool live = g < w.rlim, rows = w.r0 + wave * 32 < w.rlim;
+  const int np = (int)((w.p1 - w.p0 + BK - 1) / BK), no = (int)((w.o1 - w.o0 + BK - 1) / BK), nkv = np + no;
+  const int pn = (int)(w.p1 - w.p0), on = (int)(w.o1 - w.o0);
+
+  op_t q[3][NC];
+  int seen, all_seen;  // own keys from o0 on that this lane's row sees; that every row of the tile sees
+  {
+    const PrefixRow row = prefix_row(p, w.kv, live ? g : w.rlim - 1);
+    const int64_t len = own_len(p, w.b);
+    seen = (int)(own_seen(p, len, row.i) - w.o0);
+    all_seen = __builtin_amdgcn_readfirstlane((int)(own_seen(p, len, (w.r0 - w.b * p.Lq * p.G) / p.G) - w.o0));
+    const float *qr = reinterpret_cast<const float *>(p.q) + row.b * p.q_sb + row.h * p.q_sh + row.i * p.q_st;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float x[8];
+      Chunk<F32>::load<false>(qr + c * 16 + 8 * hh, x);
+      u32x4_t x1, x2, x3;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split3_into(x[2 * e], x[2 * e + 1], x1, x2, x3, e);
+      q[0][c] = __builtin_bit_cast(op_t, x1);
+      q[1][c] = __builtin_bit_cast(op_t, x2);
+      q[2][c] = __builtin_bit_cast(op_t, x3);
+    }
+  }
+  const float *pk = reinterpret_cast<const float *>(p.pk) + w.kv * p.pk_sh + w.p0 * p.pk_st;
+  const float *pv = reinterpret_cast<const float *>(p.pv) + w.kv * p.pv_sh + w.p0 * p.pv_st;
+  const float *ok = reinterpret_cast<const float *>(p.k) + w.b * p.k_sb + w.kv * p.k_sh + w.o0 * p.k_st;
+  const float *ov = reinterpret_cast<const float *>(p.v) + w.b * p.v_sb + w.kv * p.v_sh + w.o0 * p.v_st;
+  // staging: chunk t + 256 i holds floats 4 (c % (D / 4)) .. of the block's row c / (D / 4)
+  float4 rk[KCH], rv[KCH];
+  auto load = [&](int j) {
+    const bool pre = j < np;
+    const int at = (pre ? j : j - np) * BK, left = (pre ? pn : on) - at;
+    const int64_t kst = pre ? p.pk_st : p.k_st, vst = pre ? p.pv_st : p.v_st;
+    const float *kb = (pre ? pk : ok) + at * kst, *vb = (pre ? pv : ov) + at * vst;
+#pragma unroll
+    for (int i = 0; i < KCH; ++i) {
+      const int c = t + i * 256, r = c / (D / 4), o = (c % (D / 4)) * 4;
+      rk[i] = rv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < left) {
+        rk[i] = *reinterpret_cast<const float4 *>(kb + r * kst + o);
+        rv[i] = *reinterpret_cast<const float4 *>(vb + r * vst + o);
+      }
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < KCH; ++i) {
+      const int c = t + i * 256, off = c / (D / 4) * KROW + (c % (D / 4)) * 4;
+      const Split3 ka = split3_bf16(rk[i].x, rk[i].y), kb = split3_bf16(rk[i].z, rk[i].w);
+      const Split3 va = split3_bf16(rv[i].x, rv[i].y), vb = split3_bf16(rv[i].z, rv[i].w);
+      uint16_t *d = smem + buf * 6 * PL + off;
+      *reinterpret_cast<uint2 *>(d) = make_uint2(ka.t1, kb.t1);
+      *reinterpret_cast<uint2 *>(d + PL) = make_uint2(ka.t2, kb.t2);
+      *reinterpret_cast<uint2 *>(d + 2 * PL) = make_uint2(ka.t3, kb.t3);
+      *reinterpret_cast<uint2 *>(d + 3 * PL) = make_uint2(va.t1, vb.t1);
+      *reinterpret_cast<uint2 *>(d + 4 * PL) = make_uint2(va.t2, vb.t2);
+      *reinterpret_cast<uint2 *>(d + 5 * PL) = make_uint2(va.t3, vb.t3);
+    }
+  };
+  f32x16_t o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16_t{};
+  float m = -3e38f, l = 0.f;
+  const float c2 = p.scale * kLog2e;
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+  auto compute = [&](int j) {
+    const uint16_t *K1 = smem + (j & 1) * 6 * PL, *V1 = K1 + 3 * PL;
+    f32x16_t s = f32x16_t{};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int off = l32 * KROW + (2 * c + hh) * 8;
+      const op_t a1 = *reinterpret_cast<const op_t *>(K1 + off), a2 = *reinterpret_cast<const op_t *>(K1 + PL + off);
+      const op_t a3 = *reinterpret_cast<const op_t *>(K1 + 2 * PL + off);
+      s = M::run(a3, q[0][c], s);
+      s = M::run(a2, q[1][c], s);
+      s = M::run(a1, q[2][c], s);
+      s = M::run(a2, q[0][c], s);
+      s = M::run(a1, q[1][c], s);
+      s = M::run(a1, q[0][c], s);
+    }
+    // this lane's row sees keys below lim of the block; lane holds keys 8 (i / 4) + 4 hh + i % 4
+    if (j < np ? (j + 1) * BK > pn : (j - np + 1) * BK > all_seen) {
+      const int lim = (j < np ? pn - j * BK : seen - (j - np) * BK) - 4 * hh;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= lim) s[i] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    const float cand = half_swap_max(mx) * c2;
+    const float mn = cand > m + 8.f ? cand : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    float ls = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -mn));
+      ls += s[i];
+    }
+    l = l * alpha + ls;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+    }
+    // V^T fragments of each plane: see attn_mfma_kernel
+    auto vfrag = [&](int pl, int dt, int jj) {
+      const int g16 = lane & 15;
+      const int vrow = 16 * jj + 4 * hh + (g16 >> 2), vcol = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (g16 & 3);
+      const uint16_t *vr = V1 + pl * PL + vrow * KROW + vcol;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vr));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vr + 8 * KROW));
+      return __builtin_bit_cast(op_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      u32x4_t x1, x2, x3;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split3_into(s[8 * jj + 2 * e], s[8 * jj + 2 * e + 1], x1, x2, x3, e);
+      const op_t P1 = __builtin_bit_cast(op_t, x1), P2 = __builtin_bit_cast(op_t, x2), P3 = __builtin_bit_cast(op_t, x3);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const op_t v1 = vfrag(0, dt, jj), v2 = vfrag(1, dt, jj), v3 = vfrag(2, dt, jj);
+        o[dt] = M::run(v3, P1, o[dt]);
+        o[dt] = M::run(v2, P2, o[dt]);
+        o[dt] = M::run(v1, P3, o[dt]);
+        o[dt] = M::run(v2, P1, o[dt]);
+        o[dt] = M::run(v1, P2, o[dt]);
+        o[dt] = M::run(v1, P1, o[dt]);
+      }
+    }
+  };
+  if (nkv > 0) {
+    load(0);
+    store(0);
+    lds_barrier();
+    for (int j = 0; j < nkv; ++j) {
+      if (j + 1 < nkv) load(j + 1);
+      if (rows) compute(j);
+      if (j + 1 < nkv) store((j + 1) & 1);
+      lds_barrier();
+    }
+  }
+  const float total = half_swap_sum(l);
+  if (!live) return;
+  // lane holds dims dt * 32 + 8 g4 + 4 hh + {0..3}
+  float *dst;
+  float f = 1.f;
+  if (p.plan.parts > 1) {
+    const int64_t per = p.B * p.Lq * p.G, all = per * p.Hkv, r = w.part * all + w.kv * per + g;
+    const bool none = total == 0.f;
+    if (hh == 0) *reinterpret_cast<float2 *>(p.ws + p.plan.parts * all * D + r * 2) = make_float2(none ? -INFINITY : m, total);
+    if (none) return;
+    dst = p.ws + r * D;
+  } else {
+    const PrefixRow row = prefix_row(p, w.kv, g);
+    dst = reinterpret_cast<float *>(p.o) + row.b * p.o_sb + row.h * p.o_sh + row.i * p.o_st;
+    f = total == 0.f ? 0.f : 1.f / total;
+  }
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      *reinterpret_cast<float4 *>(dst + dt * 32 + 8 * g4 + 4 * hh) =
+          make_float4(o[dt][4 * g4] * f, o[dt][4 * g4 + 1] * f, o[dt][4 * g4 + 2] * f, o[dt][4 * g4 + 3] * f);
+}
+
 // Merges a row's partial results: M = max m_s, out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M). D / 4 lanes hold a row, 16
-// bytes each; GP groups of them take every GP th part, four loads in flight, and their results are added in group order
+// bytes each; GP groups of them take every GP th part, U loads in flight, and their results are added in group order
 // through LDS. A part that saw no key (m = -inf) has left no O: its weight is zero and what was read for it is dropped.
-template <typename T, int D, int GP>
+template <typename T, int D, int GP, int U>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixParams p) {
-  constexpr int LPR = D / 4, RPB = 256 / (LPR * GP), U = 4;
+  constexpr int LPR = D / 4, RPB = 256 / (LPR * GP);
   __shared__ float4 so[GP > 1 ? 256 : 1];
   __shared__ float2 sml[GP > 1 ? 256 : 1];
   const int64_t per = p.B * p.Lq * p.G, rows = per * p.Hkv;
@@ -895,21 +1086,27 @@ hipError_t launch_prefix_generic(const PrefixParams &p, hipStream_t s) {
 
 template <typename T, int D>
 hipError_t launch_prefix_mfma(const PrefixParams &p, hipStream_t s) {
-  const int64_t nwg = p.plan.wgs;
-  if (nwg > INT32_MAX || p.B * p.Lq * p.G > INT32_MAX) return hipErrorInvalidValue;
+  const int64_t nwg = p.plan.wgs, rows = p.B * p.H * p.Lq;
+  constexpr int LPR = D / 4;
+  if (nwg > INT32_MAX || rows > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)nwg), block(256);
-  constexpr int MINW = D == 64 ? 3 : 2;
-  if (!p.plan.joint) hipLaunchKernelGGL((prefix_attn_kernel<T, D, false, 1, 1, MINW>), grid, block, 0, s, p, nwg);
-  else if (p.plan.ks == 2) hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 2, 1, MINW>), grid, block, 0, s, p, nwg);
-  else hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 1, 1, MINW>), grid, block, 0, s, p, nwg);
+  if constexpr (T::code == LUX3D_F32) {
+    constexpr int MINW = D == 64 ? 2 : 1;
+    if (!p.plan.joint) hipLaunchKernelGGL((prefix_f32_kernel<D, false, MINW>), grid, block, 0, s, p, nwg);
+    else hipLaunchKernelGGL((prefix_f32_kernel<D, true, MINW>), grid, block, 0, s, p, nwg);
+  } else {
+    constexpr int MINW = D == 64 ? 3 : 2;
+    if (!p.plan.joint) hipLaunchKernelGGL((prefix_attn_kernel<T, D, false, 1, 1, MINW>), grid, block, 0, s, p, nwg);
+    else if (p.plan.ks == 2) hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 2, 1, MINW>), grid, block, 0, s, p, nwg);
+    else hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 1, 1, MINW>), grid, block, 0, s, p, nwg);
+  }
   if (hipError_t e = hipGetLastError()) return e;
   if (p.plan.parts > 1) {
-    const int64_t rows = p.B * p.H * p.Lq;
-    constexpr int LPR = D / 4;
     auto grid_of = [&](int gp) { return dim3((unsigned)((rows * LPR * gp + 255) / 256)); };
-    if (p.plan.parts > 32) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 256 / LPR>), grid_of(256 / LPR), block, 0, s, p);
-    else if (p.plan.parts <= 4) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1>), grid_of(1), block, 0, s, p);
-    else hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4>), grid_of(4), block, 0, s, p);
+    // few parts of many rows: a row's lanes take them all, eight loads in flight
+    if (p.plan.parts > 32) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 256 / LPR, 4>), grid_of(256 / LPR), block, 0, s, p);
+    else if (p.plan.parts > 8 || rows < 4096) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4, 4>), grid_of(4), block, 0, s, p);
+    else hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1, 8>), grid_of(1), block, 0, s, p);
   }
   return hipGetLastError();
 }
@@ -926,7 +1123,9 @@ hipError_t launch_prefix_attention(int dt, const PrefixParams &p, hipStream_t s)
     case LUX3D_F16:
       if (p.mfma) return p.D == 64 ? launch_prefix_mfma<F16, 64>(p, s) : launch_prefix_mfma<F16, 128>(p, s);
       return launch_prefix_generic<F16>(p, s);
-    case LUX3D_F32: return launch_prefix_generic<F32>(p, s);
+    case LUX3D_F32:
+      if (p.mfma) return p.D == 64 ? launch_prefix_mfma<F32, 64>(p, s) : launch_prefix_mfma<F32, 128>(p, s);
+      return launch_prefix_generic<F32>(p, s);
   }
   return hipErrorInvalidValue;
 }

@@ -30,10 +30,10 @@ inline int64_t prefix_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // 16 heads x 300 on 1029 + 300 24.7 / 20.6 / 20.6, 16 x 1374 on 10992 + 1374 165 / 98.9 / 98.9, 16 x 130 on 16000 + 130
 // 211 / 31.3 / 31.3 (D 64); 3 x 12 / 4 x 333 on 4001 + 707 85.1 / 51.0 / 51.0, 12 x 1029 on 4000 + 1029 90.4 / 58.2 / 52.3,
 // 4 x 12 x 200 on 1029 + 200 28.3 / 26.9 / 26.9, 2 x 12 x 2000 on 4000 + 2000 167 / 167 / 163 (D 128).
-inline int64_t prefix_joint_runs(int64_t tiles, int64_t blocks, int64_t rows, int64_t D) {
-  const double t64[4] = {0, 0.83, 1.25, 1.85}, t128[3] = {0, 1.07, 1.9};
-  const int per_cu = D <= 64 ? 3 : 2;
-  const double *t = D <= 64 ? t64 : t128;
+inline int64_t prefix_joint_runs(int64_t tiles, int64_t blocks, int64_t rows, int64_t D, bool f32) {
+  const double t64[4] = {0, 0.83, 1.25, 1.85}, t128[3] = {0, 1.07, 1.9}, f64[3] = {0, 3.3, 5.0}, f128[2] = {0, 6.6};
+  const int per_cu = (D <= 64 ? 3 : 2) - f32;
+  const double *t = f32 ? (D <= 64 ? f64 : f128) : D <= 64 ? t64 : t128;
   int64_t best = 1;
   double least = 0;
   for (int64_t runs = 1; runs <= 16 && (runs == 1 || runs <= blocks / 2); ++runs) {
@@ -45,19 +45,20 @@ inline int64_t prefix_joint_runs(int64_t tiles, int64_t blocks, int64_t rows, in
   return best;
 }
 
-inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t P, int64_t Ls, int64_t D) {
+inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t P, int64_t Ls, int64_t D,
+                              bool f32) {
   PrefixPlan s;
   const int64_t rows = Lq * (H / Hkv);                                    // of one sequence and key head
   const int64_t pb = prefix_ceil(P, kPrefixKeys), ob = prefix_ceil(Ls, kPrefixKeys);
   auto run_of = [](int64_t blocks, int64_t runs) { return blocks <= 0 ? 1 : runs > 1 ? prefix_ceil(blocks, runs) : blocks; };
   s.joint = rows >= 128 || B == 1;
   if (s.joint) {
-    s.ks = rows > 64 ? 1 : 2;
+    s.ks = rows > 64 || f32 ? 1 : 2;
     s.tile = 128 / s.ks;
     s.own_tiles = prefix_ceil(rows, s.tile);
     const int64_t tiles = B * Hkv * s.own_tiles, blocks = pb + ob;
     // few rows, bound by the keys' bytes: runs that fill the chip twice, two blocks or more each
-    int64_t runs = s.ks == 1 ? prefix_joint_runs(tiles, blocks, B * H * Lq, D) : 512 / tiles;
+    int64_t runs = rows > 64 ? prefix_joint_runs(tiles, blocks, B * H * Lq, D, f32) : 512 / tiles;
     if (runs > blocks / 2) runs = blocks / 2;
     s.own_run = run_of(blocks, runs);
     s.own_runs = blocks > 0 ? prefix_ceil(blocks, s.own_run) : 1;
@@ -65,6 +66,7 @@ inline PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int
     s.wgs = tiles * s.own_runs;
     return s;
   }
+  if (f32) s.own_tile = 128;
   s.prefix_tiles = prefix_ceil(B * rows, s.tile);
   s.own_tiles = prefix_ceil(rows, s.own_tile);
   // The prefix's workgroups take half of the CUs, or all where there are few own keys: with more of them the own keys'

@@ -576,15 +576,17 @@ int lux3d_sdpa(const lux3d_tensor_t *q, const lux3d_tensor_t *k,
  *   any outer strides, unit innermost stride; P and Ls may be 0; D <= 512.
  *   lens: int32 [B] on the device, len_b = lens[b] clamped to 0 .. Ls; NULL: Ls.
  *   A query that sees no key gives zeros. Own keys at or past len_b are never
- *   read.
+ *   read; those before it that causality hides from a query have to hold finite
+ *   values (they are read beside those it sees, with a probability of zero).
  *   workspace: contiguous f32, 16-byte aligned, of at least
  *   lux3d_sdpa_shared_prefix_workspace(B, H, Hkv, Lq, P, Ls, D) values (0: may
  *   be NULL); its contents do not matter and it holds nothing between calls, but
  *   no two calls that may overlap share one.
- * D = 64 or 128 of a 2-byte type with every row 16-byte aligned runs on the
- * matrix cores (f32 scores, softmax and sums, probabilities rounded to the type,
- * one rounding of the output, as lux3d_sdpa); other cases run a generic kernel in
- * f32 throughout. One or two kernels. out must not overlap an input. The
+ * D = 64 or 128 with every row 16-byte aligned runs on the matrix cores with
+ * lux3d_sdpa's arithmetic (2-byte types: f32 scores, softmax and sums,
+ * probabilities rounded to the type, one rounding of the output; f32: q, k, v and
+ * the probabilities as three bf16 terms each); other cases run a generic kernel
+ * in f32 throughout. One or two kernels. out must not overlap an input. The
  * reference attends to one sequence a call (exact_query_chunked_sdpa,
  * runtime/attention_math.rs:199-241, without a cache): this is the form of
  * several samples or frames behind one context.                             */
