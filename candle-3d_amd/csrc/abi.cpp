@@ -1013,7 +1013,6 @@ int lux3d_q8_0_linear_adapters(const lux3d_tensor_t *x, const lux3d_tensor_t *qs
   d.a = a->data; d.b = b->data; d.t = t->data;
   d.ids = reinterpret_cast<const int32_t *>(adapter_ids->data);
   d.n = (int)na; d.r = (int)rank;
-  d.b_vec = aligned16(b->data) && rank * elem_bytes(b->dtype) % 16 == 0;
   dp.ad = d;
   dp.x = p.x; dp.ldx = p.ldx; dp.M = p.M; dp.K = p.K;
   if (p.M == 0 || p.N == 0) return ok();

@@ -1,10 +1,13 @@
 // adapters.hip -- the first product of the low-rank adapters beside a Q8_0 linear: t = alpha x A^T for rows whose
-// segment has an adapter (the second, t B^T, is added in the GEMM's epilogue, adapters.hpp).
+// segment has an adapter (the second, t B^T, joins the GEMM's accumulators, adapters.hpp).
 //
-// x's bytes bound it, or for few rows A's. A workgroup takes 16 rows of one segment and 16 NT values of the rank; its
-// wavefronts take 64-deep chunks of k in turn and their sums are added in wavefront order through LDS
-// (v_mfma_f32_16x16x32_bf16, f32 sums; f32 x: v_mfma_f32_16x16x4_f32). t is rounded once to x's type, as an activation
-// between two linear layers is.
+// What bounds it: x's bytes, or for few rows the latency of one load after the other. A workgroup takes 16 rows of one
+// segment and 16 NT values of the rank; its wavefronts take 128-byte chunks of the rows in turn and their sums are added in
+// wavefront order through LDS (v_mfma_f32_16x16x32_bf16, f32 sums; f32 x: v_mfma_f32_16x16x4_f32). A chunk goes through
+// LDS, 8 lanes to a row: loaded as the matrix operand's lanes hold it, a row a lane, the cache serves 16 bytes a cycle.
+// us, operand loads / through LDS: 4096 x 2048 rank 64 bf16 15.4 / 9.7, 3087 x 4096 rank 32 f32 26 / 18, 9001 x 1536 rank
+// 12 bf16 11.0 / 8.1, 12 x 1536 rank 16 5.0 / 4.4 (50 MB of f32 x: 10.4 us at the copy rate). t is rounded once to x's
+// type, as an activation between two linear layers is.
 #include "adapters.hpp"
 
 namespace lux3d {
@@ -13,44 +16,49 @@ namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// Tile `tile` of 16 rows within segments: its segment and first row, or s = nseg past the last one. Every lane of the
-// wavefront calls it; lanes take one segment each.
+// Tile `tile` of 16 rows within segments: its first row, the segment's end and adapter; id -1 past the last
+// tile, too. Every lane of the wavefront calls it; lanes take one segment each.
 struct AdapterTile {
-  int64_t s, row;
+  int64_t row, end;
+  int id;
 };
 __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams &d, int64_t rows, int64_t tile) {
   const int lane = threadIdx.x & 63;
   int64_t before = 0;
   for (int64_t s0 = 0; s0 < d.nseg; s0 += 64) {
     const int64_t s = s0 + lane, a = adapter_row(d, rows, s), b = s < d.nseg ? adapter_row(d, rows, s + 1) : a;
-    int64_t n = b > a ? (b - a + 15) / 16 : 0, sum = n;
-    if (s >= d.nseg) sum = n = 0;
+    const int id = adapter_id(d, s < d.nseg ? s : d.nseg - 1);
+    // tiles of the segment and of those up to it; below 2^31 both, as rows / 16
+    const int n = b > a ? (int)((b - a + 15) / 16) : 0;
+    int sum = n;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-      const int64_t o = __shfl_up(sum, m, 64);
+      const int o = __shfl_up(sum, m, 64);
       if (lane >= m) sum += o;
     }
     // the first segment whose tiles reach past `tile`
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > tile);
     if (past) {
       const int at = __builtin_ctzll(past);
-      const int64_t first = before + __shfl(sum, at, 64) - __shfl(n, at, 64);
-      return {uniform(s0 + at), uniform(__shfl(a, at, 64) + (tile - first) * 16)};
+      const int64_t first = before + __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(n, at);
+      return {uniform(__shfl(a, at, 64) + (tile - first) * 16), uniform(__shfl(b, at, 64)),
+              __builtin_amdgcn_readlane(id, at)};
     }
-    before += uniform(__shfl(sum, 63, 64));
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
-  return {d.nseg, 0};
+  return {0, 0, -1};
 }
 
 template <bool XF32, int NT, int NW>
 __global__ __launch_bounds__(64 * NW) void adapter_down_kernel(AdapterDownParams p) {
   constexpr int EB = XF32 ? 4 : 2;
-  __shared__ float part[NW][NT * 256];
+  constexpr int ROWS = 16 * (1 + NT), LD = ROWS / 8;  // rows of a chunk, x's and A's; its 1 KB loads
+  __shared__ __align__(16) char lds[NW][ROWS * 128];
   const AdapterParams &d = p.ad;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, l16 = lane & 15;
   const int j0 = (int)blockIdx.y * 16 * NT;
-  if (p.bad && blockIdx.x == 0 && blockIdx.y == 0 && wave == 0) {
-    // segments whose id is neither -1 nor an adapter's
+  if (p.bad && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && wave == 0) {
+    // segments whose id is neither -1 nor an adapter's; by the last workgroup, which seldom has a tile
     int bad = 0;
     for (int64_t s = lane; s < d.nseg; s += 64) bad += d.ids[s] < -1 || d.ids[s] >= d.n;
 #pragma unroll
@@ -58,102 +66,120 @@ __global__ __launch_bounds__(64 * NW) void adapter_down_kernel(AdapterDownParams
     if (lane == 0) *p.bad = bad;
   }
   const AdapterTile w = adapter_tile(d, p.M, blockIdx.x);
-  if (w.s >= d.nseg) return;  // uniform over the workgroup, as all that follows
-  const int id = __builtin_amdgcn_readfirstlane(adapter_id(d, w.s));
-  if (id < 0) return;
-  const int64_t end = uniform(adapter_row(d, p.M, w.s + 1));
-  // rows past the segment are clamped: loaded, computed, never stored; so are values past the rank
-  const int64_t row = w.row + l16 < end ? w.row + l16 : end - 1;
-  const char *xr = reinterpret_cast<const char *>(p.x) + row * p.ldx * EB;
-  const char *ar[NT];
+  if (w.id < 0) return;  // uniform over the workgroup
+  const float alpha = d.alpha ? d.alpha[w.id] : 1.f;
+  // load i: rows 8 i .. + 7, a lane 16 bytes: piece `piece` of row 8 i + lane / 8, kept in slot lane % 8. Rows past the
+  // segment are clamped: loaded, computed, never stored; so are values past the rank.
+  const int piece = (lane & 7) ^ (lane >> 3);
+  const char *src[LD];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int j = j0 + 16 * n + l16;
-    ar[n] = reinterpret_cast<const char *>(d.a) + ((int64_t)id * d.r + (j < d.r ? j : d.r - 1)) * p.K * EB;
+  for (int i = 0; i < LD; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    if (i < 2) {
+      const int64_t row = w.row + r < w.end ? w.row + r : w.end - 1;
+      src[i] = reinterpret_cast<const char *>(p.x) + row * p.ldx * EB + piece * 16;
+    } else {
+      const int j = j0 + r - 16 < d.r ? j0 + r - 16 : d.r - 1;
+      src[i] = reinterpret_cast<const char *>(d.a) + ((int64_t)w.id * d.r + j) * p.K * EB + piece * 16;
+    }
   }
   f32x4_t acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = f32x4_t{};
-  // chunk c: values 64 c .. + 63; lane group g holds 16 g .. + 15 of them on both operands
-  const int64_t nch = p.K / 64;
+  char *const my = lds[wave];
+  uint4 v[LD];
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) v[i] = ld16<false>(src[i] + at);
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) *reinterpret_cast<uint4 *>(my + i * 1024 + lane * 16) = v[i];
+    // the wavefront's own memory: its reads follow its writes in order, and only the compiler has to know
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  // half q of the chunk: piece 4 q + g of the lane's row on both operands
+  auto products = [&](int q) {
+    const int off = l16 * 128 + (((4 * q + g) ^ (l16 & 7)) << 4);
+    const uint4 x = *reinterpret_cast<const uint4 *>(my + off);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint4 a = *reinterpret_cast<const uint4 *>(my + (1 + n) * 2048 + off);
+      if constexpr (!XF32) {
+        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8_t, x), __builtin_bit_cast(ad_bf16x8_t, a),
+                                                         acc[n], 0, 0, 0);
+      } else {
+        const f32x4_t xv = __builtin_bit_cast(f32x4_t, x), av = __builtin_bit_cast(f32x4_t, a);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[e], av[e], acc[n], 0, 0, 0);
+      }
+    }
+  };
+  const int64_t bytes = p.K * EB, nch = bytes / 128;  // chunks of 128 bytes a row
+  if (wave < nch) load(wave * 128);
   for (int64_t c = wave; c < nch; c += NW) {
-    if constexpr (!XF32) {
-      const int64_t at = (c * 64 + 16 * g) * 2;
-      const uint4 x0 = ld16<false>(xr + at), x1 = ld16<false>(xr + at + 16);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 a0 = ld16<false>(ar[n] + at), a1 = ld16<false>(ar[n] + at + 16);
-        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8_t, x0), __builtin_bit_cast(ad_bf16x8_t, a0), acc[n], 0, 0, 0);
-        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8_t, x1), __builtin_bit_cast(ad_bf16x8_t, a1), acc[n], 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t at = (c * 64 + 16 * g + 4 * q) * 4;
-        const float4 x = *reinterpret_cast<const float4 *>(xr + at);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float4 a = *reinterpret_cast<const float4 *>(ar[n] + at);
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, a.x, acc[n], 0, 0, 0);
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, a.y, acc[n], 0, 0, 0);
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, a.z, acc[n], 0, 0, 0);
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, a.w, acc[n], 0, 0, 0);
-        }
-      }
-    }
+    store();
+    if (c + NW < nch) load((c + NW) * 128);
+    products(0);
+    products(1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
-  if (p.K % 64 && wave == (int)(nch % NW)) {
-    // the last 32 values (bf16 alone): 8 a lane group
-    const int64_t at = (nch * 64 + 8 * g) * 2;
-    if constexpr (!XF32) {
-      const uint4 x0 = ld16<false>(xr + at);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 a0 = ld16<false>(ar[n] + at);
-        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8_t, x0), __builtin_bit_cast(ad_bf16x8_t, a0), acc[n], 0, 0, 0);
-      }
-    }
+  if (bytes % 128 && wave == (int)(nch % NW)) {
+    // the last 64 bytes; pieces 4 to 7 load what 0 to 3 do
+    load(nch * 128 - (piece & 4) * 16);
+    store();
+    products(0);
   }
+  __syncthreads();
   // lane holds rows 4 g + e, rank value lane % 16 of each tile
+  float *const part = reinterpret_cast<float *>(lds);
+  static_assert(NT * 1024 <= ROWS * 128, "partial sums fit");
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][n * 256 + e * 64 + lane] = acc[n][e];
+    for (int e = 0; e < 4; ++e) part[wave * NT * 256 + n * 256 + e * 64 + lane] = acc[n][e];
   __syncthreads();
-  const float alpha = d.alpha ? d.alpha[id] : 1.f;
   for (int o = t; o < NT * 256; o += 64 * NW) {
     const int64_t r = w.row + 4 * ((o & 63) >> 4) + (o >> 6 & 3);
     const int j = j0 + (o >> 8) * 16 + (o & 15);
-    if (r >= end || j >= d.tp) continue;
-    float v = part[0][o];
+    if (r >= w.end || j >= d.tp) continue;
+    float s = part[o];
 #pragma unroll
-    for (int k = 1; k < NW; ++k) v += part[k][o];
-    v = j < d.r ? v * alpha : 0.f;
-    if constexpr (XF32) reinterpret_cast<float *>(d.t)[r * d.tp + j] = v;
-    else store1<BF16>(d.t, r * d.tp + j, v);
+    for (int k = 1; k < NW; ++k) s += part[k * NT * 256 + o];
+    s = j < d.r ? s * alpha : 0.f;
+    constexpr int E = 16 / EB;
+    int next;
+    char *to = adapter_t<EB>(d, p.M, r, j & -E, next);
+    store1<std::conditional_t<XF32, F32, BF16>>(to, j & (E - 1), s);
   }
 }
 
-template <bool XF32>
+template <bool XF32, int NT, int NW>
 hipError_t launch_down(const AdapterDownParams &p, hipStream_t s) {
-  const AdapterParams &d = p.ad;
   // at most one partly filled tile a segment
-  int64_t tiles = p.M / 16 + d.nseg;
+  int64_t tiles = p.M / 16 + p.ad.nseg;
   tiles = tiles < p.M ? tiles : p.M;
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
-  const int nt = d.tp <= 16 ? 1 : d.tp <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)tiles, (unsigned)((d.tp + 16 * nt - 1) / (16 * nt)));
-  if (nt == 1) hipLaunchKernelGGL((adapter_down_kernel<XF32, 1, 8>), grid, dim3(512), 0, s, p);
-  else if (nt == 2) hipLaunchKernelGGL((adapter_down_kernel<XF32, 2, 8>), grid, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((adapter_down_kernel<XF32, 4, 8>), grid, dim3(512), 0, s, p);
+  if (p.M > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)tiles, (unsigned)((p.ad.tp + 16 * NT - 1) / (16 * NT)));
+  hipLaunchKernelGGL((adapter_down_kernel<XF32, NT, NW>), grid, dim3(64 * NW), 0, s, p);
   return hipGetLastError();
+}
+
+template <bool XF32, int NT>
+hipError_t launch_down(const AdapterDownParams &p, hipStream_t s) {
+  // us with 4 / 8 wavefronts: 9001 rows of 1536 8.1 / 9.0, 4096 of 2048 10.1 / 9.7, 3087 of 4096 in f32 20.1 / 18.0
+  return p.M > 8192 ? launch_down<XF32, NT, 4>(p, s) : launch_down<XF32, NT, 8>(p, s);
 }
 
 }  // namespace
 
 hipError_t launch_adapter_down(const AdapterDownParams &p, bool x_f32, hipStream_t s) {
   if (p.M <= 0) return hipSuccess;
-  return x_f32 ? launch_down<true>(p, s) : launch_down<false>(p, s);
+  if (p.ad.tp <= 16) return x_f32 ? launch_down<true, 1>(p, s) : launch_down<false, 1>(p, s);
+  if (p.ad.tp <= 32) return x_f32 ? launch_down<true, 2>(p, s) : launch_down<false, 2>(p, s);
+  return x_f32 ? launch_down<true, 4>(p, s) : launch_down<false, 4>(p, s);
 }
 
 }  // namespace lux3d

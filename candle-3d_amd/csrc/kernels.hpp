@@ -130,7 +130,7 @@ hipError_t launch_dequant_q8_0(const uint8_t *blocks, int64_t nblocks, int out_d
 // ---- low-rank adapters beside a linear (adapters.hip, adapters.hpp) -------------
 // Rows of segment s take adapter ids[s] (none outside 0 .. n - 1): y += t B^T, t
 // = alpha x A^T, in x's type. a [n, r, K], b [n, N, r], t [M, tp], tp = r
-// rounded up to 16; b_vec: B's rows are 16-byte aligned.
+// rounded up to 16.
 struct AdapterParams {
   const void *a = nullptr, *b = nullptr;
   const float *alpha = nullptr;      // [n] or null
@@ -138,7 +138,6 @@ struct AdapterParams {
   const int64_t *seg_off = nullptr;  // [nseg + 1] or null: equal segments
   int64_t nseg = 0, rows_per_seg = 1;
   int n = 0, r = 0, tp = 0;
-  bool b_vec = false;
   void *t = nullptr;
 };
 struct AdapterDownParams {

@@ -344,6 +344,10 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
   // for data again, so the wait counts are the same every step.
 #pragma unroll
   for (int st = 0; st < NS - 1; ++st) issue(st < nk ? st : nk - 1, st);
+  if constexpr (AD) {
+    adapter_add<false, TM, 1>(p.ad, p.M, p.N, m0, c0 + wave * 32, acc);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm((NS - 2) * kRingOps));  // stage 0 landed
   __builtin_amdgcn_s_barrier();
 
@@ -381,7 +385,6 @@ __global__ __launch_bounds__(64 * NW, 1) void q8_0_gemm_ring_kernel(Q8GemmParams
     __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads and reads
-  if constexpr (AD) adapter_add<false, TM, 1>(p.ad, p.M, p.N, m0, c0 + wave * 32, acc);
 
   char *ybase = reinterpret_cast<char *>(p.y);
   const float bias = (p.bias && ncol < p.N) ? p.bias[ncol] : 0.f;
@@ -623,6 +626,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8Ge
 
 #pragma unroll
   for (int s2 = 0; s2 < NS - 1; ++s2) issue(s2, s2);
+  if constexpr (AD) {
+    if (kg == 0) adapter_add<true, TI, TJ>(p.ad, p.M, p.N, m0 + wm * TI * 32, c0 + wn * TJ * 32, acc);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm((NS - 2) * T::OPS));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
@@ -670,7 +677,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8Ge
     __syncthreads();
     if (kg > 0) return;
   }
-  if constexpr (AD) adapter_add<true, TI, TJ>(p.ad, p.M, p.N, m0 + wm * TI * 32, c0 + wn * TJ * 32, acc);
 
   // epilogue: each wavefront's 32 TI x 32 TJ block through LDS, bias added, one
   // rounding, 16-byte row pieces
@@ -860,7 +866,7 @@ __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_kernel(Q8GemmParams p) 
     float v = part[0][o];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += part[w][o];
-    if constexpr (AD) v += adapter_dot<XF32>(p.ad, p.N, row, col);
+    if constexpr (AD) v += adapter_dot<XF32>(p.ad, p.M, p.N, row, col);
     store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
   }
 }
