@@ -461,8 +461,8 @@ def q8_0_linear_adapters(x: torch.Tensor, qs: torch.Tensor, scales: torch.Tensor
     if a.dim() != 3 or x.dim() < 1 or x.shape[-1] == 0:
         raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "a must be [adapters, rank, k], x [..., k]")
     with _device_of(x):
-        y = torch.empty(tuple(x.shape[:-1]) + (qs.shape[0],), dtype=out_dtype, device=x.device)
-        t = torch.empty((x.numel() // x.shape[-1], (a.shape[1] + 15) // 16 * 16), dtype=x.dtype, device=x.device)
+        y = x.new_empty((*x.shape[:-1], qs.shape[0]), dtype=out_dtype)
+        t = x.new_empty((x.numel() // x.shape[-1], (a.shape[1] + 15) // 16 * 16))
         _lib.call(fn, _d(x), _d(qs), _d(scales), _d(bias), _d(a), _d(b), _d(alphas), _d(adapter_ids), _d(seg_offsets),
                   _d(t), _d(bad_ids), _d(y), _stream(x))
     return y
@@ -553,7 +553,7 @@ def sdpa_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
         b, h, n, d = q.shape
         hkv, p, _ = prefix_k.shape
         size = _lib.LIB.lux3d_sdpa_shared_prefix_workspace(b, h, hkv, n, p, k.shape[2], d)
-        ws = torch.empty(size, dtype=torch.float32, device=q.device) if size else None
+        ws = q.new_empty(size, dtype=torch.float32) if size else None
         _lib.call(fn, _d(q), _d(prefix_k), _d(prefix_v), _d(k), _d(v), _d(lens), 1 if causal else 0, float(scale), _d(ws),
                   _d(out), _stream(q))
     return out
