@@ -14,7 +14,7 @@
 // [N, K/32], so the GEMM streams them with 16-byte loads.
 //
 // Four GEMM kernels (each one rounding of the f32 sum per output):
-// - q8_0_few_rows_kernel and q8_0_16_rows_kernel (K % 64 == 0, up to 16 rows or few tiles): workgroups of
+// - q8_0_few_rows_kernel and q8_0_few_rows_lds_kernel (K % 64 == 0, up to 16 rows or few tiles): workgroups of
 //   16 weight rows whose wavefronts split k.
 // - q8_0_gemm_ring_kernel (K % 64 == 0, the common case): a workgroup of NW
 //   wavefronts (8, or 4 for small shapes) computes a BM x 32 NW tile (BM 32 to
@@ -871,22 +871,24 @@ __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_kernel(Q8GemmParams p) 
   }
 }
 
-// The form for tiles of 16 rows and K from 512 on: the same sums in the same order. A lane a row, as the matrix instruction
-// holds its operands, the cache serves one lane's bytes a cycle, so that weights, scales and x here go through LDS, each
-// row's chunk loaded by neighbouring lanes; each wavefront has LDS of its own. us, operand loads / through LDS, bf16 and f32:
-// M 1, K 1536 -> N 9216 7.3 / 6.3 and 9.9 / 9.8; M 16 10.2 / 6.5 and 15.5 / 10.0; M 16, K 4096 -> N 1024 9.2 / 5.7 and 14.7
-// / 8.5; M 4, K 8192 -> N 2048 12.4 / 9.2 and 19.7 / 14.5; M 3, K 1536 -> N 1536 4.1 / 3.6 and 5.3 / 5.1; but M 1, K 320
-// -> N 4096 2.6 / 2.7 and 3.2 / 3.5.
-template <typename OUT, bool XF32, int NW, bool AD>
-__global__ __launch_bounds__(64 * NW) void q8_0_16_rows_kernel(Q8GemmParams p) {
+// The form for K from 512 on: the same sums in the same order. A lane a row, as the matrix instruction holds its operands,
+// the cache serves one lane's bytes a cycle, so that weights, scales and x here go through LDS, each row's chunk loaded by
+// neighbouring lanes; each wavefront has LDS of its own, and loads a chunk's successor as soon as the chunk is there (MT 1:
+// two chunks together, 4 to 10% faster there). us, operand loads / through LDS, bf16 and f32: M 1, K 1536 -> N 9216 7.3 /
+// 6.3 and 9.9 / 9.5; M 16 10.2 / 6.5 and 15.5 / 9.7; M 4, K 8192 -> N 2048 12.4 / 9.9 and 19.7 / 14.5; M 3, K 1536 -> N
+// 1536 4.1 / 3.6 and 5.3 / 5.0; with two row tiles for four: M 64, K 8192 -> N 2048 37.9 / 13.2 and 69.6 / 25.4; M 61, K
+// 1536 -> N 1536 8.9 / 4.7 and 14.4 / 7.0; M 2000, K 2048 -> N 16 11.1 / 5.0 and 19.2 / 7.7; but M 1, K 320 -> N 4096 2.6 /
+// 2.7 and 3.2 / 3.5.
+template <typename OUT, bool XF32, int NW, int MT, bool AD>
+__global__ __launch_bounds__(64 * NW) void q8_0_few_rows_lds_kernel(Q8GemmParams p) {
   typedef float f32x4_t __attribute__((ext_vector_type(4)));
-  constexpr int EB = XF32 ? 4 : 2, XL = EB;                       // 1 KB loads of x's chunk
-  constexpr int P = 2;                                            // chunks a turn: 4 and 6 of them are slower, as fewer wavefronts fit
+  constexpr int EB = XF32 ? 4 : 2, XL = EB * MT;                   // 1 KB loads of x's chunk
+  constexpr int P = MT == 1 ? 2 : 1;                               // chunks whose loads go together: with 4 or 6 fewer wavefronts fit
   constexpr int XB = 1024, SB = XB + XL * 1024, BYTES = SB + 128;  // a chunk in LDS: weights, x, scales
+  constexpr int OUTS = MT * 256 / (64 * NW) > 0 ? MT * 256 / (64 * NW) : 1;
   __shared__ __align__(16) char lds[NW][BYTES];
-  __shared__ float part[NW][256];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, l16 = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
   const int64_t nch = p.K / 64;
   // rows past N and M are clamped: loaded, computed, never stored
   auto wrow = [&](int r) { return n0 + r < p.N ? n0 + r : p.N - 1; };
@@ -905,25 +907,18 @@ __global__ __launch_bounds__(64 * NW) void q8_0_16_rows_kernel(Q8GemmParams p) {
   char *const wto = my + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
   uint4 w[P], x[P][XL];
   float d[P];
-  auto chunk = [&](int64_t c0, int u) { return c0 + (int64_t)(u / 2) * 2 * NW + (u & 1); };
-  auto load = [&](int64_t c0) {
+  auto load = [&](int u, int64_t c) {
+    w[u] = ld16<false>(wsrc + c * 64);
+    d[u] = ssrc[c * 2];
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const int64_t c = chunk(c0, u) < nch ? chunk(c0, u) : c0;
-      w[u] = ld16<false>(wsrc + c * 64);
-      d[u] = ssrc[c * 2];
-#pragma unroll
-      for (int i = 0; i < XL; ++i) x[u][i] = ld16<false>(xsrc[i] + c * 64 * EB);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // the compiler would issue them just before their products
+    for (int i = 0; i < XL; ++i) x[u][i] = ld16<false>(xsrc[i] + c * 64 * EB);
   };
   auto fence = [&]() {
     // the wavefront's own memory: its LDS operations keep their order, and only the compiler has to know
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  f32x4_t acc = {};
-  auto products = [&](int u) {
+  auto store = [&](int u) {
     *reinterpret_cast<uint4 *>(wto) = w[u];
     if (lane < 32) *reinterpret_cast<float *>(my + SB + lane * 4) = d[u];
 #pragma unroll
@@ -932,90 +927,129 @@ __global__ __launch_bounds__(64 * NW) void q8_0_16_rows_kernel(Q8GemmParams p) {
       *reinterpret_cast<uint4 *>(my + XB + r * 64 * EB + (((lane % PX) ^ (r & (PX - 1))) << 4)) = x[u][i];
     }
     fence();
-    auto x16 = [&](int piece) { return *reinterpret_cast<const uint4 *>(my + XB + l16 * 64 * EB + ((piece ^ (l16 & (PX - 1))) << 4)); };
+  };
+  f32x4_t acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4_t{};
+  auto products = [&]() {
+    auto x16 = [&](int i, int piece) {
+      return *reinterpret_cast<const uint4 *>(my + XB + (16 * i + l16) * 64 * EB + ((piece ^ (l16 & (PX - 1))) << 4));
+    };
     const char *const wr = my + l16 * 64;
     if constexpr (!XF32) {
       const uint4 q = *reinterpret_cast<const uint4 *>(wr + ((g ^ (l16 >> 2)) << 4));
       const float dq = *reinterpret_cast<const float *>(my + SB + l16 * 8 + (g >> 1) * 4);
-      const uint4 x0 = x16(2 * g), x1 = x16(2 * g + 1);
       const bf16x8_t b0 = dequant8(q.x, q.y, dq), b1 = dequant8(q.z, q.w, dq);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x0), b0, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x1), b1, acc, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x16(i, 2 * g)), b0, acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x16(i, 2 * g + 1)), b1, acc[i], 0, 0, 0);
+      }
     } else {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const uint2 q2 = *reinterpret_cast<const uint2 *>(wr + (((2 * b + (g >> 1)) ^ (l16 >> 2)) << 4) + (g & 1) * 8);
         const float dq = *reinterpret_cast<const float *>(my + SB + l16 * 8 + b * 4);
-        const uint4 xa = x16(8 * b + 2 * g), xb = x16(8 * b + 2 * g + 1);
-        const float xv[8] = {__uint_as_float(xa.x), __uint_as_float(xa.y), __uint_as_float(xa.z), __uint_as_float(xa.w),
-                             __uint_as_float(xb.x), __uint_as_float(xb.y), __uint_as_float(xb.z), __uint_as_float(xb.w)};
         const bf16x8_t q = dequant8(q2.x, q2.y, 1.f);
-        u32x4_t x1, x2, x3;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const Split3 r = split3_bf16(xv[2 * e], xv[2 * e + 1]);
-          x1[e] = r.t1;
-          x2[e] = r.t2;
-          x3[e] = r.t3;
+        for (int i = 0; i < MT; ++i) {
+          const uint4 xa = x16(i, 8 * b + 2 * g), xb = x16(i, 8 * b + 2 * g + 1);
+          const uint32_t xv[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
+          u32x4_t x1, x2, x3;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const Split3 r = split3_bf16(__uint_as_float(xv[2 * e]), __uint_as_float(xv[2 * e + 1]));
+            x1[e] = r.t1;
+            x2[e] = r.t2;
+            x3[e] = r.t3;
+          }
+          f32x4_t blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x3), q, f32x4_t{}, 0, 0, 0);
+          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x2), q, blk, 0, 0, 0);
+          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x1), q, blk, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(blk[e], dq, acc[i][e]);
         }
-        f32x4_t blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x3), q, f32x4_t{}, 0, 0, 0);
-        blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x2), q, blk, 0, 0, 0);
-        blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x1), q, blk, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(blk[e], dq, acc[e]);
       }
     }
     fence();
   };
-  // lane holds rows 4 g + e, column lane % 16 of the tile
-  const int64_t row = m0 + 4 * ((t & 63) >> 4) + (t >> 6 & 3), col = n0 + (t & 15);
-  const bool out = t < 256 && row < p.M && col < p.N;
-  float extra = 0.f;
-  int64_t c0 = 2 * wave;
-  if (c0 < nch) load(c0);
-  if constexpr (AD) {
-    if (out) extra = adapter_dot<XF32>(p.ad, p.M, p.N, row, col);  // while the first loads arrive
-  }
-  for (; c0 < nch; c0 += P * NW) {
-    if (c0 > 2 * wave) load(c0);
+  // the wavefront's chunks: 2 wave, 2 wave + 1, then 2 NW further
+  const int64_t begin = 2 * wave;
+  auto pair = [&](int64_t c) {  // past the last: the one before again, not used
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      if (chunk(c0, u) >= nch) break;  // uniform
-      products(u);
+    for (int u = 0; u < P; ++u) load(u, c + u < nch ? c + u : c);
+    __builtin_amdgcn_sched_barrier(0);  // the compiler would issue them just before their products
+  };
+  auto after = [&](int64_t c) { return (c & 1) ? c + 2 * NW - 1 : c + 1; };
+  if (begin < nch) {
+    if constexpr (MT == 1) pair(begin);
+    else load(0, begin);
+  }
+  if constexpr (AD) adapter_add16<XF32, MT, NW>(p.ad, p.M, p.N, m0, n0, wave, acc);  // while the first loads arrive
+  if constexpr (MT == 1) {
+    for (int64_t c = begin; c < nch; c += 2 * NW) {
+      if (c > begin) pair(c);
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        if (c + u >= nch) break;  // uniform
+        store(u);
+        products();
+      }
+    }
+  } else {
+    for (int64_t c = begin; c < nch; c = after(c)) {
+      store(0);
+      if (after(c) < nch) load(0, after(c));
+      products();
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) part[wave][e * 64 + lane] = acc[e];
+  // lane holds rows 4 g + e, column lane % 16 of each tile
   __syncthreads();
-  if (!out) return;
-  float v = part[0][t];
+  float *const part = reinterpret_cast<float *>(lds);
+  static_assert(MT * 1024 <= BYTES, "partial sums fit");
 #pragma unroll
-  for (int k = 1; k < NW; ++k) v += part[k][t];
-  if constexpr (AD) v += extra;
-  store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave * MT * 256 + i * 256 + e * 64 + lane] = acc[i][e];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < OUTS; ++n) {
+    const int o = t + n * 64 * NW;
+    if (o >= MT * 256) return;
+    const int64_t row = m0 + o / 256 * 16 + 4 * ((o & 63) >> 4) + (o >> 6 & 3), col = n0 + (o & 15);
+    if (row >= p.M || col >= p.N) continue;
+    float v = part[o];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) v += part[k * MT * 256 + o];
+    store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
+  }
 }
 
-template <typename OUT, bool XF32, int NW, int MT, bool AD>
-hipError_t launch_few_rows_of(const Q8GemmParams &p, dim3 grid, hipStream_t s) {
-  if constexpr (MT == 1) {
-    if (NW > 4 || p.K >= 512) {
-      hipLaunchKernelGGL((q8_0_16_rows_kernel<OUT, XF32, NW, AD>), grid, dim3(64 * NW), 0, s, p);
-      return hipGetLastError();
-    }
+// Rows of 16 MT a workgroup by operand loads, 16 ML through LDS.
+template <typename OUT, bool XF32, int NW, int MT, int ML, bool AD>
+hipError_t launch_few_rows_of(const Q8GemmParams &p, hipStream_t s) {
+  const auto grid = [&](int mt) { return dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * mt - 1) / (16 * mt))); };
+  if (NW > 4 || (p.K >= 512 && grid(ML).y <= 65535)) {  // more than 4 wavefronts: K past 512, few tiles
+    hipLaunchKernelGGL((q8_0_few_rows_lds_kernel<OUT, XF32, NW, ML, AD>), grid(ML), dim3(64 * NW), 0, s, p);
+  } else if constexpr (NW == 4) {
+    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, NW, MT, AD>), grid(MT), dim3(64 * NW), 0, s, p);
   }
-  if constexpr (MT > 1 || NW == 4) hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, NW, MT, AD>), grid, dim3(64 * NW), 0, s, p);
   return hipGetLastError();
 }
 
-template <typename OUT, bool XF32, int MT, bool AD>
+template <typename OUT, bool XF32, int MT, int ML, bool AD>
 hipError_t launch_few_rows(const Q8GemmParams &p, hipStream_t s) {
   // 2048 wavefronts (two per SIMD), or as many as k has chunk pairs
   const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * MT - 1) / (16 * MT);
   if (tn > INT32_MAX || tm > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)tn, (unsigned)tm);
-  if (tn * tm * 4 >= 2048 || p.K <= 512) return launch_few_rows_of<OUT, XF32, 4, MT, AD>(p, grid, s);
-  if (tn * tm * 8 >= 2048 || p.K <= 1024) return launch_few_rows_of<OUT, XF32, 8, MT, AD>(p, grid, s);
-  return launch_few_rows_of<OUT, XF32, 16, MT, AD>(p, grid, s);
+  if (tn * tm * 4 >= 2048 || p.K <= 512) return launch_few_rows_of<OUT, XF32, 4, MT, ML, AD>(p, s);
+  if (tn * tm * 8 >= 2048 || p.K <= 1024) return launch_few_rows_of<OUT, XF32, 8, MT, ML, AD>(p, s);
+  return launch_few_rows_of<OUT, XF32, 16, MT, ML, AD>(p, s);
+}
+template <typename OUT, bool XF32, bool AD>
+hipError_t launch_few_rows(const Q8GemmParams &p, int rows, hipStream_t s) {
+  if (rows == 16) return launch_few_rows<OUT, XF32, 1, 1, AD>(p, s);
+  return launch_few_rows<OUT, XF32, 4, 2, AD>(p, s);
 }
 
 template <typename OUT, bool AD, int WM, int WN, int TI, int TJ, int KG>
@@ -1031,7 +1065,7 @@ hipError_t launch_x3(const Q8GemmParams &p, hipStream_t s) {
 template <typename OUT, bool AD>
 hipError_t launch_f32(const Q8GemmParams &p, hipStream_t s) {
   const Q8Tile tile = q8_tile_f32(p.M, p.N, p.K);
-  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, true, 1, AD>(p, s) : launch_few_rows<OUT, true, 4, AD>(p, s);
+  if (tile.few()) return launch_few_rows<OUT, true, AD>(p, tile.rows, s);
   if (tile.rows == 128) return launch_x3<OUT, AD, 2, 4, 2, 2, 1>(p, s);
   if (tile.rows == 32) return launch_x3<OUT, AD, 1, 4, 1, 1, 3>(p, s);
   return tile.groups == 1 ? launch_x3<OUT, AD, 2, 2, 1, 2, 1>(p, s) : launch_x3<OUT, AD, 2, 2, 1, 2, 2>(p, s);
@@ -1058,7 +1092,7 @@ hipError_t launch_ring(const Q8GemmParams &p, hipStream_t s) {
 template <typename OUT, bool AD>
 hipError_t launch_bf16(const Q8GemmParams &p, hipStream_t s) {
   const Q8Tile tile = q8_tile_bf16(p.M, p.N, p.K);
-  if (tile.few()) return tile.rows == 16 ? launch_few_rows<OUT, false, 1, AD>(p, s) : launch_few_rows<OUT, false, 4, AD>(p, s);
+  if (tile.few()) return launch_few_rows<OUT, false, AD>(p, tile.rows, s);
   if (tile.cols == 256) return tile.rows == 256 ? launch_ring<OUT, AD, 256, 8>(p, s) : launch_ring<OUT, AD, 128, 8>(p, s);
   switch (tile.rows) {
     case 32: return launch_ring<OUT, AD, 32, 4>(p, s);

@@ -173,6 +173,24 @@ def test_neighbours_do_not_leak(ops, dev, m):
     assert torch.equal(z[keep], y[keep]) and torch.isnan(z[cuts[1]:cuts[2]]).all()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k,n", [(9, 512, 160), (30, 512, 160), (60, 64, 200), (61, 1024, 1536), (300, 512, 1000), (700, 512, 4096),
+                                   (2500, 512, 2048)])
+def test_an_adapter_that_is_not_finite_stays_with_its_rows(ops, dev, m, k, n, dt):
+    """Segments of a few rows, several in every tile of rows; every other one's adapter becomes NaN."""
+    cuts, at = [0], 0
+    while at < m:
+        at = min(m, at + (1, 3, 7, 2, 20)[len(cuts) % 5])
+        cuts.append(at)
+    ids = [(0, 1, 2, -1)[i % 4] for i in range(len(cuts) - 1)]
+    c, ids_t, offs, y = run(ops, dev, m, k, n, 20, dt, cuts, ids)
+    c["a"][1], c["b"][1] = float("nan"), float("inf")
+    z = ops.q8_0_linear_adapters(c["x"], c["qs"], c["scales"], c["a"], c["b"], ids_t, alphas=c["alphas"], seg_offsets=offs,
+                                 bias=c["bias"], out_dtype=DT[dt])
+    hit = (torch.tensor(ids)[segment_of_rows(offs, m, len(ids))] == 1).to(dev)
+    assert torch.equal(z[~hit], y[~hit]) and torch.isnan(z[hit]).all()
+
+
 def test_batches_strided_rows_and_defaults(ops, dev):
     c = make(dev, 6 * 50, 256, 160, 8, 3, "bf16")
     ids = torch.tensor([2, 0, -1], dtype=torch.int32, device=dev)
