@@ -6,7 +6,8 @@
 //   x_out = x + a1 * (h - mean) * rstd + a0,   y = b1 * (x_out - mean') * rstd' + b0
 // with a1 = post_w ls_gamma gate, a0 = post_b ls_gamma gate, b1 = pre_w (scale + 1), b0 = pre_b (scale + 1) + shift.
 // All arithmetic is f32; x_out is rounded once to its type, and y's statistics and values are those of the rounded
-// x_out. Reads x and h and writes x_out and y once: memory bounds it.
+// x_out. Reads x and h and writes x_out and y once: memory bounds it, 64000 x 1536 bf16 at 5.0 TB/s (156 us for 786 MB),
+// 4098 x 2048 f16 at 3.9 TB/s (17.2 us), 1029 x 1024 f32 6.4 us.
 //
 // Statistics take two passes over the registers (the mean, then the centred squares). The row's values and sums are
 // those of rows.hpp.
@@ -305,8 +306,9 @@ hipError_t launch_block_norm_t(const BlockNormParams &p, bool vec, hipStream_t s
   if (p.rows > INT32_MAX) return hipErrorInvalidValue;
   const int64_t chunks = p.d / 8;
   if (vec && p.rows >= 2048 && chunks <= 256) {
-    // two workgroups per CU walk the rows
-    const int64_t wgs = 2 * (int64_t)cu_count(s), per = (p.rows + wgs - 1) / wgs;
+    // Two workgroups per CU walk the rows, three of long jobs. us with 2 / 3 / 4 / a workgroup a row: 4098 x 2048 f16 17.2 /
+    // 18.2 / 20.4 / 28.5, 64000 x 1536 bf16 modulated 162 / 156 / 159 / 249.
+    const int64_t wgs = (p.rows >= 32768 ? 3 : 2) * (int64_t)cu_count(s), per = (p.rows + wgs - 1) / wgs;
     const dim3 grid((unsigned)((p.rows + per - 1) / per));
     const int nc = (int)((chunks + 63) / 64);
     const size_t lds = (size_t)nc * 512 * 16;

@@ -202,6 +202,13 @@ def test_a_row_that_is_not_finite_stays_alone(ops, dev, rows):
     assert torch.isnan(xo[11]).sum() == 1
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_long_jobs(ops, dev, kind):
+    """Enough rows for three workgroups a CU, in segments that end inside a workgroup's run."""
+    offs = torch.tensor([0, 7, 16001, 16002, 33001], device=dev)
+    run_case(ops, dev, 33001, 512, "bf16", kind, offs=offs, base=True)
+
+
 def test_empty_rows(ops, dev):
     run_case(ops, dev, 0, 1024, "bf16", "rms")
 
