@@ -1199,7 +1199,7 @@ int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *pref
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(LUX3D_ERR_VALUE, "%s: scale must be finite and > 0", fn);
   if (p.B == 0 || p.H == 0 || p.Lq == 0) return ok();
   p.G = p.H / p.Hkv;
-  if (p.P > INT32_MAX - 256 || p.Ls > INT32_MAX - 256) return fail(LUX3D_ERR_SHAPE, "%s: more than 2^31 keys", fn);
+  if (p.P > INT32_MAX - 512 || p.Ls > INT32_MAX - 512 - p.P) return fail(LUX3D_ERR_SHAPE, "%s: more than 2^31 keys", fn);
   if (p.Lq > INT32_MAX / p.B / p.G) return fail(LUX3D_ERR_SHAPE, "%s: more than 2^31 query rows a key head", fn);
   p.q = q->data; p.pk = prefix_k->data; p.pv = prefix_v->data; p.k = k->data; p.v = v->data; p.o = out->data;
   p.q_sb = q->stride[0]; p.q_sh = q->stride[1]; p.q_st = q->stride[2];

@@ -32,18 +32,12 @@ __device__ __forceinline__ int adapter_id(const AdapterParams &d, int64_t s) {
   return id >= 0 && id < d.n ? id : -1;
 }
 
-// Segment of `row`, the same for the whole wavefront: as segment_of has it, with one load a lane in place of a search.
+// Segment of `row`, the same for the whole wavefront: as segment_of has it, up to 65 segments with one load a lane in place
+// of a search.
 __device__ __forceinline__ int64_t adapter_segment(const AdapterParams &d, int64_t row) {
-  if (!d.seg_off) {
-    const int64_t s = row / d.rows_per_seg;
-    return s < d.nseg ? s : d.nseg - 1;
-  }
-  int64_t n = 0;
-  for (int64_t s0 = 1; s0 < d.nseg; s0 += 64) {
-    const int64_t s = s0 + (threadIdx.x & 63);
-    n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(s < d.nseg && d.seg_off[s < d.nseg ? s : d.nseg] <= row));
-  }
-  return uniform(n);
+  if (!d.seg_off || d.nseg > 65) return uniform(segment_of(d.seg_off, d.nseg, d.rows_per_seg, row));
+  const int64_t s = (threadIdx.x & 63) + 1;
+  return __builtin_popcountll(__builtin_amdgcn_ballot_w64(s < d.nseg && d.seg_off[s < d.nseg ? s : d.nseg] <= row));
 }
 
 // Where t holds values k .. of `row`, k a multiple of 16 / EB, and the bytes from a piece to the row's next one.

@@ -386,7 +386,8 @@ int lux3d_q8_0_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *qs,
  *      zero rows of A); alphas: f32 [adapters] or NULL (1);
  *   adapter_ids: int32 [S] on the device; -1: the weight alone. Any other id
  *      outside 0 .. adapters - 1 counts as -1 and into bad_ids (int32 [1] or
- *      NULL: set to the number of such segments);
+ *      NULL: set to the number of such segments; left as it is where x or y is
+ *      empty);
  *   seg_offsets: int64 [S + 1], ascending, or NULL: S equal segments, as in
  *      lux3d_adaln_modulate (rows before the first offset are segment 0's, rows
  *      from the last one on segment S - 1's; segments may be empty);

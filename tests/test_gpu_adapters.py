@@ -174,6 +174,15 @@ def test_neighbours_do_not_leak(ops, dev, m):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,nseg", [(40, 160, 65), (40, 160, 66), (1500, 256, 256), (1500, 256, 257), (1500, 256, 1500), (3000, 1000, 900), (8200, 160, 700)])
+def test_many_segments(ops, dev, m, n, nseg, dt):
+    """Past 64 and past 256 segments, many of them empty."""
+    g = torch.Generator().manual_seed(nseg)
+    cuts = [0] + sorted(torch.randint(0, m + 1, (nseg - 1,), generator=g).tolist()) + [m]
+    run(ops, dev, m, 192, n, 20, dt, cuts, (torch.randint(0, 4, (nseg,), generator=g) - 1).tolist())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("m,k,n", [(9, 512, 160), (30, 512, 160), (60, 64, 200), (61, 1024, 1536), (300, 512, 1000), (700, 512, 4096),
                                    (2500, 512, 2048)])
 def test_an_adapter_that_is_not_finite_stays_with_its_rows(ops, dev, m, k, n, dt):
