@@ -6,7 +6,9 @@
 
 namespace lux3d {
 
-// Few: q8_0_few_rows_kernel, rows x 16 (rows 16: one row tile, 64: four);
+// Few: the few-rows kernels, rows x 16 (rows 16: one row tile, 64: four, or
+// twice two through LDS, which the costs below do not know: they keep every
+// size at the kernel, and the bits, that it had);
 // else a GEMM tile of rows x cols whose k is shared by `groups` groups of
 // wavefronts.
 struct Q8Tile {
