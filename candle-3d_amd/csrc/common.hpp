@@ -572,16 +572,22 @@ __device__ __forceinline__ i32x4_t buffer_rsrc(const void *base, int64_t bytes) 
 // pipelines; here the callers place their waits themselves. hipcc warns that
 // m0 is a reserved register in the clobber list: the statement overwrites
 // m0 without the compiler knowing its old value, which is safe only while
-// the compiler keeps nothing of its own in m0 in these kernels. The build
-// verifies that for every translation unit that calls these (check_m0.py
-// over its device assembly: no m0 use outside these pairs), and fails
+// the compiler keeps nothing of its own in m0 in these kernels. The s_nop is
+// the wait state that gfx9 needs between a scalar write of m0 and a load to
+// LDS: without it the load may take the m0 of the load before. The compiler
+// adds wait states to its own instructions only, not to inline assembly. The
+// build verifies both, and the five wait states from a vector instruction
+// that writes an SGPR to a load that reads it, for every translation unit
+// that calls these (check_m0.py over its device assembly), and fails
 // otherwise.
 __device__ __forceinline__ void lds_load16(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
+               "s"(rs), "s"(soff)
                : "memory", "m0");
 }
 __device__ __forceinline__ void lds_load4(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
+               "s"(rs), "s"(soff)
                : "memory", "m0");
 }
 // s_waitcnt immediates (gfx9 layout): vmcnt(n) with lgkmcnt(0), and vmcnt(n) alone
