@@ -1103,9 +1103,9 @@ hipError_t launch_prefix_mfma(const PrefixParams &p, hipStream_t s) {
   if (hipError_t e = hipGetLastError()) return e;
   if (p.plan.parts > 1) {
     auto grid_of = [&](int gp) { return dim3((unsigned)((rows * LPR * gp + 255) / 256)); };
-    // few parts of many rows: a row's lanes take them all, eight loads in flight
-    if (p.plan.parts > 32) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 256 / LPR, 4>), grid_of(256 / LPR), block, 0, s, p);
-    else if (p.plan.parts > 8 || rows < 4096) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4, 4>), grid_of(4), block, 0, s, p);
+    const int groups = prefix_merge_groups(p.plan.parts, rows);
+    if (groups == 0) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 256 / LPR, 4>), grid_of(256 / LPR), block, 0, s, p);
+    else if (groups == 4) hipLaunchKernelGGL((prefix_merge_kernel<T, D, 4, 4>), grid_of(4), block, 0, s, p);
     else hipLaunchKernelGGL((prefix_merge_kernel<T, D, 1, 8>), grid_of(1), block, 0, s, p);
   }
   return hipGetLastError();

@@ -92,4 +92,10 @@ inline int64_t prefix_workspace(const PrefixPlan &s, int64_t B, int64_t H, int64
   return s.parts > 1 ? s.parts * B * H * Lq * (D + 2) : 0;
 }
 
+// How many groups of lanes share a row's partial results in the merge: a row's lanes alone where few parts of many rows keep
+// every lane busy, the whole workgroup (0) where a row has many.
+inline int prefix_merge_groups(int64_t parts, int64_t rows) {
+  return parts > 32 ? 0 : parts > 8 || rows < 4096 ? 4 : 1;
+}
+
 }  // namespace lux3d
