@@ -1140,21 +1140,29 @@ bool prefix_block_fits(const lux3d_tensor_t *t, int64_t D) {
   const int64_t st = t->stride[t->rank - 2], e = elem_bytes(t->dtype);
   return t->shape[t->rank - 2] <= 1 || (st >= D && st < (int64_t(1) << 31) / (kPrefixKeys + 1) / e);
 }
+// head dims of the matrix-core kernels, the only ones that leave partial results
+bool prefix_mfma_dim(int64_t D) { return D == 64 || D == 128; }
 // the stride of a lone row counts for nothing: a descriptor's end must follow from it all the same
 int64_t prefix_row_stride(const lux3d_tensor_t *t, int64_t D) {
   return t->shape[t->rank - 2] <= 1 ? D : t->stride[t->rank - 2];
 }
 }  // namespace
 
+int64_t lux3d_sdpa_shared_prefix_workspace_dtype(int32_t dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                                                 int64_t queries, int64_t prefix, int64_t own, int64_t head_dim) {
+  if (!is_float(dtype) || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries <= 0 || prefix < 0 ||
+      own < 0 || !prefix_mfma_dim(head_dim))
+    return 0;
+  const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own, head_dim, dtype == LUX3D_F32);
+  return prefix_workspace(plan, batch, heads, queries, head_dim);
+}
+
 int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t prefix,
                                            int64_t own, int64_t head_dim) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries <= 0 || prefix < 0 || own < 0 || head_dim <= 0)
-    return 0;
   // the larger of the two element sizes' plans
   int64_t most = 0;
-  for (bool f32 : {false, true}) {
-    const PrefixPlan plan = prefix_plan(batch, heads, kv_heads, queries, prefix, own, head_dim, f32);
-    const int64_t n = prefix_workspace(plan, batch, heads, queries, head_dim);
+  for (int32_t dtype : {LUX3D_F32, LUX3D_BF16}) {
+    const int64_t n = lux3d_sdpa_shared_prefix_workspace_dtype(dtype, batch, heads, kv_heads, queries, prefix, own, head_dim);
     most = n > most ? n : most;
   }
   return most;
@@ -1213,7 +1221,7 @@ int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *pref
   // no keys: an address that exists in place of an empty tensor's, for descriptors of no bytes
   if (p.P == 0) p.pk = p.pv = p.q, p.pk_sh = p.pv_sh = 0, p.pk_st = p.pv_st = p.D;
   if (p.Ls == 0) p.k = p.v = p.q, p.k_sb = p.v_sb = p.k_sh = p.v_sh = 0, p.k_st = p.v_st = p.D;
-  p.mfma = (p.D == 64 || p.D == 128) && prefix_aligned(q) && prefix_aligned(prefix_k) &&
+  p.mfma = prefix_mfma_dim(p.D) && prefix_aligned(q) && prefix_aligned(prefix_k) &&
            prefix_aligned(prefix_v) && prefix_aligned(k) && prefix_aligned(v) && prefix_aligned(out) &&
            prefix_block_fits(prefix_k, p.D) && prefix_block_fits(prefix_v, p.D) && prefix_block_fits(k, p.D) &&
            prefix_block_fits(v, p.D);

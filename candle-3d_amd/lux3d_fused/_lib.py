@@ -73,6 +73,7 @@ SIGNATURES = {
     "lux3d_q8_0_quantize": [TP, TP, TP, S],
     "lux3d_sdpa": [TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_sdpa_shared_prefix_workspace": [ctypes.c_int64] * 7,
+    "lux3d_sdpa_shared_prefix_workspace_dtype": [ctypes.c_int32] + [ctypes.c_int64] * 7,
     "lux3d_sdpa_shared_prefix": [TP, TP, TP, TP, TP, TP, ctypes.c_int32, ctypes.c_float, TP, TP, S],
     "lux3d_sdpa_heads_f32": [TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_sdpa_layernorm_rope2d": [TP, TP, TP, ctypes.c_float, TP, TP, TP, TP, ctypes.c_float, TP, S],
@@ -91,7 +92,7 @@ SIGNATURES = {
 }
 
 # entries that return a size (int64), not a status
-SIZES = ("lux3d_sdpa_shared_prefix_workspace",)
+SIZES = ("lux3d_sdpa_shared_prefix_workspace", "lux3d_sdpa_shared_prefix_workspace_dtype")
 
 
 class Lux3dError(RuntimeError):

@@ -552,7 +552,7 @@ def sdpa_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
             out = _new(q)
         b, h, n, d = q.shape
         hkv, p, _ = prefix_k.shape
-        size = _lib.LIB.lux3d_sdpa_shared_prefix_workspace(b, h, hkv, n, p, k.shape[2], d)
+        size = _lib.LIB.lux3d_sdpa_shared_prefix_workspace_dtype(_DT.get(q.dtype, -1), b, h, hkv, n, p, k.shape[2], d)
         ws = q.new_empty(size, dtype=torch.float32) if size else None
         _lib.call(fn, _d(q), _d(prefix_k), _d(prefix_v), _d(k), _d(v), _d(lens), 1 if causal else 0, float(scale), _d(ws),
                   _d(out), _stream(q))

@@ -580,9 +580,11 @@ int lux3d_sdpa(const lux3d_tensor_t *q, const lux3d_tensor_t *k,
  *   read; those before it that causality hides from a query have to hold finite
  *   values (they are read beside those it sees, with a probability of zero).
  *   workspace: contiguous f32, 16-byte aligned, of at least
- *   lux3d_sdpa_shared_prefix_workspace(B, H, Hkv, Lq, P, Ls, D) values (0: may
- *   be NULL); its contents do not matter and it holds nothing between calls, but
- *   no two calls that may overlap share one.
+ *   lux3d_sdpa_shared_prefix_workspace_dtype(q's dtype, B, H, Hkv, Lq, P, Ls, D)
+ *   values (0: may be NULL; ..._workspace without the dtype: what suffices for
+ *   each); its contents do not matter and it holds nothing between calls, but no
+ *   two calls that may overlap share one. A call whose rows are not 16-byte
+ *   aligned needs none, whatever the function says.
  * D = 64 or 128 with every row 16-byte aligned runs on the matrix cores with
  * lux3d_sdpa's arithmetic (2-byte types: f32 scores, softmax and sums,
  * probabilities rounded to the type, one rounding of the output; f32: q, k, v and
@@ -594,6 +596,9 @@ int lux3d_sdpa(const lux3d_tensor_t *q, const lux3d_tensor_t *k,
 int64_t lux3d_sdpa_shared_prefix_workspace(int64_t batch, int64_t heads, int64_t kv_heads,
                                            int64_t queries, int64_t prefix, int64_t own,
                                            int64_t head_dim);
+int64_t lux3d_sdpa_shared_prefix_workspace_dtype(int32_t dtype, int64_t batch, int64_t heads,
+                                                 int64_t kv_heads, int64_t queries, int64_t prefix,
+                                                 int64_t own, int64_t head_dim);
 int lux3d_sdpa_shared_prefix(const lux3d_tensor_t *q, const lux3d_tensor_t *prefix_k,
                              const lux3d_tensor_t *prefix_v, const lux3d_tensor_t *k,
                              const lux3d_tensor_t *v, const lux3d_tensor_t *lens, int32_t causal,
