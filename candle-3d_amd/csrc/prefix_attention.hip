@@ -5,7 +5,7 @@
 //
 // What bounds it. Long queries: the matrix cores, 4 D operations a visible (query, key) pair. Decoding: the bytes of K
 // and V. The rows that share a key head's prefix, of all sequences and of the group's heads, are therefore taken
-// together, 64 rows a tile: the prefix is read once for up to 64 of them instead of once a row. Own keys are read by
+// together, 128 rows a tile: the prefix is read once for up to 128 of them instead of once a row. Own keys are read by
 // workgroups of their own. Every workgroup takes a run of key blocks, so that few rows still fill the chip, and leaves
 // an unnormalised partial result (maximum, sum, O); a second kernel merges a row's partials in their order.
 //
@@ -122,26 +122,26 @@ __device__ __forceinline__ PrefixRow prefix_row(const PrefixParams &p, int64_t k
   return {(int64_t)b, (int64_t)i, kv * p.G + (int64_t)(r - i * G)};
 }
 
-// Matrix-core kernel of the 2-byte types. Four wavefronts: 4 / KS row groups of 32 rows, the KS wavefronts of a group
-// taking every block's 64 / KS keys. S^T = K Q^T, O^T += V^T P^T as attn_mfma_kernel does it: each lane holds one row's
+// Few rows in the 2-byte types. Four wavefronts: two row groups of 32 rows, the KS = 2 wavefronts of a group taking 32 of
+// every block's 64 keys each. S^T = K Q^T, O^T += V^T P^T as attn_mfma_kernel does it: each lane holds one row's
 // scores of 16 keys, K and V blocks come by direct global -> LDS loads, two blocks deep.
-template <typename T, int D, int KS> struct PrefixLds {
+template <int D> struct PrefixLds {
   // the ring of two K and two V blocks; at the end the key groups' partial results
-  static constexpr int PW = KS > 1 ? (D / 32 * 16 + 2) * 64 : 0;  // floats of a wavefront
+  static constexpr int PW = (D / 32 * 16 + 2) * 64;  // floats of a wavefront
   static constexpr int bytes = 4 * kPrefixKeys * D * 2 > 4 * PW * 4 ? 4 * kPrefixKeys * D * 2 : 4 * PW * 4;
 };
-template <typename T, int D, int KS>
+template <typename T, int D>
 __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const PrefixItem &w, uint16_t *smem) {
   using M = Mma<T>;
   using op_t = typename M::op_t;
-  constexpr int BKV = kPrefixKeys, NKT = BKV / 32 / KS, NDT = D / 32;
+  constexpr int KS = 2, BKV = kPrefixKeys, NDT = D / 32;
   constexpr int KCH = BKV * D / 8 / 256;   // 16-byte chunks of K (and V) per thread and block
   constexpr int BUF = BKV * D;             // 2-byte elements of a block
-  constexpr bool VEARLY = D == 128 && KS == 2;  // 128 rows leave no registers for it
-  constexpr int PW = PrefixLds<T, D, KS>::PW;
+  constexpr bool VEARLY = D == 128;        // V's fragments before the softmax
+  constexpr int PW = PrefixLds<D>::PW;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
-  const int qg = wave / KS, kg = wave % KS, kt0 = kg * NKT;
+  const int qg = wave / KS, kg = wave % KS;  // kg: the block's 32 keys, too
 
   const int64_t g = w.r0 + qg * 32 + l32;          // this lane's row
   const bool live = g < w.rlim;
@@ -209,33 +209,27 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
       return;
     }
     const uint16_t *Ks = smem + buf * BUF, *Vs = smem + 2 * BUF + buf * BUF;
-    f32x16_t s[NKT];
+    f32x16_t s = f32x16_t{};
 #pragma unroll
-    for (int kt = 0; kt < NKT; ++kt) {
-      s[kt] = f32x16_t{};
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const int krow = (kt0 + kt) * 32 + l32;
-        const op_t a = *reinterpret_cast<const op_t *>(Ks + krow * D + ((2 * c + hh) ^ k_swz<D>(krow)) * 8);
-        s[kt] = M::run(a, qf[c], s[kt]);
-      }
+    for (int c = 0; c < D / 16; ++c) {
+      const int krow = kg * 32 + l32;
+      const op_t a = *reinterpret_cast<const op_t *>(Ks + krow * D + ((2 * c + hh) ^ k_swz<D>(krow)) * 8);
+      s = M::run(a, qf[c], s);
     }
-    // this lane's row sees keys below lim of the block; lane holds keys 8 (i / 4) + 4 hh + i % 4 of each 32-key tile
+    // this lane's row sees keys below lim of the block; lane holds keys 8 (i / 4) + 4 hh + i % 4 of its 32
     int lim = BKV;
     if constexpr (MASK) {
       lim = j < np ? (int)(w.p1 - w.p0) - j * BKV : seen - (int)w.o0 - (j - np) * BKV;
 #pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if ((kt0 + kt) * 32 + 8 * (i >> 2) + (i & 3) >= lim - 4 * hh) s[kt][i] = -INFINITY;
+      for (int i = 0; i < 16; ++i)
+        if (kg * 32 + 8 * (i >> 2) + (i & 3) >= lim - 4 * hh) s[i] = -INFINITY;
     }
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
     // V^T fragment of dim tile dt, keys 16 jj ..: see attn_mfma_kernel
-    auto vfrag = [&](int dt, int kt, int jj) {
+    auto vfrag = [&](int dt, int jj) {
       const int g16 = lane & 15;
-      const int vrow = (kt0 + kt) * 32 + 16 * jj + 4 * hh + (g16 >> 2);
+      const int vrow = kg * 32 + 16 * jj + 4 * hh + (g16 >> 2);
       const int vcol = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (g16 & 3);
       const uint16_t *vr = Vs + vrow * D + ((vcol >> 3) ^ v_swz<D>(vrow)) * 8 + (vcol & 7);
       const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vr));
@@ -243,23 +237,19 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
       return __builtin_bit_cast(op_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     // V's fragments are read before the softmax, which hides their latency
-    op_t vf[VEARLY ? NDT * NKT * 2 : 1];
+    op_t vf[VEARLY ? NDT * 2 : 1];
     if constexpr (VEARLY) {
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) vf[(dt * NKT + kt) * 2 + jj] = vfrag(dt, kt, jj);
+        for (int jj = 0; jj < 2; ++jj) vf[dt * 2 + jj] = vfrag(dt, jj);
       __builtin_amdgcn_sched_barrier(0);
     }
 
     // running maximum: it moves when a block's exceeds it by 2^8, so that most blocks need no rescale
     float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
     const float cand = half_swap_max(mx) * c2;
     const float mn = cand > m + 8.f ? cand : m;
     const float mb = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is exp2(-inf)
@@ -269,30 +259,25 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
       for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
     }
     m = mn;
-    op_t pf[NKT * 2];
+    op_t pf[2];
     float ls = 0.f;
 #pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
+    for (int jj = 0; jj < 2; ++jj) {
+      u32x4_t pk4;
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        u32x4_t pk4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * jj + 2 * e], c2, -mb));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * jj + 2 * e + 1], c2, -mb));
-          pk4[e] = M::pack(p0, p1);
-          ls = M::sum2(pk4[e], ls);
-        }
-        pf[kt * 2 + jj] = __builtin_bit_cast(op_t, pk4);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * jj + 2 * e], c2, -mb));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * jj + 2 * e + 1], c2, -mb));
+        pk4[e] = M::pack(p0, p1);
+        ls = M::sum2(pk4[e], ls);
       }
+      pf[jj] = __builtin_bit_cast(op_t, pk4);
+    }
     l = l * alpha + ls;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
-          o[dt] = M::run(VEARLY ? vf[(dt * NKT + kt) * 2 + jj] : vfrag(dt, kt, jj), pf[kt * 2 + jj], o[dt]);
+      for (int jj = 0; jj < 2; ++jj) o[dt] = M::run(VEARLY ? vf[dt * 2 + jj] : vfrag(dt, jj), pf[jj], o[dt]);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // this wavefront's part of block j + 1 landed
     lds_barrier();
   };
@@ -308,38 +293,36 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
     }
   }
 
-  if constexpr (KS > 1) {
-    // a row group's KS partial results, through LDS in key-group order; wavefront kg keeps the dim tiles dt % KS == kg
-    float *part = reinterpret_cast<float *>(smem), *mine = part + wave * PW;
+  // a row group's KS partial results, through LDS in key-group order; wavefront kg keeps the dim tiles dt % KS == kg
+  float *part = reinterpret_cast<float *>(smem), *mine = part + wave * PW;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
+  for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mine[(dt * 16 + i) * 64 + lane] = o[dt][i];
-    mine[NDT * 16 * 64 + lane] = m;
-    mine[(NDT * 16 + 1) * 64 + lane] = l;
-    lds_barrier();
-    const float *grp = part + qg * KS * PW;
-    float a[KS], mm = -INFINITY;
+    for (int i = 0; i < 16; ++i) mine[(dt * 16 + i) * 64 + lane] = o[dt][i];
+  mine[NDT * 16 * 64 + lane] = m;
+  mine[(NDT * 16 + 1) * 64 + lane] = l;
+  lds_barrier();
+  const float *grp = part + qg * KS * PW;
+  float a[KS], mm = -INFINITY;
 #pragma unroll
-    for (int k2 = 0; k2 < KS; ++k2) mm = fmaxf(mm, grp[k2 * PW + NDT * 16 * 64 + lane]);
-    const float mb = mm == -INFINITY ? 0.f : mm;
-    l = 0.f;
+  for (int k2 = 0; k2 < KS; ++k2) mm = fmaxf(mm, grp[k2 * PW + NDT * 16 * 64 + lane]);
+  const float mb = mm == -INFINITY ? 0.f : mm;
+  l = 0.f;
 #pragma unroll
-    for (int k2 = 0; k2 < KS; ++k2) {
-      a[k2] = __builtin_amdgcn_exp2f(grp[k2 * PW + NDT * 16 * 64 + lane] - mb);
-      l += grp[k2 * PW + (NDT * 16 + 1) * 64 + lane] * a[k2];
-    }
-    m = mm;
+  for (int k2 = 0; k2 < KS; ++k2) {
+    a[k2] = __builtin_amdgcn_exp2f(grp[k2 * PW + NDT * 16 * 64 + lane] - mb);
+    l += grp[k2 * PW + (NDT * 16 + 1) * 64 + lane] * a[k2];
+  }
+  m = mm;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      if (dt % KS != kg) continue;
+  for (int dt = 0; dt < NDT; ++dt) {
+    if (dt % KS != kg) continue;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float acc = 0.f;
+    for (int i = 0; i < 16; ++i) {
+      float acc = 0.f;
 #pragma unroll
-        for (int k2 = 0; k2 < KS; ++k2) acc += grp[k2 * PW + (dt * 16 + i) * 64 + lane] * a[k2];
-        o[dt][i] = acc;
-      }
+      for (int k2 = 0; k2 < KS; ++k2) acc += grp[k2 * PW + (dt * 16 + i) * 64 + lane] * a[k2];
+      o[dt][i] = acc;
     }
   }
 
@@ -353,7 +336,7 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
     if (m == -INFINITY) return;  // no key seen: the merge does not take this part's O
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
-      if (KS > 1 && dt % KS != kg) continue;
+      if (dt % KS != kg) continue;
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4)
         *reinterpret_cast<float4 *>(po + dt * 32 + 8 * g4 + 4 * hh) =
@@ -366,7 +349,7 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
   char *orow = reinterpret_cast<char *>(p.o) + (row.b * p.o_sb + row.h * p.o_sh + row.i * p.o_st) * 2;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) {
-    if (KS > 1 && dt % KS != kg) continue;
+    if (dt % KS != kg) continue;
 #pragma unroll
     for (int g4 = 0; g4 < 4; ++g4)
       *reinterpret_cast<uint2 *>(orow + (dt * 32 + 8 * g4 + 4 * hh) * 2) =
@@ -375,16 +358,16 @@ __device__ __forceinline__ void prefix_attend(const PrefixParams &p, const Prefi
   }
 }
 
-// ---- pipelined form: 128 QT rows a workgroup -------------------------------------
+// ---- pipelined form: 128 rows a workgroup ----------------------------------------
 //
 // attn_pipe_kernel's pipeline over the blocks of two key ranges: keys go by 32, two steps to a pair, and step j is one
 // straight line of MFMAs (scores of block j + 2, O += P V of block j) with the exponentials, the maximum and the LDS reads
-// in the gaps between them. Each of the 4 wavefronts keeps QT tiles of 32 rows. A block lies in one range: the prefix's
+// in the gaps between them. Each of the 4 wavefronts keeps 32 rows. A block lies in one range: the prefix's
 // last one ends where the prefix ends, and the next begins the own keys. K and V arrive by direct global -> LDS loads in
 // two stages of 64 keys, of which wavefronts 0 and 1 load the first block and 2 and 3 the second, so that each builds the
 // descriptor of its block's range; what lies past the range reads as zeros.
 // The running maximum starts at -3e38 rather than -inf: a row that has seen nothing yet forms exp2(-inf) = 0.
-template <typename T, int D, int QT>
+template <typename T, int D>
 __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const PrefixItem &w, char *ring, int *seen_lds) {
   using M = Mma<T>;
   using op_t = typename M::op_t;
@@ -395,23 +378,20 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
   static_assert(SEGW * RS == 16, "two wavefronts load a block");
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
-  int *const seen = seen_lds + wave * (QT * 32) + l32;  // own keys from o0 on that the lane's rows see: read for a mask only
+  int *const seen = seen_lds + wave * 32 + l32;  // own keys from o0 on that the lane's row sees: read for a mask only
   const int np = (int)((w.p1 - w.p0 + BK - 1) / BK), no = (int)((w.o1 - w.o0 + BK - 1) / BK), nkv = np + no;
 
-  op_t qf[QT][NC];
+  op_t qf[NC];
   int all_seen;  // own keys from o0 on that every row of the tile sees
   {
     const int64_t len = own_len(p, w.b);
     all_seen = __builtin_amdgcn_readfirstlane((int)(own_seen(p, len, (w.r0 - w.b * p.Lq * p.G) / p.G) - w.o0));
+    const int64_t g = w.r0 + wave * 32 + l32;
+    const PrefixRow row = prefix_row(p, w.kv, g < w.rlim ? g : w.rlim - 1);
+    *seen = (int)(own_seen(p, len, row.i) - w.o0);
+    const char *q = reinterpret_cast<const char *>(p.q) + (row.b * p.q_sb + row.h * p.q_sh + row.i * p.q_st) * 2;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const int64_t g = w.r0 + wave * (QT * 32) + qt * 32 + l32;
-      const PrefixRow row = prefix_row(p, w.kv, g < w.rlim ? g : w.rlim - 1);
-      seen[qt * 32] = (int)(own_seen(p, len, row.i) - w.o0);
-      const char *q = reinterpret_cast<const char *>(p.q) + (row.b * p.q_sb + row.h * p.q_sh + row.i * p.q_st) * 2;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) qf[qt][c] = *reinterpret_cast<const op_t *>(q + (c * 16 + 8 * hh) * 2);
-    }
+    for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const op_t *>(q + (c * 16 + 8 * hh) * 2);
   }
 
   // the lane's part of a load: row r0 + RS i of its wavefront's block, the chunk that its slot holds
@@ -481,43 +461,35 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
         (lds_s16x4_t *)(ring + at + (vfo ^ (dt << 6)) + (16 * jj + 8 * h) * 2 * D));
   };
 
-  f32x16_t o[QT][NDT], sa[QT], sb[QT];
-  float m[QT], l[QT], ls[QT], alpha[QT], mx[QT];
-  op_t kf[NC], pf[QT][2];
+  f32x16_t o[NDT], sa, sb;
+  float m = -3e38f, l = 0.f, ls = 0.f, alpha, mx;
+  op_t kf[NC], pf[2];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    m[qt] = -3e38f;
-    l[qt] = ls[qt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[qt][dt] = f32x16_t{};
-  }
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16_t{};
   const float c2 = p.scale * kLog2e;
 
   // block j's keys that a row does not see (past the prefix's end, the sequence's, or by causality) score -inf
-  auto mask = [&](int j, f32x16_t (&s)[QT]) {
+  auto mask = [&](int j, f32x16_t &s) {
+    const int lim = (j < np ? pn - j * BK : j < nkv ? *seen - (j - np) * BK : 0) - 4 * hh;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const int lim = (j < np ? pn - j * BK : j < nkv ? seen[qt * 32] - (j - np) * BK : 0) - 4 * hh;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i >> 2) + (i & 3) >= lim) s[qt][i] = -INFINITY;
-    }
+    for (int i = 0; i < 16; ++i)
+      if (8 * (i >> 2) + (i & 3) >= lim) s[i] = -INFINITY;
   };
   // blocks that need a mask: the prefix's last where it is not whole, and from own_first on
   const int cut = pn % BK ? np - 1 : -1, all = all_seen > 0 ? all_seen / BK : 0, own_first = np + (all < no ? all : no);
   auto partial = [&](int j) { return (j == cut) | (j >= own_first); };
-  auto max_step = [&](const f32x16_t (&s)[QT], int qt, int i, bool first) {
-    if (first && i == 0) mx[qt] = fmaxf(s[qt][0], s[qt][1]);
-    else mx[qt] = fmaxf(fmaxf(mx[qt], s[qt][2 * i]), s[qt][2 * i + 1]);
+  auto max_step = [&](const f32x16_t &s, int i, bool first) {
+    if (first && i == 0) mx = fmaxf(s[0], s[1]);
+    else mx = fmaxf(fmaxf(mx, s[2 * i]), s[2 * i + 1]);
   };
-  auto max_done = [&](int qt) {
-    const float cand = half_swap_max(mx[qt]) * c2;
-    float mn = m[qt];
+  auto max_done = [&]() {
+    const float cand = half_swap_max(mx) * c2;
+    float mn = m;
     if (cand > mn + 8.f) mn = cand;
-    alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mn);
-    m[qt] = mn;
+    alpha = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
   };
-  auto sum_pair = [&](int qt) { l[qt] = __builtin_fmaf(l[qt], alpha[qt], ls[qt]); };
+  auto sum_pair = [&]() { l = __builtin_fmaf(l, alpha, ls); };
 
   if (nkv > 0) {
     // prologue: K's blocks 0, 1 and 2, 3 into the slot of stage 1, stage 0; the scores of the first pair, its maximum
@@ -535,11 +507,9 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * SEGW));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    auto scores = [&](f32x16_t (&s)[QT]) {
+    auto scores = [&](f32x16_t &s) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) s[qt] = M::run(kf[c], qf[qt][c], c == 0 ? f32x16_t{} : s[qt]);
+      for (int c = 0; c < NC; ++c) s = M::run(kf[c], qf[c], c == 0 ? f32x16_t{} : s);
     };
 #pragma unroll
     for (int c = 0; c < NC; ++c) kf[c] = kfrag(STAGE, c);
@@ -552,22 +522,19 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
     mask(0, sa);
     mask(1, sb);
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
+    for (int i = 0; i < 8; ++i) max_step(sa, i, true);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) max_step(sa, qt, i, true);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) max_step(sb, qt, i, false);
-      max_done(qt);
-    }
+    for (int i = 0; i < 8; ++i) max_step(sb, i, false);
+    max_done();
 
     // One step on block j, of parity PAR, whose scores are in s. NEXT: there is a next pair, and the scores of block
     // j + 2 replace them. The mask is a branch inside the step: a second form of the step beside it, chosen by the block,
     // spills 157 registers.
-    auto step = [&](int j, f32x16_t (&s)[QT], auto par_c, auto next_c) {
+    auto step = [&](int j, f32x16_t &s, auto par_c, auto next_c) {
       constexpr int PAR = decltype(par_c)::value;
       constexpr bool NEXT = decltype(next_c)::value;
       // MFMAs: the scores but for their last chunk, one half of P v, the scores' last chunk, the other half
-      constexpr int NA = NEXT ? QT * (NC - 1) : 0, NL = NEXT ? QT : 0, NB = QT * 2 * NDT, NM = NA + NB + NL;
+      constexpr int NA = NEXT ? NC - 1 : 0, NL = NEXT ? 1 : 0, NB = 2 * NDT, NM = NA + NB + NL;
       constexpr int LAST = NA + NB / 2;  // the scores' last chunk
       constexpr int at = PAR * KB;
       if constexpr (PAR == 0) {
@@ -576,38 +543,32 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         load_stage(slot ^ 1);
-        bool any = false;
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) any = any || alpha[qt] != 1.f;
-        if (__builtin_amdgcn_ballot_w64(any)) {
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[qt][dt] *= alpha[qt];
+          for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
         }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) ls[qt] = 0.f;
+        ls = 0.f;
       }
       __builtin_amdgcn_sched_barrier(0);
       s16x4_t vh[NDT][2][2];
-      f32x16_t sn[QT];
+      f32x16_t sn;
       // exponentials, two pairs of scores at a time: 4 FMAs, 4 exponentials, 2 packs, 2 sums
       auto exp_op = [&](int n) {
-        const int g = n / 12, r = n % 12, qt = g / 4, e0 = 4 * (g % 4);
+        const int r = n % 12, e0 = 4 * (n / 12);
         if (r < 4) {
-          s[qt][e0 + r] = __builtin_fmaf(s[qt][e0 + r], c2, -m[qt]);
+          s[e0 + r] = __builtin_fmaf(s[e0 + r], c2, -m);
         } else if (r < 8) {
-          s[qt][e0 + r - 4] = __builtin_amdgcn_exp2f(s[qt][e0 + r - 4]);
+          s[e0 + r - 4] = __builtin_amdgcn_exp2f(s[e0 + r - 4]);
         } else {
           const int h = r & 1, pe = e0 / 2 + h;  // packed pair pe of the tile: element pe % 4 of fragment pe / 4
-          u32x4_t pk4 = __builtin_bit_cast(u32x4_t, pf[qt][pe / 4]);
-          if (r < 10) pk4[pe % 4] = M::pack(s[qt][e0 + 2 * h], s[qt][e0 + 2 * h + 1]);
-          else ls[qt] = M::sum2(pk4[pe % 4], ls[qt]);
-          pf[qt][pe / 4] = __builtin_bit_cast(op_t, pk4);
+          u32x4_t pk4 = __builtin_bit_cast(u32x4_t, pf[pe / 4]);
+          if (r < 10) pk4[pe % 4] = M::pack(s[e0 + 2 * h], s[e0 + 2 * h + 1]);
+          else ls = M::sum2(pk4[pe % 4], ls);
+          pf[pe / 4] = __builtin_bit_cast(op_t, pk4);
         }
       };
-      // VALU items: 4 groups of 12 per tile; 8 steps of the maximum per tile and the pair's end
-      constexpr int NEXP = 48 * QT, NMT = PAR == 1 ? 9 : 8, NMAX = NEXT ? NMT * QT : 0, REST = NB / 2;
+      // VALU items: 4 groups of 12; 8 steps of the maximum and the pair's end
+      constexpr int NEXP = 48, NMAX = !NEXT ? 0 : PAR == 1 ? 9 : 8, REST = NB / 2;
       if constexpr (!NEXT) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
@@ -621,37 +582,30 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
 #pragma unroll
       for (int u = 0; u < NM; ++u) {
         if (u < NA) {
-          const int c = u / QT, qt = u % QT;
-          sn[qt] = M::run(kf[c], qf[qt][c], c == 0 ? f32x16_t{} : sn[qt]);
+          sn = M::run(kf[u], qf[u], u == 0 ? f32x16_t{} : sn);
           // V's 4 NDT fragment halves, spread over these MFMAs
 #pragma unroll
           for (int x = 0; x < 4 * NDT; ++x)
             if (x >= u * 4 * NDT / (NA ? NA : 1) && x < (u + 1) * 4 * NDT / (NA ? NA : 1))
               vh[x / 4][x / 2 % 2][x % 2] = vhalf(at, x / 4, x / 2 % 2, x % 2);
         } else if (u >= LAST && u < LAST + NL) {
-          const int qt = u - LAST;
-          s[qt] = M::run(kf[NC - 1], qf[qt][NC - 1], sn[qt]);
-          keep(sn[qt]);  // the product goes to s's registers, not to sn's and a copy
+          s = M::run(kf[NC - 1], qf[NC - 1], sn);
+          keep(sn);  // the product goes to s's registers, not to sn's and a copy
         } else {
-          const int b = u < LAST ? u - NA : u - NA - NL, qt = b / (2 * NDT), jj = b / NDT % 2, dt = b % NDT;
+          const int b = u < LAST ? u - NA : u - NA - NL, jj = b / NDT, dt = b % NDT;
           const op_t a = __builtin_bit_cast(op_t, __builtin_shufflevector(vh[dt][jj][0], vh[dt][jj][1], 0, 1, 2, 3, 4, 5, 6, 7));
-          o[qt][dt] = M::run(a, pf[qt][jj], o[qt][dt]);
-          if (NEXT && b % QT == 0 && b / QT < NC) kf[b / QT] = kfrag(at, b / QT);
+          o[dt] = M::run(a, pf[jj], o[dt]);
+          if (NEXT && b < NC) kf[b] = kfrag(at, b);
         }
         if constexpr (NEXT) {
 #pragma unroll
           for (int n = 0; n < NEXP; ++n)
             if (n >= u * NEXP / LAST && n < (u + 1) * NEXP / LAST) exp_op(n);
-          if (PAR == 1 && u == LAST - 1) {
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) sum_pair(qt);
-          }
+          if (PAR == 1 && u == LAST - 1) sum_pair();
           if (u == LAST + NL - 1) {
             // formed by here: the compiler would move what is used behind the branch there, away from the MFMAs before it
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-              for (int jj = 0; jj < 2; ++jj) asm volatile("" ::"v"(pf[qt][jj]), "v"(ls[qt]), "v"(l[qt]));
+            for (int jj = 0; jj < 2; ++jj) asm volatile("" ::"v"(pf[jj]), "v"(ls), "v"(l));
 #pragma unroll
             for (int x = 0; x < 4 * NDT; ++x) asm volatile("" ::"v"(vh[x / 4][x / 2 % 2][x % 2]));
             if (partial(j + 2)) mask(j + 2, s);
@@ -666,8 +620,8 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
 #pragma unroll
           for (int n = 0; n < NMAX; ++n)
             if (r >= 0 && n >= r * NMAX / REST && n < (r + 1) * NMAX / REST) {
-              if (n % NMT < 8) max_step(s, n / NMT, n % NMT, PAR == 0);
-              else max_done(n / NMT);
+              if (n < 8) max_step(s, n, PAR == 0);
+              else max_done();
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -689,61 +643,57 @@ __device__ __forceinline__ void prefix_attend_pipe(const PrefixParams &p, const 
     }
     step(j, sa, even, no_);
     if (j + 2 == nkv) step(j + 1, sb, odd, no_);
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) sum_pair(qt);
+    sum_pair();
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads
   }
 
   // lane holds dims dt * 32 + 8 g4 + 4 hh + {0..3}, g4 = 0..3
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int64_t g = w.r0 + wave * (QT * 32) + qt * 32 + l32;
-    const float total = half_swap_sum(l[qt]);
-    if (g >= w.rlim) continue;
-    if (p.plan.parts > 1) {
-      const int64_t per = p.B * p.Lq * p.G, rows = per * p.Hkv, r = w.part * rows + w.kv * per + g;
-      const bool none = total == 0.f;
-      if (hh == 0) *reinterpret_cast<float2 *>(p.ws + p.plan.parts * rows * D + r * 2) = make_float2(none ? -INFINITY : m[qt], total);
-      if (none) continue;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4)
-          *reinterpret_cast<float4 *>(p.ws + r * D + dt * 32 + 8 * g4 + 4 * hh) =
-              make_float4(o[qt][dt][4 * g4], o[qt][dt][4 * g4 + 1], o[qt][dt][4 * g4 + 2], o[qt][dt][4 * g4 + 3]);
-      continue;
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const PrefixRow row = prefix_row(p, w.kv, g);
-    char *orow = reinterpret_cast<char *>(p.o) + (row.b * p.o_sb + row.h * p.o_sh + row.i * p.o_st) * 2;
+  const int64_t g = w.r0 + wave * 32 + l32;
+  const float total = half_swap_sum(l);
+  if (g >= w.rlim) return;
+  if (p.plan.parts > 1) {
+    const int64_t per = p.B * p.Lq * p.G, rows = per * p.Hkv, r = w.part * rows + w.kv * per + g;
+    const bool none = total == 0.f;
+    if (hh == 0) *reinterpret_cast<float2 *>(p.ws + p.plan.parts * rows * D + r * 2) = make_float2(none ? -INFINITY : m, total);
+    if (none) return;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4)
-        *reinterpret_cast<uint2 *>(orow + (dt * 32 + 8 * g4 + 4 * hh) * 2) =
-            make_uint2(M::pack(o[qt][dt][4 * g4] * inv, o[qt][dt][4 * g4 + 1] * inv),
-                       M::pack(o[qt][dt][4 * g4 + 2] * inv, o[qt][dt][4 * g4 + 3] * inv));
+        *reinterpret_cast<float4 *>(p.ws + r * D + dt * 32 + 8 * g4 + 4 * hh) =
+            make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+    return;
   }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const PrefixRow row = prefix_row(p, w.kv, g);
+  char *orow = reinterpret_cast<char *>(p.o) + (row.b * p.o_sb + row.h * p.o_sh + row.i * p.o_st) * 2;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      *reinterpret_cast<uint2 *>(orow + (dt * 32 + 8 * g4 + 4 * hh) * 2) =
+          make_uint2(M::pack(o[dt][4 * g4] * inv, o[dt][4 * g4 + 1] * inv),
+                     M::pack(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv));
 }
 
-// JOINT: every workgroup 128 / KS rows (KS 1: pipelined, 128 QT rows) of one sequence through prefix and own keys. Else
-// pipelined prefix items of 128 rows, and own items whose few rows split each block's keys between two wavefronts.
-template <typename T, int D, bool JOINT, int KS, int QT, int MINW>
+// JOINT: every workgroup 128 / KS rows (128: pipelined) of one sequence through prefix and own keys. Else pipelined prefix
+// items of 128 rows, and own items whose few rows split each block's keys between two wavefronts.
+template <typename T, int D, bool JOINT, int KS, int MINW>
 __global__ __launch_bounds__(256, MINW) void prefix_attn_kernel(PrefixParams p, int64_t nwg) {
-  constexpr int RING = 8 * 32 * D * 2, LDS = JOINT && KS == 1 ? RING : PrefixLds<T, D, 2>::bytes;
+  constexpr int RING = 8 * 32 * D * 2, LDS = JOINT && KS == 1 ? RING : PrefixLds<D>::bytes;
   static_assert(LDS >= RING, "both item kinds fit");
   __shared__ __align__(16) uint16_t smem[LDS / 2];
-  __shared__ int seen[JOINT && KS > 1 ? 1 : 128 * QT];
+  __shared__ int seen[JOINT && KS > 1 ? 1 : 128];
   if constexpr (JOINT && KS > 1) {
-    prefix_attend<T, D, KS>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), smem);
+    prefix_attend<T, D>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), smem);
   } else if constexpr (JOINT) {
-    prefix_attend_pipe<T, D, QT>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), reinterpret_cast<char *>(smem), seen);
+    prefix_attend_pipe<T, D>(p, prefix_item(p, xcd_logical_id(blockIdx.x, nwg), true), reinterpret_cast<char *>(smem), seen);
   } else {
     const int64_t np = p.Hkv * p.plan.prefix_tiles * p.plan.prefix_runs;
     if ((int64_t)blockIdx.x < np)
-      prefix_attend_pipe<T, D, QT>(p, prefix_item(p, xcd_logical_id(blockIdx.x, np), true), reinterpret_cast<char *>(smem), seen);
+      prefix_attend_pipe<T, D>(p, prefix_item(p, xcd_logical_id(blockIdx.x, np), true), reinterpret_cast<char *>(smem), seen);
     else
-      prefix_attend<T, D, 2>(p, prefix_item(p, (int64_t)blockIdx.x - np, false), smem);
+      prefix_attend<T, D>(p, prefix_item(p, (int64_t)blockIdx.x - np, false), smem);
   }
 }
 
@@ -999,7 +949,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixParams p) {
   }
 }
 
-// Any head dim up to 512, any alignment, f32: one wavefront per row, f32 throughout; lanes over keys for the scores,
+// The other head dims up to 512 and unaligned rows, each type: one wavefront per row, f32 throughout; lanes over keys for the scores,
 // over dims for the output. DPL: dims per lane.
 __device__ __forceinline__ float wave_max_xor(float v) {
 #pragma unroll
@@ -1096,9 +1046,9 @@ hipError_t launch_prefix_mfma(const PrefixParams &p, hipStream_t s) {
     else hipLaunchKernelGGL((prefix_f32_kernel<D, true, MINW>), grid, block, 0, s, p, nwg);
   } else {
     constexpr int MINW = D == 64 ? 3 : 2;
-    if (!p.plan.joint) hipLaunchKernelGGL((prefix_attn_kernel<T, D, false, 1, 1, MINW>), grid, block, 0, s, p, nwg);
-    else if (p.plan.ks == 2) hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 2, 1, MINW>), grid, block, 0, s, p, nwg);
-    else hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 1, 1, MINW>), grid, block, 0, s, p, nwg);
+    if (!p.plan.joint) hipLaunchKernelGGL((prefix_attn_kernel<T, D, false, 1, MINW>), grid, block, 0, s, p, nwg);
+    else if (p.plan.ks == 2) hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 2, MINW>), grid, block, 0, s, p, nwg);
+    else hipLaunchKernelGGL((prefix_attn_kernel<T, D, true, 1, MINW>), grid, block, 0, s, p, nwg);
   }
   if (hipError_t e = hipGetLastError()) return e;
   if (p.plan.parts > 1) {
