@@ -13,9 +13,9 @@
 // are only 2-byte aligned, into int8 [N, K] row-major plus f32 scales
 // [N, K/32], so the GEMM streams them with 16-byte loads.
 //
-// Four GEMM kernels (each one rounding of the f32 sum per output):
-// - q8_0_few_rows_kernel and q8_0_few_rows_lds_kernel (K % 64 == 0, up to 16 rows or few tiles): workgroups of
-//   16 weight rows whose wavefronts split k.
+// Five GEMM kernels (each one rounding of the f32 sum per output):
+// - q8_0_few_rows_kernel and q8_0_few_rows_lds_kernel (K % 64 == 0, up to 16
+//   rows or few tiles): workgroups of 16 weight rows whose wavefronts split k.
 // - q8_0_gemm_ring_kernel (K % 64 == 0, the common case): a workgroup of NW
 //   wavefronts (8, or 4 for small shapes) computes a BM x 32 NW tile (BM 32 to
 //   256); x, the
@@ -749,136 +749,112 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 1) void q8_0_gemm_x3_kernel(Q8Ge
 // One modulation or conditioning vector per batch element, short sequences: the
 // weights' bytes bound them, and tiles of 128 rows leave most CUs idle (72
 // workgroups at N 9216) behind a serial k loop. A workgroup owns 16 weight rows
-// and 16 MT rows of x; its NW wavefronts take pairs of 64-deep chunks of k in
-// turn, and their sums (v_mfma_f32_16x16x32_bf16: x rows x weight rows) are
-// added in wavefront order through LDS. A turn of the loop takes U chunks, but
-// as compiled a wavefront waits for each chunk's loads and multiplies before it
-// issues the next chunk's (the branch after each chunk keeps them apart: 51
-// VGPRs): one chunk is in flight per wavefront, and only the other wavefronts
-// of the SIMD cover its latency. k order inside a chunk: lane group g = lane / 16 holds weights
-// 16 g .. 16 g + 15 of its row as one 16-byte load (one Q8_0 block, one scale),
-// bytes 8 s .. + 7 in MFMA s, and x alike. XF32: f32 x in three exact bf16
-// terms, the int8 weights exact, one MFMA per term and Q8_0 block (lane group
-// g: weights 8 g .. + 7), the block's sum scaled by d, as q8_0_gemm_x3_kernel
-// does. Before / after, us: M 2, K 1536 -> N 9216 16.9 / 8.0 in bf16 (16 MB of
-// weights: 3.1 us at the copy rate) and 71 / 10.8 in f32; M 64, K 8192 -> N
-// 2048 68 / 38 and 363 / 69.
-template <typename OUT, bool XF32, int NW, int MT, bool AD>
-__global__ __launch_bounds__(64 * NW) void q8_0_few_rows_kernel(Q8GemmParams p) {
+// and one or two tiles of 16 rows of x; its NW wavefronts take pairs of 64-deep
+// chunks of k in turn, and their sums (v_mfma_f32_16x16x32_bf16: x rows x weight
+// rows) are added in wavefront order through LDS. k order inside a chunk: lane
+// group g = lane / 16 holds weights 16 g .. 16 g + 15 of its row (one Q8_0 block,
+// one scale), bytes 8 s .. + 7 in MFMA s, and x alike. XF32: f32 x in three exact
+// bf16 terms, the int8 weights exact, one MFMA per term and Q8_0 block (lane
+// group g: weights 8 g .. + 7), the block's sum scaled by d, as
+// q8_0_gemm_x3_kernel does.
+//
+// q8_0_few_rows_kernel, up to 16 rows of K below 512: operands loaded as the
+// matrix instruction's lanes hold them, at most one pair of chunks a wavefront.
+// us, this / through LDS as below, bf16 and f32: M 1, K 64 -> N 1536 1.99 / 2.04
+// and 2.08 / 2.47, K 320 -> 4096 2.21 / 2.34 and 2.64 / 3.13, K 448 -> 9216 2.89 /
+// 3.05 and 3.78 / 4.44; M 16, K 64 -> 4096 2.08 / 2.16 and 2.25 / 2.60, K 320 ->
+// 4096 2.39 / 2.47 and 3.11 / 3.24, but K 448 -> 9216 3.58 / 3.17 and 5.28 / 4.56.
+template <typename OUT, bool XF32, bool AD>
+__global__ __launch_bounds__(256) void q8_0_few_rows_kernel(Q8GemmParams p) {
   typedef float f32x4_t __attribute__((ext_vector_type(4)));
-  constexpr int U = MT == 1 ? (XF32 ? 4 : 8) : 2;  // chunks per turn
-  __shared__ float part[NW][MT * 256];
+  constexpr int NW = 4, U = 2;  // wavefronts; chunks of a turn, of which K below 512 has one
+  __shared__ float part[NW][256];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, m = lane & 15;
   // rows past N and M are clamped: loaded, computed, never stored
   const int64_t n = n0 + (lane & 15) < p.N ? n0 + (lane & 15) : p.N - 1;
   const int64_t nch = p.K / 64;
   const int8_t *wr = p.qs + n * p.K;
   const float *sr = p.scales + n * (p.K / 32);
-  const char *xr[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t m = m0 + 16 * i + (lane & 15);
-    xr[i] = reinterpret_cast<const char *>(p.x) + (m < p.M ? m : p.M - 1) * p.ldx * (XF32 ? 4 : 2);
-  }
-  f32x4_t acc[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4_t{};
+  const char *xr = reinterpret_cast<const char *>(p.x) + (m < p.M ? m : p.M - 1) * p.ldx * (XF32 ? 4 : 2);
+  f32x4_t acc = f32x4_t{};
   // chunks go to the wavefronts in pairs: whole 128-byte lines of the weights
   for (int64_t c0 = 2 * wave; c0 < nch; c0 += U * NW) {
-    auto chunk = [&](int u) { return c0 + (int64_t)(u / 2) * 2 * NW + (u & 1); };
     if constexpr (!XF32) {
-      uint4 w[U], x[U][MT][2];
+      uint4 w[U], x[U][2];
       float d[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t c = chunk(u) < nch ? chunk(u) : c0;
+        const int64_t c = c0 + u < nch ? c0 + u : c0;
         w[u] = ld16<false>(wr + c * 64 + 16 * g);
         d[u] = sr[c * 2 + (g >> 1)];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          x[u][i][0] = ld16<false>(xr[i] + (c * 64 + 16 * g) * 2);
-          x[u][i][1] = ld16<false>(xr[i] + (c * 64 + 16 * g) * 2 + 16);
-        }
+        x[u][0] = ld16<false>(xr + (c * 64 + 16 * g) * 2);
+        x[u][1] = ld16<false>(xr + (c * 64 + 16 * g) * 2 + 16);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (chunk(u) >= nch) break;  // uniform
+        if (c0 + u >= nch) break;  // uniform
         const bf16x8_t b0 = dequant8(w[u].x, w[u].y, d[u]), b1 = dequant8(w[u].z, w[u].w, d[u]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][i][0]), b0, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][i][1]), b1, acc[i], 0, 0, 0);
-        }
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][0]), b0, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][1]), b1, acc, 0, 0, 0);
       }
     } else {
       uint2 w[U][2];
-      float d[U][2], x[U][2][MT][8];
+      float d[U][2], x[U][2][8];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t c = chunk(u) < nch ? chunk(u) : c0;
+        const int64_t c = c0 + u < nch ? c0 + u : c0;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           w[u][b] = *reinterpret_cast<const uint2 *>(wr + c * 64 + 32 * b + 8 * g);
           d[u][b] = sr[c * 2 + b];
-#pragma unroll
-          for (int i = 0; i < MT; ++i) Chunk<F32>::load<false>(xr[i] + (c * 64 + 32 * b + 8 * g) * 4, x[u][b][i]);
+          Chunk<F32>::load<false>(xr + (c * 64 + 32 * b + 8 * g) * 4, x[u][b]);
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (chunk(u) >= nch) break;  // uniform
+        if (c0 + u >= nch) break;  // uniform
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const bf16x8_t q = dequant8(w[u][b].x, w[u][b].y, 1.f);
+          u32x4_t x1, x2, x3;
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            uint32_t x1[4], x2[4], x3[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const Split3 r = split3_bf16(x[u][b][i][2 * e], x[u][b][i][2 * e + 1]);
-              x1[e] = r.t1;
-              x2[e] = r.t2;
-              x3[e] = r.t3;
-            }
-            f32x4_t blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, u32x4_t{x3[0], x3[1], x3[2], x3[3]}), q, f32x4_t{}, 0, 0, 0);
-            blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, u32x4_t{x2[0], x2[1], x2[2], x2[3]}), q, blk, 0, 0, 0);
-            blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, u32x4_t{x1[0], x1[1], x1[2], x1[3]}), q, blk, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(blk[e], d[u][b], acc[i][e]);
+          for (int e = 0; e < 4; ++e) {
+            const Split3 r = split3_bf16(x[u][b][2 * e], x[u][b][2 * e + 1]);
+            x1[e] = r.t1;
+            x2[e] = r.t2;
+            x3[e] = r.t3;
           }
+          f32x4_t blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x3), q, f32x4_t{}, 0, 0, 0);
+          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x2), q, blk, 0, 0, 0);
+          blk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x1), q, blk, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(blk[e], d[u][b], acc[e]);
         }
       }
     }
   }
-  // lane holds rows 4 g + e, column lane % 16 of each 16-row tile
+  // lane holds rows 4 g + e, column lane % 16
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][i * 256 + e * 64 + lane] = acc[i][e];
+  for (int e = 0; e < 4; ++e) part[wave][e * 64 + lane] = acc[e];
   __syncthreads();
-  for (int o = t; o < MT * 256; o += 64 * NW) {
-    const int64_t row = m0 + o / 256 * 16 + 4 * ((o & 63) >> 4) + (o >> 6 & 3), col = n0 + (o & 15);
-    if (row >= p.M || col >= p.N) continue;
-    float v = part[0][o];
+  const int64_t row = 4 * ((t & 63) >> 4) + (t >> 6), col = n0 + (t & 15);
+  if (row >= p.M || col >= p.N) return;
+  float v = part[0][t];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += part[w][o];
-    if constexpr (AD) v += adapter_dot<XF32>(p.ad, p.M, p.N, row, col);
-    store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
-  }
+  for (int w = 1; w < NW; ++w) v += part[w][t];
+  if constexpr (AD) v += adapter_dot<XF32>(p.ad, p.M, p.N, row, col);
+  store1<OUT>(p.y, row * p.ldy + col, v + (p.bias ? p.bias[col] : 0.f));
 }
 
-// The form for K from 512 on: the same sums in the same order. A lane a row, as the matrix instruction holds its operands,
-// the cache serves one lane's bytes a cycle, so that weights, scales and x here go through LDS, each row's chunk loaded by
-// neighbouring lanes; each wavefront has LDS of its own, and loads a chunk's successor as soon as the chunk is there (MT 1:
-// two chunks together, 4 to 10% faster there). us, operand loads / through LDS, bf16 and f32: M 1, K 1536 -> N 9216 7.3 /
-// 6.3 and 9.9 / 9.5; M 16 10.2 / 6.5 and 15.5 / 9.7; M 4, K 8192 -> N 2048 12.4 / 9.9 and 19.7 / 14.5; M 3, K 1536 -> N
-// 1536 4.1 / 3.6 and 5.3 / 5.0; with two row tiles for four: M 64, K 8192 -> N 2048 37.9 / 13.2 and 69.6 / 25.4; M 61, K
-// 1536 -> N 1536 8.9 / 4.7 and 14.4 / 7.0; M 2000, K 2048 -> N 16 11.1 / 5.0 and 19.2 / 7.7; but M 1, K 320 -> N 4096 2.6 /
-// 2.7 and 3.2 / 3.5.
+// The form for K from 512 on and for more than 16 rows: the same sums in the same order. A lane a row, as the matrix
+// instruction holds its operands, the cache serves one lane's bytes a cycle, so that weights, scales and x here go through
+// LDS, each row's chunk loaded by neighbouring lanes; each wavefront has LDS of its own, and loads a chunk's successor as
+// soon as the chunk is there (MT 1: two chunks together, 4 to 10% faster there). us, operand loads / through LDS, bf16 and
+// f32: M 1, K 1536 -> N 9216 7.3 / 6.3 and 9.9 / 9.5; M 16 10.2 / 6.5 and 15.5 / 9.7; M 4, K 8192 -> N 2048 12.4 / 9.9 and
+// 19.7 / 14.5; M 3, K 1536 -> N 1536 4.1 / 3.6 and 5.3 / 5.0. Two row tiles, against four by operand loads: M 64, K 8192 -> N
+// 2048 37.9 / 13.2 and 69.6 / 25.4; M 61, K 1536 -> N 1536 8.9 / 4.7 and 14.4 / 7.0; M 2000, K 2048 -> N 16 11.1 / 5.0 and
+// 19.2 / 7.7; M 64, K 448 -> N 1024 4.1 / 2.9 and 6.1 / 4.2; M 33, K 64 -> N 512 2.41 / 2.36 and 3.40 / 2.96.
 template <typename OUT, bool XF32, int NW, int MT, bool AD>
 __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_lds_kernel(Q8GemmParams p) {
   typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -888,7 +864,8 @@ __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_lds_kernel(Q8GemmParams
   constexpr int OUTS = MT * 256 / (64 * NW) > 0 ? MT * 256 / (64 * NW) : 1;
   __shared__ __align__(16) char lds[NW][BYTES];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, l16 = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 16 * MT;
+  if (m0 >= p.M) return;  // uniform
   const int64_t nch = p.K / 64;
   // rows past N and M are clamped: loaded, computed, never stored
   auto wrow = [&](int r) { return n0 + r < p.N ? n0 + r : p.N - 1; };
@@ -1025,31 +1002,32 @@ __global__ __launch_bounds__(64 * NW) void q8_0_few_rows_lds_kernel(Q8GemmParams
   }
 }
 
-// Rows of 16 MT a workgroup by operand loads, 16 ML through LDS.
-template <typename OUT, bool XF32, int NW, int MT, int ML, bool AD>
-hipError_t launch_few_rows_of(const Q8GemmParams &p, hipStream_t s) {
-  const auto grid = [&](int mt) { return dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * mt - 1) / (16 * mt))); };
-  if (NW > 4 || (p.K >= 512 && grid(ML).y <= 65535)) {  // more than 4 wavefronts: K past 512, few tiles
-    hipLaunchKernelGGL((q8_0_few_rows_lds_kernel<OUT, XF32, NW, ML, AD>), grid(ML), dim3(64 * NW), 0, s, p);
-  } else if constexpr (NW == 4) {
-    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, NW, MT, AD>), grid(MT), dim3(64 * NW), 0, s, p);
-  }
+template <typename OUT, bool XF32, int NW, int MT, bool AD>
+hipError_t launch_few_rows_lds(const Q8GemmParams &p, hipStream_t s) {
+  // a grid's y and z end at 65535
+  const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), z = (tm + 65534) / 65535;
+  const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)((tm + z - 1) / z), (unsigned)z);
+  hipLaunchKernelGGL((q8_0_few_rows_lds_kernel<OUT, XF32, NW, MT, AD>), grid, dim3(64 * NW), 0, s, p);
   return hipGetLastError();
 }
 
-template <typename OUT, bool XF32, int MT, int ML, bool AD>
-hipError_t launch_few_rows(const Q8GemmParams &p, hipStream_t s) {
-  // 2048 wavefronts (two per SIMD), or as many as k has chunk pairs
-  const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * MT - 1) / (16 * MT);
-  if (tn > INT32_MAX || tm > 65535) return hipErrorInvalidValue;
-  if (tn * tm * 4 >= 2048 || p.K <= 512) return launch_few_rows_of<OUT, XF32, 4, MT, ML, AD>(p, s);
-  if (tn * tm * 8 >= 2048 || p.K <= 1024) return launch_few_rows_of<OUT, XF32, 8, MT, ML, AD>(p, s);
-  return launch_few_rows_of<OUT, XF32, 16, MT, ML, AD>(p, s);
-}
+// rows of the tile that was chosen: 16, or 64 (two of two row tiles of 16)
 template <typename OUT, bool XF32, bool AD>
 hipError_t launch_few_rows(const Q8GemmParams &p, int rows, hipStream_t s) {
-  if (rows == 16) return launch_few_rows<OUT, XF32, 1, 1, AD>(p, s);
-  return launch_few_rows<OUT, XF32, 4, 2, AD>(p, s);
+  // 2048 wavefronts (two per SIMD), or as many as k has chunk pairs
+  const int64_t tn = (p.N + 15) / 16, tm = (p.M + rows - 1) / rows;
+  if (tn > INT32_MAX || p.M > kFewRowsMaxM) return hipErrorInvalidValue;
+  const int nw = tn * tm * 4 >= 2048 || p.K <= 512 ? 4 : tn * tm * 8 >= 2048 || p.K <= 1024 ? 8 : 16;
+  if (rows > 16) {
+    if (nw == 4) return launch_few_rows_lds<OUT, XF32, 4, 2, AD>(p, s);
+    return nw == 8 ? launch_few_rows_lds<OUT, XF32, 8, 2, AD>(p, s) : launch_few_rows_lds<OUT, XF32, 16, 2, AD>(p, s);
+  }
+  if (p.K < 512) {
+    hipLaunchKernelGGL((q8_0_few_rows_kernel<OUT, XF32, AD>), dim3((unsigned)tn), dim3(256), 0, s, p);
+    return hipGetLastError();
+  }
+  if (nw == 4) return launch_few_rows_lds<OUT, XF32, 4, 1, AD>(p, s);
+  return nw == 8 ? launch_few_rows_lds<OUT, XF32, 8, 1, AD>(p, s) : launch_few_rows_lds<OUT, XF32, 16, 1, AD>(p, s);
 }
 
 template <typename OUT, bool AD, int WM, int WN, int TI, int TJ, int KG>

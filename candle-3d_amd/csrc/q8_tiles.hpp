@@ -6,9 +6,9 @@
 
 namespace lux3d {
 
-// Few: the few-rows kernels, rows x 16 (rows 16: one row tile, 64: four, or
-// twice two through LDS, which the costs below do not know: they keep every
-// size at the kernel, and the bits, that it had);
+// Few: the few-rows kernels, rows x 16 (rows 16: one row tile; 64: two
+// workgroups of two row tiles. The costs below are those of an earlier kernel
+// of four and keep every size at the bits that it had);
 // else a GEMM tile of rows x cols whose k is shared by `groups` groups of
 // wavefronts.
 struct Q8Tile {
@@ -21,7 +21,7 @@ inline double q8_tiles(int64_t m, int64_t n, int64_t bm, int64_t bn) {
 }
 inline double q8_rounds(double tiles) { return std::ceil(tiles / 256); }
 
-// The few-rows kernel's grid: its row tiles are the launch's y, at most 65535.
+// Beyond this many rows another kernel takes the call.
 constexpr int64_t kFewRowsMaxM = 65535 * 64;
 
 // f32 activations: the kernel and tile that take the shortest time by these
