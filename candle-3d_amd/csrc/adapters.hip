@@ -2,9 +2,10 @@
 // segment has an adapter (the second, t B^T, joins the GEMM's accumulators, adapters.hpp).
 //
 // What bounds it: x's bytes, or for few rows the latency of one load after the other. A workgroup takes 16 rows of one
-// segment (past 256 segments: 16 rows, segment after segment) and 16 NT values of the rank; its wavefronts take 128-byte chunks of the rows in turn and their sums are added in
-// wavefront order through LDS (v_mfma_f32_16x16x32_bf16, f32 sums; f32 x: v_mfma_f32_16x16x4_f32). A chunk goes through
-// LDS, 8 lanes to a row: loaded as the matrix operand's lanes hold it, a row a lane, the cache serves 16 bytes a cycle.
+// segment (past 256 segments: 16 rows, segment after segment) and 16 NT values of the rank; its wavefronts take 128-byte
+// chunks of the rows in turn and their sums are added in wavefront order through LDS (v_mfma_f32_16x16x32_bf16, f32 sums;
+// f32 x: v_mfma_f32_16x16x4_f32). A chunk goes through LDS, 8 lanes to a row: loaded as the matrix operand's lanes hold it,
+// a row a lane, the cache serves 16 bytes a cycle.
 // us, operand loads / through LDS: 4096 x 2048 rank 64 bf16 15.4 / 9.7, 3087 x 4096 rank 32 f32 26 / 18, 9001 x 1536 rank
 // 12 bf16 11.0 / 8.1, 12 x 1536 rank 16 5.0 / 4.4 (50 MB of f32 x: 10.4 us at the copy rate). t is rounded once to x's
 // type, as an activation between two linear layers is.
@@ -202,7 +203,10 @@ hipError_t launch_down(const AdapterDownParams &p, hipStream_t s) {
 
 template <bool XF32, int NT>
 hipError_t launch_down(const AdapterDownParams &p, hipStream_t s) {
-  // us with 4 / 8 wavefronts: 9001 rows of 1536 8.1 / 9.0, 4096 of 2048 10.1 / 9.7, 3087 of 4096 in f32 20.1 / 18.0
+  // us of a call with 64 columns, with 4 / 8 wavefronts in this kernel: 1024 x 4096 f32 rank 8 31.9 / 27.7, 3087 x 2048 bf16
+  // rank 8 18.8 / 17.7, 32768 x 1024 bf16 rank 32 37.4 / 43.0; over 24 sizes each, 8 take 0.94 of the time at 1024 rows, 0.97
+  // at 3087, and 1.02 from 4096 rows on (0.98 to 1.07 up to 8192). The border stays above where the two meet: another number
+  // of wavefronts is another order of t's sums.
   return p.M > 8192 ? launch_down<XF32, NT, 4>(p, s) : launch_down<XF32, NT, 8>(p, s);
 }
 
