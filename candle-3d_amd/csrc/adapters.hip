@@ -8,7 +8,8 @@
 // a row a lane, the cache serves 16 bytes a cycle.
 // us, operand loads / through LDS: 4096 x 2048 rank 64 bf16 15.4 / 9.7, 3087 x 4096 rank 32 f32 26 / 18, 9001 x 1536 rank
 // 12 bf16 11.0 / 8.1, 12 x 1536 rank 16 5.0 / 4.4 (50 MB of f32 x: 10.4 us at the copy rate). t is rounded once to x's
-// type, as an activation between two linear layers is.
+// type, as an activation between two linear layers is, and as the second product's operands are (error of y against 64
+// bits 0.0019 of its norm in bf16, 0.0017 by y's own rounding alone).
 #include "adapters.hpp"
 
 namespace lux3d {

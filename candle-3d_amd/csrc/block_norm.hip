@@ -309,8 +309,9 @@ hipError_t launch_block_norm_t(const BlockNormParams &p, bool vec, hipStream_t s
     // Two or three workgroups a CU walk the rows, four at a time: three where they take no more turns in all. us with 2 / 3
     // of them (inputs warm): RMS 3000 x 1536 bf16 11.8 / 8.9, LayerNorm 4098 x 2048 f16 17.2 / 15.5, 12000 x 1024 f32 36.9 /
     // 35.6, 64000 x 1536 bf16 159 / 155, but 2048 x 2048 f32 14.9 / 16.6, 8192 x 1024 bf16 13.5 / 13.9, 32768 x 2048 f16 104 /
-    // 110; rows that end inside a chunk gain less (24000 x 1000 bf16 41.6 / 43.8). f32 rows above 1024 gain from 12000 rows on only (78.6 / 74.8; 4098 x 2048 26.5 / 29.6). A workgroup a row takes
-    // 1.2 to 1.7 times as long from 3000 rows of 2 bytes on, and 0.6 to 0.95 of it at 1029.
+    // 110. Rows that end inside a chunk gain less (24000 x 1000 bf16 41.6 / 43.8), f32 rows above 1024 from 12000 rows on only
+    // (78.6 / 74.8; 4098 x 2048 26.5 / 29.6). A workgroup a row takes 1.2 to 1.7 times as long from 3000 rows of 2 bytes on,
+    // and 0.6 to 0.95 of it at 1029.
     const int nc = (int)((chunks + 63) / 64);
     const int64_t cus = cu_count(s);
     auto turns = [&](int64_t wgs) { return wgs * (((p.rows + wgs * cus - 1) / (wgs * cus) + 3) / 4); };

@@ -536,8 +536,9 @@ __device__ __forceinline__ int64_t segment_of(const int64_t *off, int64_t nseg, 
     return s < nseg ? s : nseg - 1;
   }
   // read through the constant address space: with r uniform over the
-  // wavefront (every caller) these are scalar loads, counted by lgkmcnt, so
-  // the search does not wait on the wavefront's outstanding vector loads
+  // wavefront (every caller but adapter_dot, whose lanes hold rows of their
+  // own) these are scalar loads, counted by lgkmcnt, so the search does not
+  // wait on the wavefront's outstanding vector loads
   typedef const __attribute__((address_space(4))) int64_t *coff_t;
   const coff_t c = (coff_t)off;
   int64_t lo = 0, hi = nseg - 1;

@@ -230,7 +230,7 @@ hipError_t launch_attention(int dt, const AttnParams &p, hipStream_t s);
 // Attention of a batch that shares a prefix of keys (prefix_attention.hip):
 // q, o [B, H, Lq, D]; pk, pv [Hkv, P, D]; k, v [B, Hkv, Ls, D], G = H / Hkv;
 // lens [B] (own keys of a sequence, clamped to 0 .. Ls) or null: Ls. `mfma`
-// selects the matrix-core kernels (2-byte types, D 64 or 128, every row
+// selects the matrix-core kernels (each type, D 64 or 128, every row
 // 16-byte aligned, block offsets below 2^31 bytes), which follow `plan` and
 // use ws where it has several parts; otherwise the generic kernel.
 struct PrefixParams {
