@@ -512,7 +512,7 @@ def _q8_linear(dev, cfg, m, k, n, what, xdt=torch.bfloat16, name="") -> Workload
                       f"x[{m},{k}] f32 @ W[{n},{k}]^T ({what})", launch, n_sets, flops=2 * m * k * n,
                       peak_tflops=2500.0 / 3)
     else:
-        kern = "q8_0_few_rows_kernel<BF16>" if m <= 16 else "q8_0_gemm_ring_kernel<BF16,...>"
+        kern = "q8_0_few_rows_lds_kernel<BF16>" if m <= 16 else "q8_0_gemm_ring_kernel<BF16,...>"
         wl = Workload(name or "q8_0_linear", cfg, kern, "bf16 x int8(Q8_0) -> f32 acc", nbytes,
                       f"x[{m},{k}] @ W[{n},{k}]^T ({what})", launch, n_sets, flops=2 * m * k * n)
     wl._keep = (xs, ys, qs, scales, bias, blocks, dx, dy, dq, dsc, db)
