@@ -1100,6 +1100,166 @@ int lux3d_q8_0_linear_int8(const lux3d_tensor_t *x, const lux3d_tensor_t *qs, co
 }
 
 namespace {
+// A packed microscaled matrix [rows, k]: q u8 [..., k / 2], scales u8 [ceil(k / 128), rows, 4].
+struct MxView {
+  uint8_t *q = nullptr, *s = nullptr;
+  int64_t rows = 0, k = 0;
+};
+int mx_packed(const char *fn, const lux3d_tensor_t *q, const char *qn, const lux3d_tensor_t *s, const char *sn, MxView &v) {
+  int r;
+  if ((r = check_desc(q, fn, qn)) || (r = check_desc(s, fn, sn))) return r;
+  if (q->dtype != LUX3D_U8 || s->dtype != LUX3D_U8) return fail(LUX3D_ERR_DTYPE, "%s: `%s` and `%s` must be u8", fn, qn, sn);
+  if (q->rank < 2) return fail(LUX3D_ERR_SHAPE, "%s: `%s` must be [rows, k / 2]", fn, qn);
+  const int64_t half = q->shape[q->rank - 1];
+  if (half == 0 || half % 16) return fail(LUX3D_ERR_SHAPE, "%s: `%s` has %lld bytes a row: k must be a positive multiple of 32", fn, qn,
+                                          (long long)half);
+  v.k = 2 * half;
+  v.rows = 1;
+  for (int i = 0; i < q->rank - 1; ++i) v.rows *= q->shape[i];
+  const int64_t groups = (v.k + 127) / 128;
+  if (s->rank != 3 || s->shape[0] != groups || s->shape[1] != v.rows || s->shape[2] != 4)
+    return fail(LUX3D_ERR_SHAPE, "%s: `%s` must be [%lld, %lld, 4] for [%lld, %lld] values", fn, sn, (long long)groups,
+                (long long)v.rows, (long long)v.rows, (long long)v.k);
+  if (!is_contiguous(q) || !is_contiguous(s)) return fail(LUX3D_ERR_LAYOUT, "%s: `%s` and `%s` must be contiguous", fn, qn, sn);
+  if (!aligned16(q->data) || (reinterpret_cast<uintptr_t>(s->data) & 3u))
+    return fail(LUX3D_ERR_LAYOUT, "%s: `%s` must be 16-byte and `%s` 4-byte aligned", fn, qn, sn);
+  v.q = reinterpret_cast<uint8_t *>(q->data);
+  v.s = reinterpret_cast<uint8_t *>(s->data);
+  return LUX3D_OK;
+}
+
+// Plain rows beside a packed matrix: any float type, 16-byte aligned rows.
+int mx_rows(const char *fn, const lux3d_tensor_t *t, const char *name, RowView &v) {
+  int r;
+  if ((r = row_tensor(t, fn, name, -1, v))) return r;
+  if (v.d % 32 || v.d == 0) return fail(LUX3D_ERR_SHAPE, "%s: `%s` rows must hold a positive multiple of 32 values", fn, name);
+  if (!aligned16(v.p) || (v.rows > 1 && (v.rs * elem_bytes(t->dtype)) % 16))
+    return fail(LUX3D_ERR_LAYOUT, "%s: `%s` rows must be 16-byte aligned", fn, name);
+  return LUX3D_OK;
+}
+
+int mx_bias(const char *fn, const lux3d_tensor_t *b, const char *name, int64_t n, const float *&to) {
+  to = nullptr;
+  if (!b) return LUX3D_OK;
+  int r;
+  if ((r = check_desc(b, fn, name))) return r;
+  if (b->dtype != LUX3D_F32 || !is_contiguous(b) || numel(b) != n)
+    return fail(LUX3D_ERR_SHAPE, "%s: `%s` must be a contiguous f32 [%lld]", fn, name, (long long)n);
+  to = reinterpret_cast<const float *>(b->data);
+  return LUX3D_OK;
+}
+
+// x, packed or plain, and y of a linear on packed weights [n, k], in p.
+int mx_linear(const char *fn, const lux3d_tensor_t *x, const lux3d_tensor_t *xq, const lux3d_tensor_t *xs, bool fp4, int64_t n,
+              int64_t k, const lux3d_tensor_t *y, MxLinearParams &p) {
+  int r;
+  RowView xv{nullptr, 0, k, 0}, yv;
+  if (x || !fp4) {
+    if ((r = mx_rows(fn, x, "x", xv))) return r;
+    p.x = xv.p; p.ldx = xv.rs; p.x_dt = x->dtype;
+  }
+  p.fp4 = fp4;
+  if (fp4 && (!x || xq || xs || xv.rows > kMxFewRows)) {
+    MxView v;
+    if ((r = mx_packed(fn, xq, "xq", xs, "xs", v))) return r;
+    if (x && (v.rows != xv.rows || v.k != xv.d))
+      return fail(LUX3D_ERR_SHAPE, "%s: `xq` holds [%lld, %lld] values, x [%lld, %lld]", fn, (long long)v.rows, (long long)v.k,
+                  (long long)xv.rows, (long long)xv.d);
+    p.xq = v.q; p.xs = v.s;
+    xv.rows = v.rows; xv.d = v.k;
+  }
+  if (xv.d != k) return fail(LUX3D_ERR_SHAPE, "%s: x has %lld features, the weight %lld", fn, (long long)xv.d, (long long)k);
+  if ((r = row_tensor(y, fn, "y", -1, yv))) return r;
+  if (yv.d != n || yv.rows != xv.rows)
+    return fail(LUX3D_ERR_SHAPE, "%s: y must be [%lld, %lld]", fn, (long long)xv.rows, (long long)n);
+  p.y = const_cast<void *>(yv.p); p.ldy = yv.rs; p.y_dt = y->dtype;
+  p.M = xv.rows; p.N = n; p.K = k;
+  return LUX3D_OK;
+}
+}  // namespace
+
+int lux3d_mxfp4_quantize(const lux3d_tensor_t *x, const lux3d_tensor_t *q, const lux3d_tensor_t *scales,
+                         lux3d_stream_t stream) {
+  const char *fn = "lux3d_mxfp4_quantize";
+  RowView xv;
+  MxView v;
+  int r;
+  if ((r = mx_rows(fn, x, "x", xv)) || (r = mx_packed(fn, q, "q", scales, "scales", v))) return r;
+  if (v.rows != xv.rows || v.k != xv.d)
+    return fail(LUX3D_ERR_SHAPE, "%s: `q` holds [%lld, %lld] values, x [%lld, %lld]", fn, (long long)v.rows, (long long)v.k,
+                (long long)xv.rows, (long long)xv.d);
+  const MxQuantParams p = {xv.p, xv.rs, x->dtype, v.q, v.s, v.rows, v.k};
+  return hip_status(launch_mx_quantize(p, stream_of(stream)), fn);
+}
+
+int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales, const lux3d_tensor_t *y,
+                           lux3d_stream_t stream) {
+  const char *fn = "lux3d_mxfp4_dequantize";
+  RowView yv;
+  MxView v;
+  int r;
+  if ((r = mx_packed(fn, q, "q", scales, "scales", v)) || (r = mx_rows(fn, y, "y", yv))) return r;
+  if (v.rows != yv.rows || v.k != yv.d)
+    return fail(LUX3D_ERR_SHAPE, "%s: y must be [%lld, %lld]", fn, (long long)v.rows, (long long)v.k);
+  const MxDequantParams p = {v.q, v.s, const_cast<void *>(yv.p), yv.rs, y->dtype, v.rows, v.k};
+  return hip_status(launch_mx_dequantize(p, stream_of(stream)), fn);
+}
+
+int lux3d_mxfp4_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *w, const lux3d_tensor_t *w_scales,
+                       const lux3d_tensor_t *bias, const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_mxfp4_linear";
+  MxLinearParams p;
+  MxView v;
+  int r;
+  if ((r = mx_packed(fn, w, "w", w_scales, "w_scales", v)) || (r = mx_bias(fn, bias, "bias", v.rows, p.bias[0])) ||
+      (r = mx_linear(fn, x, nullptr, nullptr, false, v.rows, v.k, y, p)))
+    return r;
+  p.w[0] = v.q; p.ws[0] = v.s;
+  return hip_status(launch_mx_linear(p, stream_of(stream)), fn);
+}
+
+int lux3d_mxfp4_linear_fp4(const lux3d_tensor_t *x, const lux3d_tensor_t *xq, const lux3d_tensor_t *xs,
+                           const lux3d_tensor_t *w, const lux3d_tensor_t *w_scales, const lux3d_tensor_t *bias,
+                           const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_mxfp4_linear_fp4";
+  MxLinearParams p;
+  MxView v;
+  int r;
+  if ((r = mx_packed(fn, w, "w", w_scales, "w_scales", v)) || (r = mx_bias(fn, bias, "bias", v.rows, p.bias[0])) ||
+      (r = mx_linear(fn, x, xq, xs, true, v.rows, v.k, y, p)))
+    return r;
+  p.w[0] = v.q; p.ws[0] = v.s;
+  return hip_status(launch_mx_linear(p, stream_of(stream)), fn);
+}
+
+int lux3d_mxfp4_linear_gated(const lux3d_tensor_t *x, const lux3d_tensor_t *xq, const lux3d_tensor_t *xs,
+                             const lux3d_tensor_t *gate, const lux3d_tensor_t *gate_scales, const lux3d_tensor_t *gate_bias,
+                             const lux3d_tensor_t *up, const lux3d_tensor_t *up_scales, const lux3d_tensor_t *up_bias,
+                             int32_t act, int32_t fp4, const lux3d_tensor_t *y, lux3d_stream_t stream) {
+  const char *fn = "lux3d_mxfp4_linear_gated";
+  MxLinearParams p;
+  MxView g, u;
+  int r;
+  if (act != ACT_GELU_ERF && act != ACT_GELU_TANH && act != ACT_SILU)
+    return fail(LUX3D_ERR_VALUE, "%s: unknown activation %d", fn, act);
+  if (fp4 != 0 && fp4 != 1) return fail(LUX3D_ERR_VALUE, "%s: fp4 must be 0 or 1", fn);
+  if (!fp4 && (xq || xs)) return fail(LUX3D_ERR_VALUE, "%s: `xq` and `xs` belong to fp4 1", fn);
+  if ((r = mx_packed(fn, gate, "gate", gate_scales, "gate_scales", g)) ||
+      (r = mx_packed(fn, up, "up", up_scales, "up_scales", u)))
+    return r;
+  if (g.rows != u.rows || g.k != u.k)
+    return fail(LUX3D_ERR_SHAPE, "%s: `gate` is [%lld, %lld], `up` [%lld, %lld]", fn, (long long)g.rows, (long long)g.k,
+                (long long)u.rows, (long long)u.k);
+  if ((r = mx_bias(fn, gate_bias, "gate_bias", g.rows, p.bias[1])) || (r = mx_bias(fn, up_bias, "up_bias", u.rows, p.bias[0])) ||
+      (r = mx_linear(fn, x, xq, xs, fp4 != 0, u.rows, u.k, y, p)))
+    return r;
+  p.w[0] = u.q; p.ws[0] = u.s;
+  p.w[1] = g.q; p.ws[1] = g.s;
+  p.act = act;
+  return hip_status(launch_mx_linear(p, stream_of(stream)), fn);
+}
+
+namespace {
 // Validates q, k, v, out for attention and fills the strides; `mfma` tells
 // whether every row is 16-byte aligned with D 64 / 128. `f32_out_ok`: out
 // may also be f32 when q, k, v are 2-byte.

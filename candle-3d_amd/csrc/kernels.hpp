@@ -180,6 +180,42 @@ struct Q8IntParams {
 hipError_t launch_q8_0_quantize_rows(const Q8IntParams &p, hipStream_t s);
 hipError_t launch_q8_0_int8_gemm(const Q8IntParams &p, hipStream_t s);
 
+// ---- microscaled 4-bit values (mxfp4.hip, mxfp4_gemm.hip; the format: mxfp4.hpp) --
+// A packed matrix [rows, K]: q [rows, K / 2] bytes, s [ceil(K / 128), rows, 4].
+// Up to this many rows a linear's own kernel quantises x as it reads it.
+constexpr int64_t kMxFewRows = 16;
+
+struct MxQuantParams {
+  const void *x = nullptr; int64_t ldx = 0; int x_dt = 0;  // [M, K] rows, 16-byte aligned
+  uint8_t *q = nullptr, *s = nullptr;                      // packed, q 16-byte and s 4-byte aligned
+  int64_t M = 0, K = 0;
+};
+hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s);
+struct MxDequantParams {
+  const uint8_t *q = nullptr, *s = nullptr;
+  void *y = nullptr; int64_t ldy = 0; int y_dt = 0;        // [M, K] rows, 16-byte aligned
+  int64_t M = 0, K = 0;
+};
+hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s);
+
+// The polynomial of a gated linear's activation (mxfp4.hpp, mx_activate).
+struct MxAct {
+  float p[9];
+  float top;  // v^2 enters the polynomial no larger than this
+};
+// y = x W^T + bias, or act(x W1^T + bias1) * (x W0^T + bias0).
+struct MxLinearParams {
+  const void *x = nullptr; int64_t ldx = 0; int x_dt = -1;  // [M, K] rows, 16-byte aligned; null: packed x given
+  bool fp4 = false;                                         // x enters in 4 bits
+  uint8_t *xq = nullptr, *xs = nullptr;                     // packed x: given, or written here (fp4, more than kMxFewRows rows)
+  const uint8_t *w[2] = {nullptr, nullptr}, *ws[2] = {nullptr, nullptr};  // packed [N, K]; 1: the gate
+  const float *bias[2] = {nullptr, nullptr};                // [N] or null
+  int act = -1;                                             // Act; -1: no gate
+  void *y = nullptr; int64_t ldy = 0; int y_dt = 0;         // [M, N] rows
+  int64_t M = 0, N = 0, K = 0;
+};
+hipError_t launch_mx_linear(const MxLinearParams &p, hipStream_t s);
+
 // Scaled dot-product attention over [B, H, L, D] views (element strides per
 // batch, head and token; unit inner stride). out = softmax(q k^T * scale) v.
 // `mfma` selects the matrix-core kernels (D 64 or 128, every row

@@ -1,0 +1,311 @@
+// mxfp4.hip -- microscaled 4-bit values on gfx950: quantisation, its inverse,
+// and the linear layers of few rows (mxfp4.hpp: the format).
+#include <type_traits>
+
+#include "mxfp4.hpp"
+
+namespace lux3d {
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+// ---- quantisation ---------------------------------------------------------------
+//
+// A stream: x read once, 17 / 32 byte a value written. A workgroup takes 32
+// rows x 512 values; a wavefront reads a row's 512 with 8 values a lane (4
+// lanes a block, the block's maximum by two DPP steps), 8 rows in flight, and
+// writes 256 contiguous bytes of codes a row. The scales go through LDS: a
+// group's bytes of 32 rows are one 128-byte line.
+constexpr int kQuantRows = 32, kQuantCols = 512;
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
+  constexpr int NV = T::bytes == 4 ? 2 : 1, R = kQuantRows / 4;  // 16-byte loads a lane and row; rows a wavefront
+  __shared__ uint32_t sc[4][kQuantRows];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
+  const int64_t r0 = rt * kQuantRows, k = kt * kQuantCols + lane * 8;
+  const bool live = k < p.K;
+  uint32_t v[R][4 * NV];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t r = r0 + wave * R + i;
+#pragma unroll
+    for (int j = 0; j < 4 * NV; ++j) v[i][j] = 0;
+    if (live && r < p.M) {
+      const char *src = reinterpret_cast<const char *>(p.x) + (r * p.ldx + k) * T::bytes;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint4 u = ld16(src + 16 * j);
+        v[i][4 * j] = u.x;
+        v[i][4 * j + 1] = u.y;
+        v[i][4 * j + 2] = u.z;
+        v[i][4 * j + 3] = u.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t r = r0 + wave * R + i;
+    uint32_t top = mx_top<T>(v[i]);
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, DPP_XOR1, 0xF, 0xF, false));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, DPP_XOR2, 0xF, 0xF, false));
+    const uint32_t s = mx_scale(top);  // values past K count as 0: so do the scales that fill up the last group
+    const uint32_t codes = mx_codes<T>(v[i], s);
+    if (live && r < p.M) *reinterpret_cast<uint32_t *>(p.q + (r * p.K + k) / 2) = codes;
+    if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(&sc[lane >> 4][wave * R + i])[(lane >> 2) & 3] = (uint8_t)s;
+  }
+  __syncthreads();
+  const int64_t g = kt * 4 + (t >> 5), r = r0 + (t & 31);
+  if (t < 128 && g * 128 < p.K && r < p.M) reinterpret_cast<uint32_t *>(p.s)[g * p.M + r] = sc[t >> 5][t & 31];
+}
+
+// ---- and back -------------------------------------------------------------------
+//
+// 16 values a lane (8 bytes of codes), so that a wavefront writes 2 KB (2-byte
+// types) of one row.
+template <typename T>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
+  const int64_t per = (p.K + 15) / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.M * per) return;
+  const int64_t r = i / per, k = (i - r * per) * 16;
+  const uint2 c = *reinterpret_cast<const uint2 *>(p.q + (r * p.K + k) / 2);
+  const uint32_t s = p.s[((k >> 7) * p.M + r) * 4 + ((k >> 5) & 3)];
+  char *dst = reinterpret_cast<char *>(p.y) + (r * p.ldy + k) * T::bytes;
+  if constexpr (T::code == LUX3D_F32) {
+    const float sc = __uint_as_float(s << 23);
+    const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 1);
+      const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 3);
+      st16(dst + 32 * j, make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])));
+      st16(dst + 32 * j + 16, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(e[0]), __float_as_uint(e[1])));
+    }
+  } else {
+    const u32x4_t a = mx_values8<T>(c.x, s), b = mx_values8<T>(c.y, s);
+    st16(dst, make_uint4(a[0], a[1], a[2], a[3]));
+    st16(dst + 16, make_uint4(b[0], b[1], b[2], b[3]));
+  }
+}
+
+// ---- linear, few rows -----------------------------------------------------------
+//
+// A workgroup owns 16 weight rows (of each matrix) and MT tiles of 16 rows of
+// x; its NW wavefronts take groups of 128 of k in turn and add their sums in
+// wavefront order through LDS. Lane l holds row l % 16 and block l / 16 of the
+// group of either operand: 16 bytes of a packed row, 32 values of a plain one.
+//   fp4    one v_mfma_scale_f32_16x16x128_f8f6f4 a group, each lane's scale its
+//          own block's; plain x is quantised in the lane that holds the block
+//   plain  four v_mfma_f32_16x16x32 on the block's four eighths; the weights'
+//          values are exact in bf16; f32 x in three exact bf16 terms
+template <typename X, bool FP4, bool GATED, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAct act) {
+  constexpr bool PACKED = std::is_void_v<X>;
+  constexpr int NM = GATED ? 2 : 1;
+  __shared__ float part[NW][NM][MT][256];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, l16 = lane & 15;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 16 * MT;
+  if (m0 >= p.M) return;  // uniform
+  const int64_t n = n0 + l16 < p.N ? n0 + l16 : p.N - 1;  // past N: clamped, never stored
+  const int64_t nb = p.K / 32, groups = (nb + 3) / 4;
+  f32x4_t acc[NM][MT];
+#pragma unroll
+  for (int j = 0; j < NM; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
+  for (int64_t c = wave; c < groups; c += NW) {
+    const int64_t b = 4 * c + g;
+    const bool live = b < nb;  // a last group may have fewer than four blocks: the others count as 0
+    uint4 w[NM];
+    uint32_t sw[NM];
+#pragma unroll
+    for (int j = 0; j < NM; ++j) {
+      w[j] = ld16<false>(p.w[j] + n * (p.K / 2) + (live ? b : nb - 1) * 16);
+      sw[j] = live ? p.ws[j][(c * p.N + n) * 4 + g] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + 16 * i + l16;
+      const bool have = live && m < p.M;
+      if constexpr (FP4) {
+        u32x4_t xc = u32x4_t{};
+        uint32_t sx = 0;
+        if constexpr (PACKED) {
+          if (have) {
+            const uint4 u = ld16<false>(p.xq + m * (p.K / 2) + b * 16);
+            xc = u32x4_t{u.x, u.y, u.z, u.w};
+            sx = p.xs[(c * p.M + m) * 4 + g];
+          }
+        } else {
+          constexpr int NV = X::bytes * 2;  // 16-byte loads of a block
+          uint32_t v[4 * NV];
+#pragma unroll
+          for (int e = 0; e < 4 * NV; ++e) v[e] = 0;
+          if (have) {
+            const char *src = reinterpret_cast<const char *>(p.x) + (m * p.ldx + b * 32) * X::bytes;
+#pragma unroll
+            for (int e = 0; e < NV; ++e) {
+              const uint4 u = ld16<false>(src + 16 * e);
+              v[4 * e] = u.x;
+              v[4 * e + 1] = u.y;
+              v[4 * e + 2] = u.z;
+              v[4 * e + 3] = u.w;
+            }
+          }
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, mx_top<X>(v + e * NV));
+          sx = mx_scale(top);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xc[e] = mx_codes<X>(v + e * NV, sx);
+        }
+        const i32x8_t xb = {(int)xc[0], (int)xc[1], (int)xc[2], (int)xc[3], 0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NM; ++j) {
+          const i32x8_t wa = {(int)w[j].x, (int)w[j].y, (int)w[j].z, (int)w[j].w, 0, 0, 0, 0};
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[j][i], 4, 4, 0, (int)sw[j], 0, (int)sx);
+        }
+      } else {
+        constexpr int NV = X::bytes * 2;
+        uint4 v[NV];
+#pragma unroll
+        for (int e = 0; e < NV; ++e) v[e] = make_uint4(0, 0, 0, 0);
+        if (have) {
+          const char *src = reinterpret_cast<const char *>(p.x) + (m * p.ldx + b * 32) * X::bytes;
+#pragma unroll
+          for (int e = 0; e < NV; ++e) v[e] = ld16<false>(src + 16 * e);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          u32x4_t x1, x2, x3;
+          if constexpr (X::code == LUX3D_F32) {
+            const uint32_t f[8] = {v[2 * s].x, v[2 * s].y, v[2 * s].z, v[2 * s].w, v[2 * s + 1].x, v[2 * s + 1].y, v[2 * s + 1].z, v[2 * s + 1].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const Split3 r = split3_bf16(__uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1]));
+              x1[e] = r.t1;
+              x2[e] = r.t2;
+              x3[e] = r.t3;
+            }
+          } else {
+            x1 = u32x4_t{v[s].x, v[s].y, v[s].z, v[s].w};
+          }
+#pragma unroll
+          for (int j = 0; j < NM; ++j) {
+            const uint32_t ws = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w;
+            if constexpr (X::code == LUX3D_F16) {
+              acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, mx_values8<F16>(ws, sw[j])),
+                                                                 __builtin_bit_cast(f16x8_t, x1), acc[j][i], 0, 0, 0);
+            } else {
+              const bf16x8_t wv = __builtin_bit_cast(bf16x8_t, mx_values8<BF16>(ws, sw[j]));
+              if constexpr (X::code == LUX3D_F32) {
+                acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x3), acc[j][i], 0, 0, 0);
+                acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x2), acc[j][i], 0, 0, 0);
+              }
+              acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x1), acc[j][i], 0, 0, 0);
+            }
+          }
+        }
+      }
+    }
+  }
+  // lane holds weight rows 4 g + e, x row l16 of each tile
+#pragma unroll
+  for (int j = 0; j < NM; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][j][i][e * 64 + lane] = acc[j][i][e];
+  __syncthreads();
+  for (int o = t; o < MT * 256; o += 64 * NW) {
+    const int c = o & 15, r = (o >> 4) & 15, i = o >> 8, at = (c & 3) * 64 + (c >> 2) * 16 + r;
+    const int64_t row = m0 + 16 * i + r, col = n0 + c;
+    if (row >= p.M || col >= p.N) continue;
+    float v[NM];
+#pragma unroll
+    for (int j = 0; j < NM; ++j) {
+      v[j] = part[0][j][i][at];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) v[j] += part[k][j][i][at];
+      if (p.bias[j]) v[j] += p.bias[j][col];
+    }
+    float y = v[0];
+    if constexpr (GATED) y *= mx_activate(act, v[NM - 1]);
+    mx_store(p.y, p.y_dt, row * p.ldy + col, y);
+  }
+}
+
+template <typename X, bool FP4, bool GATED>
+hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
+  const int mt = p.M <= 16 ? 1 : 2;
+  const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * mt - 1) / (16 * mt), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
+  if (tn > INT32_MAX || z > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)tn, (unsigned)((tm + z - 1) / z), (unsigned)z);
+  const MxAct act = mx_act(p.act);
+  if (mt == 1) hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, 1, 8>), grid, dim3(512), 0, s, p, act);
+  else hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, 2, 8>), grid, dim3(512), 0, s, p, act);
+  return hipGetLastError();
+}
+
+template <typename X, bool FP4>
+hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
+  return p.act >= 0 ? launch_rows_kernel<X, FP4, true>(p, s) : launch_rows_kernel<X, FP4, false>(p, s);
+}
+
+template <typename X> hipError_t launch_rows_x(const MxLinearParams &p, hipStream_t s) {
+  return p.fp4 ? launch_rows_kernel<X, true>(p, s) : launch_rows_kernel<X, false>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s) {
+  if (p.M <= 0) return hipSuccess;
+  const int64_t tiles = (p.K + kQuantCols - 1) / kQuantCols * ((p.M + kQuantRows - 1) / kQuantRows);
+  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)tiles);
+  switch (p.x_dt) {
+    case LUX3D_F32: hipLaunchKernelGGL(mx_quantize_kernel<F32>, grid, dim3(256), 0, s, p); break;
+    case LUX3D_BF16: hipLaunchKernelGGL(mx_quantize_kernel<BF16>, grid, dim3(256), 0, s, p); break;
+    case LUX3D_F16: hipLaunchKernelGGL(mx_quantize_kernel<F16>, grid, dim3(256), 0, s, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s) {
+  const int64_t blocks = (p.M * ((p.K + 15) / 16) + 255) / 256;
+  if (blocks <= 0) return hipSuccess;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks);
+  switch (p.y_dt) {
+    case LUX3D_F32: hipLaunchKernelGGL(mx_dequantize_kernel<F32>, grid, dim3(256), 0, s, p); break;
+    case LUX3D_BF16: hipLaunchKernelGGL(mx_dequantize_kernel<BF16>, grid, dim3(256), 0, s, p); break;
+    case LUX3D_F16: hipLaunchKernelGGL(mx_dequantize_kernel<F16>, grid, dim3(256), 0, s, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_linear(const MxLinearParams &given, hipStream_t s) {
+  MxLinearParams p = given;
+  if (p.M <= 0 || p.N <= 0) return hipSuccess;
+  if (p.fp4 && p.x && p.M > kMxFewRows) {
+    const MxQuantParams q = {p.x, p.ldx, p.x_dt, p.xq, p.xs, p.M, p.K};
+    if (hipError_t e = launch_mx_quantize(q, s)) return e;
+    p.x = nullptr;
+  }
+  if (!p.x) return launch_rows_kernel<void, true>(p, s);
+  switch (p.x_dt) {
+    case LUX3D_F32: return launch_rows_x<F32>(p, s);
+    case LUX3D_BF16: return launch_rows_x<BF16>(p, s);
+    case LUX3D_F16: return launch_rows_x<F16>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace lux3d

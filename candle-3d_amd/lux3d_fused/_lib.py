@@ -71,6 +71,11 @@ SIGNATURES = {
     "lux3d_q8_0_linear_adapters": [TP] * 12 + [S],
     "lux3d_q8_0_linear_int8": [TP, TP, TP, TP, TP, TP, TP, S],
     "lux3d_q8_0_quantize": [TP, TP, TP, S],
+    "lux3d_mxfp4_quantize": [TP, TP, TP, S],
+    "lux3d_mxfp4_dequantize": [TP, TP, TP, S],
+    "lux3d_mxfp4_linear": [TP] * 5 + [S],
+    "lux3d_mxfp4_linear_fp4": [TP] * 7 + [S],
+    "lux3d_mxfp4_linear_gated": [TP] * 9 + [ctypes.c_int32, ctypes.c_int32, TP, S],
     "lux3d_sdpa": [TP, TP, TP, ctypes.c_float, TP, S],
     "lux3d_sdpa_shared_prefix_workspace": [ctypes.c_int64] * 7,
     "lux3d_sdpa_shared_prefix_workspace_dtype": [ctypes.c_int32] + [ctypes.c_int64] * 7,

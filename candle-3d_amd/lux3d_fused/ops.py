@@ -522,6 +522,144 @@ class QMatMul:
         return q8_0_linear_adapters(xs, self.qs, self.scales, a, b, adapter_ids, **kw)
 
 
+# ---------------------------------------------------------------------------
+# Microscaled 4-bit weights
+# ---------------------------------------------------------------------------
+
+_MX_FEW_ROWS = 16  # LUX3D_MXFP4_FEW_ROWS: up to here a linear quantizes x as it reads it
+_ACTS = {"gelu_erf": 0, "gelu_tanh": 1, "silu": 2}
+
+
+def _mx_packed(rows: int, lead, k: int, device):
+    """Empty packed storage of [rows, k] values: codes u8 [*lead, k / 2], scales u8 [ceil(k / 128), rows, 4]."""
+    return (torch.empty((*lead, k // 2), dtype=torch.uint8, device=device),
+            torch.empty(((k + 127) // 128, rows, 4), dtype=torch.uint8, device=device))
+
+
+def mxfp4_quantize(x: torch.Tensor):
+    """x (f32, bf16 or f16) [..., k], k a multiple of 32 -> (q, scales): e2m1 codes, two a byte, u8 [..., k / 2], and
+    one exponent byte per 32 values, by groups of four blocks, u8 [ceil(k / 128), rows, 4]."""
+    fn = "lux3d_mxfp4_quantize"
+    _one_device(fn, x)
+    if x.dim() < 2 or x.shape[-1] == 0:
+        raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "x must be [..., k]")
+    with _device_of(x):
+        q, scales = _mx_packed(x.numel() // x.shape[-1], x.shape[:-1], x.shape[-1], x.device)
+        _lib.call(fn, _d(x), _d(q), _d(scales), _stream(x))
+    return q, scales
+
+
+def mxfp4_dequantize(q: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values of a packed matrix, in `dtype` (exact in f32 and bf16)."""
+    fn = "lux3d_mxfp4_dequantize"
+    _one_device(fn, q, scales)
+    if q.dim() < 2:
+        raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "q must be [..., k / 2]")
+    with _device_of(q):
+        y = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=dtype, device=q.device)
+        _lib.call(fn, _d(q), _d(scales), _d(y), _stream(q))
+    return y
+
+
+def mxfp4_scales(exponents: torch.Tensor) -> torch.Tensor:
+    """Exponent bytes u8 [rows, k / 32], as checkpoints hold them, to the grouped layout [ceil(k / 128), rows, 4] that the
+    operators take (once, at load)."""
+    rows, blocks = exponents.shape
+    groups = (blocks + 3) // 4
+    padded = exponents.new_zeros((rows, 4 * groups))
+    padded[:, :blocks] = exponents
+    return padded.view(rows, groups, 4).transpose(0, 1).contiguous()
+
+
+def mxfp4_linear(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 out_dtype=None) -> torch.Tensor:
+    """`Linear::forward` (runtime/nn_blocks.rs:83-93) on a packed weight [n, k], x as it is (f32, bf16 or f16 [..., k]):
+    x @ W^T (+ bias) -> [..., n] in out_dtype (default: x's)."""
+    fn = "lux3d_mxfp4_linear"
+    _one_device(fn, x, q, scales, bias)
+    with _device_of(x):
+        y = x.new_empty((*x.shape[:-1], q.shape[0]), dtype=out_dtype or x.dtype)
+        _lib.call(fn, _d(x), _d(q), _d(scales), _d(bias), _d(y), _stream(x))
+    return y
+
+
+def _mx_x(fn: str, x):
+    """(plain x or None, xq, xs, the tensor that leads) of an x that enters in 4 bits: a tensor, or the pair that
+    mxfp4_quantize gave. More rows than few take a workspace for x's packed form."""
+    if not isinstance(x, torch.Tensor):
+        return None, x[0], x[1], x[0]
+    if x.dim() < 1 or x.shape[-1] == 0 or not x.is_cuda:
+        return x, None, None, x
+    rows = x.numel() // x.shape[-1]
+    if rows <= _MX_FEW_ROWS:
+        return x, None, None, x
+    return (x, *_mx_packed(rows, (rows,), x.shape[-1], x.device), x)
+
+
+def mxfp4_linear_fp4(x, q: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                     out_dtype=None) -> torch.Tensor:
+    """mxfp4_linear with x in 4 bits too: quantized here (x a tensor), or the pair that mxfp4_quantize gave (one
+    quantization for several projections). out_dtype defaults to x's type, bf16 for a pair."""
+    fn = "lux3d_mxfp4_linear_fp4"
+    plain, xq, xs, lead = _mx_x(fn, x)
+    _one_device(fn, lead, xs, q, scales, bias)
+    with _device_of(lead):
+        dt = out_dtype or (torch.bfloat16 if plain is None else plain.dtype)
+        y = torch.empty((*lead.shape[:-1], q.shape[0]), dtype=dt, device=lead.device)
+        _lib.call(fn, _d(plain), _d(xq), _d(xs), _d(q), _d(scales), _d(bias), _d(y), _stream(lead))
+    return y
+
+
+def mxfp4_linear_gated(x, gate, up, act: str = "silu", *, gate_bias: Optional[torch.Tensor] = None,
+                       up_bias: Optional[torch.Tensor] = None, fp4: bool = False, out_dtype=None) -> torch.Tensor:
+    """act(x @ Wg^T + gate_bias) * (x @ Wu^T + up_bias) in one kernel, the first half of a gated feed-forward block
+    (GeGlu::forward, runtime/nn_blocks.rs:238-254, and its kin). gate, up: (q, scales) of packed weights [n, k]; act
+    "silu", "gelu_erf" or "gelu_tanh". fp4: x enters in 4 bits, as in mxfp4_linear_fp4 (a pair is possible then)."""
+    fn = "lux3d_mxfp4_linear_gated"
+    if act not in _ACTS:
+        raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"act must be one of {sorted(_ACTS)}, not {act!r}")
+    plain, xq, xs, lead = _mx_x(fn, x) if fp4 else (x, None, None, x)
+    _one_device(fn, lead, xs, *gate, gate_bias, *up, up_bias)
+    with _device_of(lead):
+        dt = out_dtype or (torch.bfloat16 if plain is None else plain.dtype)
+        y = torch.empty((*lead.shape[:-1], up[0].shape[0]), dtype=dt, device=lead.device)
+        _lib.call(fn, _d(plain), _d(xq), _d(xs), _d(gate[0]), _d(gate[1]), _d(gate_bias), _d(up[0]), _d(up[1]), _d(up_bias),
+                  _ACTS[act], 1 if fp4 else 0, _d(y), _stream(lead))
+    return y
+
+
+class Mxfp4MatMul:
+    """A linear layer's weight [n, k] in microscaled 4-bit form, as QMatMul is for Q8_0."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor):
+        self.q, self.scales = q, scales
+
+    @classmethod
+    def from_dense(cls, weight: torch.Tensor) -> "Mxfp4MatMul":
+        return cls(*mxfp4_quantize(weight))
+
+    def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
+        return mxfp4_dequantize(self.q, self.scales, dtype)
+
+    def forward(self, xs, bias: Optional[torch.Tensor] = None, out_dtype=None, fp4: bool = False) -> torch.Tensor:
+        return (mxfp4_linear_fp4 if fp4 else mxfp4_linear)(xs, self.q, self.scales, bias, out_dtype)
+
+
+class Mxfp4GatedMlp:
+    """A gated feed-forward block: down(act(gate(x)) * up(x)), three packed weights (GeGlu, runtime/nn_blocks.rs:238-254,
+    and the Linear after it). fp4: x and the hidden values enter their products in 4 bits."""
+
+    def __init__(self, gate: Mxfp4MatMul, up: Mxfp4MatMul, down: Mxfp4MatMul, act: str = "silu", *, gate_bias=None,
+                 up_bias=None, down_bias=None, fp4: bool = False):
+        self.gate, self.up, self.down, self.act, self.fp4 = gate, up, down, act, fp4
+        self.gate_bias, self.up_bias, self.down_bias = gate_bias, up_bias, down_bias
+
+    def forward(self, xs, out_dtype=None) -> torch.Tensor:
+        h = mxfp4_linear_gated(xs, (self.gate.q, self.gate.scales), (self.up.q, self.up.scales), self.act,
+                               gate_bias=self.gate_bias, up_bias=self.up_bias, fp4=self.fp4, out_dtype=out_dtype)
+        return self.down.forward(h, self.down_bias, out_dtype, self.fp4)
+
+
 def sdpa(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(q k^T * scale) v over [B, H, L, D] views, one kernel, no scores

@@ -434,6 +434,81 @@ int lux3d_q8_0_linear_int8(const lux3d_tensor_t *x, const lux3d_tensor_t *qs,
 int lux3d_q8_0_quantize(const lux3d_tensor_t *x, const lux3d_tensor_t *xq,
                         const lux3d_tensor_t *xd, lux3d_stream_t stream);
 
+/* ---- microscaled 4-bit weights ---------------------------------------------
+ * Half the bytes of Q8_0: 32 consecutive values of a row share a power of two,
+ * and each is e2m1 (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives). A packed
+ * matrix [rows, k], k a positive multiple of 32, is
+ *   q       u8 [rows, k / 2]: two codes a byte, the value of even k in the low
+ *           half; code = sign << 3 | index into the list above; contiguous (any
+ *           leading dims), 16-byte aligned;
+ *   scales  u8 [ceil(k / 128), rows, 4]: byte j of group g is the exponent s of
+ *           the row's block 4 g + j, which stands for 2^(s - 127), 255 for a
+ *           block of NaN; contiguous, 4-byte aligned. Bytes past the row's last
+ *           block are not read as scales (lux3d_mxfp4_quantize writes 0).
+ * This is the OCP microscaling format MXFP4 with its scales regrouped for the
+ * matrix instructions, which take a row's four blocks at a time. The reference
+ * quantizes to Q8_0 alone (weights/quantize.rs:319-338); these are the same
+ * steps at half the size.
+ *
+ * lux3d_mxfp4_quantize: x (f32, bf16 or f16 rows [..., k], 16-byte aligned) ->
+ * q, scales. s = max(floor(log2(max |x|)) - 2 + 127, 0) of the block, each value
+ * the nearest of the format's times 2^(s - 127), ties to the even code, at most
+ * 6; a block with an infinity or NaN gets s = 255, its codes mean nothing.
+ * lux3d_mxfp4_dequantize: the values, in y's type (f32, bf16 or f16 rows, 16-byte
+ * aligned): exact in f32 and bf16 (an overflow past f32 is infinite), rounded to
+ * f16. One kernel each; the counterpart of lux3d_dequant_q8_0.                */
+int lux3d_mxfp4_quantize(const lux3d_tensor_t *x, const lux3d_tensor_t *q,
+                         const lux3d_tensor_t *scales, lux3d_stream_t stream);
+int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales,
+                           const lux3d_tensor_t *y, lux3d_stream_t stream);
+
+/* lux3d_mxfp4_linear: y = x W^T (+ bias), Linear::forward (runtime/nn_blocks.rs:
+ * 83-93) on a packed weight, x as it is:
+ *   x: f32, bf16 or f16 rows [..., k], 16-byte aligned; w, w_scales: packed [n,
+ *      k]; bias: f32 [n] or NULL; y: [..., n] rows, f32 / bf16 / f16.
+ * Weights enter as x's type holds them (exact in bf16 and f32; f16: exact for
+ * block scales 2^-23 to 2^13, rounded beyond), products and sums are f32, f32 x
+ * in three exact bf16 terms; y is rounded once. One kernel.
+ *
+ * lux3d_mxfp4_linear_fp4: x is quantized as by lux3d_mxfp4_quantize first, and
+ * the products of 4-bit values run on the scaled matrix instructions, four times
+ * the bf16 rate (the counterpart of lux3d_q8_0_linear_int8): y = sum over blocks
+ * of 2^(sx + sw - 254) * sum of products of codes, in f32.
+ *   xq u8 [rows, k / 2], xs u8 [ceil(k / 128), rows, 4]: receive x's packed form.
+ *      With at most LUX3D_MXFP4_FEW_ROWS rows x is quantized as it is read, and
+ *      both may be NULL (given, they are left as they are). They hold nothing
+ *      between calls; no two calls that may overlap share them.
+ *   x NULL: xq and xs hold the packed x already (one quantization for several
+ *      projections); its bits are those that the quantization of x would give.
+ * One kernel for few rows or packed x, else two.
+ *
+ * lux3d_mxfp4_linear_gated: act(x Wg^T + bg) * (x Wu^T + bu), the first half of
+ * a gated feed-forward block, in one kernel: GeGlu::forward (runtime/nn_blocks.rs:
+ * 238-254: Linear, chunk, gelu_erf, product) and its kin. fp4 0: the arithmetic
+ * of lux3d_mxfp4_linear (xq, xs NULL); fp4 1: of lux3d_mxfp4_linear_fp4 (x, xq,
+ * xs as there). gate, up: packed [n, k] of one shape; biases f32 [n] or NULL.
+ * The activation is taken of the f32 sum (SiLU and tanh GELU to a few f32 ulp,
+ * erf GELU to 1.7e-7 absolute), the product rounded once.
+ *
+ * In all three the order of the f32 sums depends on the shape, the number of
+ * rows among it; the same shape gives the same bits. y must not overlap an
+ * input. An infinity or NaN in x reaches its own row of y alone.             */
+#define LUX3D_MXFP4_FEW_ROWS 16
+typedef enum { LUX3D_GELU_ERF = 0, LUX3D_GELU_TANH = 1, LUX3D_SILU = 2 } lux3d_act;
+int lux3d_mxfp4_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *w,
+                       const lux3d_tensor_t *w_scales, const lux3d_tensor_t *bias,
+                       const lux3d_tensor_t *y, lux3d_stream_t stream);
+int lux3d_mxfp4_linear_fp4(const lux3d_tensor_t *x, const lux3d_tensor_t *xq,
+                           const lux3d_tensor_t *xs, const lux3d_tensor_t *w,
+                           const lux3d_tensor_t *w_scales, const lux3d_tensor_t *bias,
+                           const lux3d_tensor_t *y, lux3d_stream_t stream);
+int lux3d_mxfp4_linear_gated(const lux3d_tensor_t *x, const lux3d_tensor_t *xq,
+                             const lux3d_tensor_t *xs, const lux3d_tensor_t *gate,
+                             const lux3d_tensor_t *gate_scales, const lux3d_tensor_t *gate_bias,
+                             const lux3d_tensor_t *up, const lux3d_tensor_t *up_scales,
+                             const lux3d_tensor_t *up_bias, int32_t act, int32_t fp4,
+                             const lux3d_tensor_t *y, lux3d_stream_t stream);
+
 /* ---- TRELLIS.2 sparse voxel ops (runtime/trellis2_sparse.rs) ----------------
  * lux3d_sparse_neighbors: CoordMap::new + the per-offset lookups of
  * SparseConv3d::forward (trellis2_sparse.rs:62-91, 205-222), on the device;
