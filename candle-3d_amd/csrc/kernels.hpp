@@ -215,6 +215,9 @@ struct MxLinearParams {
   int64_t M = 0, N = 0, K = 0;
 };
 hipError_t launch_mx_linear(const MxLinearParams &p, hipStream_t s);
+// Its kernel for many rows (mxfp4_gemm.hip): whether a call's sizes fit it; with packed x (p.x null) or plain, not fp4.
+bool mx_gemm_fits(const MxLinearParams &p);
+hipError_t launch_mx_gemm(const MxLinearParams &p, int tile, hipStream_t s);
 
 // Scaled dot-product attention over [B, H, L, D] views (element strides per
 // batch, head and token; unit inner stride). out = softmax(q k^T * scale) v.

@@ -299,6 +299,7 @@ hipError_t launch_mx_linear(const MxLinearParams &given, hipStream_t s) {
     if (hipError_t e = launch_mx_quantize(q, s)) return e;
     p.x = nullptr;
   }
+  if (p.M > 64 && mx_gemm_fits(p)) return launch_mx_gemm(p, p.K >= 4096 && p.M * p.N >= (int64_t)200 * 256 * 256 ? 256 : 128, s);
   if (!p.x) return launch_rows_kernel<void, true>(p, s);
   switch (p.x_dt) {
     case LUX3D_F32: return launch_rows_x<F32>(p, s);
