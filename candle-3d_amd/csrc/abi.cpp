@@ -1165,7 +1165,7 @@ int mx_linear(const char *fn, const lux3d_tensor_t *x, const lux3d_tensor_t *xq,
     if (x && (v.rows != xv.rows || v.k != xv.d))
       return fail(LUX3D_ERR_SHAPE, "%s: `xq` holds [%lld, %lld] values, x [%lld, %lld]", fn, (long long)v.rows, (long long)v.k,
                   (long long)xv.rows, (long long)xv.d);
-    p.xq = v.q; p.xs = v.s;
+    p.xq = v.q; p.xs = v.s; p.xs_rows = v.rows;
     xv.rows = v.rows; xv.d = v.k;
   }
   if (xv.d != k) return fail(LUX3D_ERR_SHAPE, "%s: x has %lld features, the weight %lld", fn, (long long)xv.d, (long long)k);

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
+#include "mxfp4_tiles.hpp"
 #include "prefix_plan.hpp"
 
 namespace lux3d {
@@ -208,6 +209,7 @@ struct MxLinearParams {
   const void *x = nullptr; int64_t ldx = 0; int x_dt = -1;  // [M, K] rows, 16-byte aligned; null: packed x given
   bool fp4 = false;                                         // x enters in 4 bits
   uint8_t *xq = nullptr, *xs = nullptr;                     // packed x: given, or written here (fp4, more than kMxFewRows rows)
+  int64_t xs_rows = 0;                                      // rows of xs
   const uint8_t *w[2] = {nullptr, nullptr}, *ws[2] = {nullptr, nullptr};  // packed [N, K]; 1: the gate
   const float *bias[2] = {nullptr, nullptr};                // [N] or null
   int act = -1;                                             // Act; -1: no gate
@@ -217,7 +219,7 @@ struct MxLinearParams {
 hipError_t launch_mx_linear(const MxLinearParams &p, hipStream_t s);
 // Its kernel for many rows (mxfp4_gemm.hip): whether a call's sizes fit it; with packed x (p.x null) or plain, not fp4.
 bool mx_gemm_fits(const MxLinearParams &p);
-hipError_t launch_mx_gemm(const MxLinearParams &p, int tile, hipStream_t s);
+hipError_t launch_mx_gemm(const MxLinearParams &p, const MxTileId &tile, hipStream_t s);
 
 // Scaled dot-product attention over [B, H, L, D] views (element strides per
 // batch, head and token; unit inner stride). out = softmax(q k^T * scale) v.

@@ -66,30 +66,42 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
 
 // ---- and back -------------------------------------------------------------------
 //
-// 16 values a lane (8 bytes of codes), so that a wavefront writes 2 KB (2-byte
-// types) of one row.
+// The same tiles of 32 rows x 512 values, 8 rows of a wavefront in flight. A
+// lane writes 16 bytes and the next lane the 16 behind them: 8 values of a
+// 2-byte type, 4 of f32, which takes the row's half in two steps (16 values a
+// lane and four stores 64 bytes apart instead: 8192 x 2048 f32 50 us).
 template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
-  const int64_t per = (p.K + 15) / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.M * per) return;
-  const int64_t r = i / per, k = (i - r * per) * 16;
-  const uint2 c = *reinterpret_cast<const uint2 *>(p.q + (r * p.K + k) / 2);
-  const uint32_t s = p.s[((k >> 7) * p.M + r) * 4 + ((k >> 5) & 3)];
-  char *dst = reinterpret_cast<char *>(p.y) + (r * p.ldy + k) * T::bytes;
-  if constexpr (T::code == LUX3D_F32) {
-    const float sc = __uint_as_float(s << 23);
-    const uint32_t w[2] = {c.x, c.y};
+  constexpr int V = 16 / T::bytes, STEPS = 8 / V, R = kQuantRows / 4;  // values a lane and step
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
+  const int64_t r0 = rt * kQuantRows + wave * R;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 1);
-      const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], sc, 3);
-      st16(dst + 32 * j, make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])));
-      st16(dst + 32 * j + 16, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(e[0]), __float_as_uint(e[1])));
+  for (int step = 0; step < STEPS; ++step) {
+    const int64_t k = kt * kQuantCols + step * (kQuantCols / STEPS) + lane * V;
+    if (k >= p.K) return;
+    uint32_t c[R], s[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = r0 + i < p.M ? r0 + i : p.M - 1;
+      const uint8_t *src = p.q + (r * p.K + k) / 2;
+      if constexpr (V == 8) c[i] = *reinterpret_cast<const uint32_t *>(src);
+      else c[i] = *reinterpret_cast<const uint16_t *>(src);
+      s[i] = p.s[((k >> 7) * p.M + r) * 4 + ((k >> 5) & 3)];
     }
-  } else {
-    const u32x4_t a = mx_values8<T>(c.x, s), b = mx_values8<T>(c.y, s);
-    st16(dst, make_uint4(a[0], a[1], a[2], a[3]));
-    st16(dst + 16, make_uint4(b[0], b[1], b[2], b[3]));
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= p.M) break;
+      void *dst = reinterpret_cast<char *>(p.y) + ((r0 + i) * p.ldy + k) * T::bytes;
+      if constexpr (V == 8) {
+        const u32x4_t v = mx_values8<T>(c[i], s[i]);
+        st16(dst, make_uint4(v[0], v[1], v[2], v[3]));
+      } else {
+        const float sc = __uint_as_float(s[i] << 23);
+        const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], sc, 1);
+        st16(dst, make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])));
+      }
+    }
   }
 }
 
@@ -118,73 +130,75 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
   for (int j = 0; j < NM; ++j)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
-  for (int64_t c = wave; c < groups; c += NW) {
+  // what a lane holds of a group: its block of each matrix and of each row tile
+  constexpr int XN = PACKED ? 1 : 2 * std::conditional_t<PACKED, F32, X>::bytes;  // 16-byte pieces of x's block
+  struct Group {
+    uint4 w[NM], x[MT][XN];
+    uint32_t sw[NM], sx[MT];
+  };
+  auto load = [&](Group &q, int64_t c) {
     const int64_t b = 4 * c + g;
     const bool live = b < nb;  // a last group may have fewer than four blocks: the others count as 0
-    uint4 w[NM];
-    uint32_t sw[NM];
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
-      w[j] = ld16<false>(p.w[j] + n * (p.K / 2) + (live ? b : nb - 1) * 16);
-      sw[j] = live ? p.ws[j][(c * p.N + n) * 4 + g] : 0;
+      q.w[j] = ld16<false>(p.w[j] + n * (p.K / 2) + (live ? b : nb - 1) * 16);
+      q.sw[j] = live ? p.ws[j][(c * p.N + n) * 4 + g] : 0;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int64_t m = m0 + 16 * i + l16;
-      const bool have = live && m < p.M;
-      if constexpr (FP4) {
-        u32x4_t xc = u32x4_t{};
-        uint32_t sx = 0;
+#pragma unroll
+      for (int e = 0; e < XN; ++e) q.x[i][e] = make_uint4(0, 0, 0, 0);
+      q.sx[i] = 0;
+      if (live && m < p.M) {
         if constexpr (PACKED) {
-          if (have) {
-            const uint4 u = ld16<false>(p.xq + m * (p.K / 2) + b * 16);
-            xc = u32x4_t{u.x, u.y, u.z, u.w};
-            sx = p.xs[(c * p.M + m) * 4 + g];
-          }
+          q.x[i][0] = ld16<false>(p.xq + m * (p.K / 2) + b * 16);
+          q.sx[i] = p.xs[(c * p.xs_rows + m) * 4 + g];
         } else {
-          constexpr int NV = X::bytes * 2;  // 16-byte loads of a block
-          uint32_t v[4 * NV];
+          const char *src = reinterpret_cast<const char *>(p.x) + (m * p.ldx + b * 32) * X::bytes;
 #pragma unroll
-          for (int e = 0; e < 4 * NV; ++e) v[e] = 0;
-          if (have) {
-            const char *src = reinterpret_cast<const char *>(p.x) + (m * p.ldx + b * 32) * X::bytes;
+          for (int e = 0; e < XN; ++e) q.x[i][e] = ld16<false>(src + 16 * e);
+        }
+      }
+    }
+  };
+  auto products = [&](Group &q) {
 #pragma unroll
-            for (int e = 0; e < NV; ++e) {
-              const uint4 u = ld16<false>(src + 16 * e);
-              v[4 * e] = u.x;
-              v[4 * e + 1] = u.y;
-              v[4 * e + 2] = u.z;
-              v[4 * e + 3] = u.w;
-            }
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (FP4) {
+        u32x4_t xc;
+        uint32_t sx = q.sx[i];
+        if constexpr (PACKED) {
+          xc = u32x4_t{q.x[i][0].x, q.x[i][0].y, q.x[i][0].z, q.x[i][0].w};
+        } else {
+          uint32_t v[4 * XN];
+#pragma unroll
+          for (int e = 0; e < XN; ++e) {
+            v[4 * e] = q.x[i][e].x;
+            v[4 * e + 1] = q.x[i][e].y;
+            v[4 * e + 2] = q.x[i][e].z;
+            v[4 * e + 3] = q.x[i][e].w;
           }
           uint32_t top = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, mx_top<X>(v + e * NV));
+          for (int e = 0; e < 4; ++e) top = max(top, mx_top<X>(v + e * XN));
           sx = mx_scale(top);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) xc[e] = mx_codes<X>(v + e * NV, sx);
+          for (int e = 0; e < 4; ++e) xc[e] = mx_codes<X>(v + e * XN, sx);
         }
         const i32x8_t xb = {(int)xc[0], (int)xc[1], (int)xc[2], (int)xc[3], 0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < NM; ++j) {
-          const i32x8_t wa = {(int)w[j].x, (int)w[j].y, (int)w[j].z, (int)w[j].w, 0, 0, 0, 0};
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[j][i], 4, 4, 0, (int)sw[j], 0, (int)sx);
+          const i32x8_t wa = {(int)q.w[j].x, (int)q.w[j].y, (int)q.w[j].z, (int)q.w[j].w, 0, 0, 0, 0};
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[j][i], 4, 4, 0, (int)q.sw[j], 0, (int)sx);
         }
       } else {
-        constexpr int NV = X::bytes * 2;
-        uint4 v[NV];
-#pragma unroll
-        for (int e = 0; e < NV; ++e) v[e] = make_uint4(0, 0, 0, 0);
-        if (have) {
-          const char *src = reinterpret_cast<const char *>(p.x) + (m * p.ldx + b * 32) * X::bytes;
-#pragma unroll
-          for (int e = 0; e < NV; ++e) v[e] = ld16<false>(src + 16 * e);
-        }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           u32x4_t x1, x2, x3;
           if constexpr (X::code == LUX3D_F32) {
-            const uint32_t f[8] = {v[2 * s].x, v[2 * s].y, v[2 * s].z, v[2 * s].w, v[2 * s + 1].x, v[2 * s + 1].y, v[2 * s + 1].z, v[2 * s + 1].w};
+            const uint4 a = q.x[i][2 * s], c = q.x[i][2 * s + 1];
+            const uint32_t f[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const Split3 r = split3_bf16(__uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1]));
@@ -193,16 +207,16 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
               x3[e] = r.t3;
             }
           } else {
-            x1 = u32x4_t{v[s].x, v[s].y, v[s].z, v[s].w};
+            x1 = u32x4_t{q.x[i][s].x, q.x[i][s].y, q.x[i][s].z, q.x[i][s].w};
           }
 #pragma unroll
           for (int j = 0; j < NM; ++j) {
-            const uint32_t ws = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w;
+            const uint32_t ws = s == 0 ? q.w[j].x : s == 1 ? q.w[j].y : s == 2 ? q.w[j].z : q.w[j].w;
             if constexpr (X::code == LUX3D_F16) {
-              acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, mx_values8<F16>(ws, sw[j])),
+              acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, mx_values8<F16>(ws, q.sw[j])),
                                                                  __builtin_bit_cast(f16x8_t, x1), acc[j][i], 0, 0, 0);
             } else {
-              const bf16x8_t wv = __builtin_bit_cast(bf16x8_t, mx_values8<BF16>(ws, sw[j]));
+              const bf16x8_t wv = __builtin_bit_cast(bf16x8_t, mx_values8<BF16>(ws, q.sw[j]));
               if constexpr (X::code == LUX3D_F32) {
                 acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x3), acc[j][i], 0, 0, 0);
                 acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x2), acc[j][i], 0, 0, 0);
@@ -213,6 +227,11 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
         }
       }
     }
+  };
+  for (int64_t c = wave; c < groups; c += NW) {
+    Group q;
+    load(q, c);
+    products(q);
   }
   // lane holds weight rows 4 g + e, x row l16 of each tile
 #pragma unroll
@@ -240,16 +259,24 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
   }
 }
 
-template <typename X, bool FP4, bool GATED>
+template <typename X, bool FP4, bool GATED, int MT, int NW>
 hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
-  const int mt = p.M <= 16 ? 1 : 2;
-  const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * mt - 1) / (16 * mt), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
+  const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * MT - 1) / (16 * MT), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
   if (tn > INT32_MAX || z > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tn, (unsigned)((tm + z - 1) / z), (unsigned)z);
-  const MxAct act = mx_act(p.act);
-  if (mt == 1) hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, 1, 8>), grid, dim3(512), 0, s, p, act);
-  else hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, 2, 8>), grid, dim3(512), 0, s, p, act);
+  hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, MT, NW>), grid, dim3(64 * NW), 0, s, p, mx_act(p.act));
   return hipGetLastError();
+}
+
+// us with 4 / 8 / 16 wavefronts: 1 row, 8192 -> 2048 bf16 12.9 / 8.9 / 7.4, f32
+// 19.3 / 13.8 / 11.0; 2048 -> 8192 4.5 / 4.5 / 4.5, f32 6.8 / 6.4 / 6.9; 1536 ->
+// 9216 5.1 / 4.8 / 5.3; 33 rows, 8192 -> 2048 23.6 / 20.4 / 20.2, 1536 -> 9216
+// 13.6 / 13.0 / 14.1. Four row tiles instead of two: 64 rows, 8192 -> 2048 20.7 ->
+// 35.6, 2048 -> 8192 19.9 -> 19.6. Two groups in flight a wavefront: within 8%.
+template <typename X, bool FP4, bool GATED>
+hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
+  if (p.M > 16) return launch_rows_kernel<X, FP4, GATED, 2, 8>(p, s);
+  return p.K >= 6144 ? launch_rows_kernel<X, FP4, GATED, 1, 16>(p, s) : launch_rows_kernel<X, FP4, GATED, 1, 8>(p, s);
 }
 
 template <typename X, bool FP4>
@@ -278,10 +305,10 @@ hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s) {
 }
 
 hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s) {
-  const int64_t blocks = (p.M * ((p.K + 15) / 16) + 255) / 256;
-  if (blocks <= 0) return hipSuccess;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks);
+  if (p.M <= 0) return hipSuccess;
+  const int64_t tiles = (p.K + kQuantCols - 1) / kQuantCols * ((p.M + kQuantRows - 1) / kQuantRows);
+  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)tiles);
   switch (p.y_dt) {
     case LUX3D_F32: hipLaunchKernelGGL(mx_dequantize_kernel<F32>, grid, dim3(256), 0, s, p); break;
     case LUX3D_BF16: hipLaunchKernelGGL(mx_dequantize_kernel<BF16>, grid, dim3(256), 0, s, p); break;
@@ -291,6 +318,18 @@ hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s) {
   return hipGetLastError();
 }
 
+namespace {
+hipError_t launch_rows(const MxLinearParams &p, hipStream_t s) {
+  if (!p.x) return launch_rows_kernel<void, true>(p, s);
+  switch (p.x_dt) {
+    case LUX3D_F32: return launch_rows_x<F32>(p, s);
+    case LUX3D_BF16: return launch_rows_x<BF16>(p, s);
+    case LUX3D_F16: return launch_rows_x<F16>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+}  // namespace
+
 hipError_t launch_mx_linear(const MxLinearParams &given, hipStream_t s) {
   MxLinearParams p = given;
   if (p.M <= 0 || p.N <= 0) return hipSuccess;
@@ -299,14 +338,17 @@ hipError_t launch_mx_linear(const MxLinearParams &given, hipStream_t s) {
     if (hipError_t e = launch_mx_quantize(q, s)) return e;
     p.x = nullptr;
   }
-  if (p.M > 64 && mx_gemm_fits(p)) return launch_mx_gemm(p, p.K >= 4096 && p.M * p.N >= (int64_t)200 * 256 * 256 ? 256 : 128, s);
-  if (!p.x) return launch_rows_kernel<void, true>(p, s);
-  switch (p.x_dt) {
-    case LUX3D_F32: return launch_rows_x<F32>(p, s);
-    case LUX3D_BF16: return launch_rows_x<BF16>(p, s);
-    case LUX3D_F16: return launch_rows_x<F16>(p, s);
-  }
-  return hipErrorInvalidValue;
+  const MxKind kind = !p.x ? MX_PACKED : p.x_dt == LUX3D_F32 ? MX_F32 : MX_2BYTE;
+  const MxChoice c = mx_choose(kind, p.M, p.N, p.K, p.act >= 0);
+  if (c.rows == 0 || !mx_gemm_fits(p)) return launch_rows(p, s);
+  MxLinearParams rest = p;
+  p.M = c.rows;
+  if (hipError_t e = launch_mx_gemm(p, c.tile, s)) return e;
+  if ((rest.M -= c.rows) == 0) return hipSuccess;
+  if (rest.x) rest.x = reinterpret_cast<const char *>(p.x) + c.rows * p.ldx * (p.x_dt == LUX3D_F32 ? 4 : 2);
+  else rest.xq += c.rows * (p.K / 2), rest.xs += c.rows * 4;
+  rest.y = reinterpret_cast<char *>(p.y) + c.rows * p.ldy * (p.y_dt == LUX3D_F32 ? 4 : 2);
+  return launch_rows(rest, s);
 }
 
 }  // namespace lux3d

@@ -16,14 +16,24 @@
 // k order inside a stage: lane half h = lane / 32 holds, packed, block 2 h + s of
 // the stage's four in sub-step s, so that its two scale bytes are adjacent; 2
 // bytes, values 8 s .. + 7 of block h; f32, values 16 h + 8 s .. + 7 of the one
-// block. Stages arrive by direct loads (buffer_load ... lds) NS - 1 ahead, with
-// the 16-byte pieces of a row swizzled so that the reads below, 16 rows at a
-// time, meet every bank once. One barrier a stage, before the last sub-step's
-// products, as in the Q8_0 ring kernel.
+// block. Stages arrive by direct loads (buffer_load ... lds) ahead of their use,
+// with the 16-byte pieces of a row swizzled so that the reads below, 16 rows at a
+// time, meet every bank once. One barrier a stage.
+//
+// A sub-step's fragments are read during the products of the one before.
+//
+// KG: where tiles are few, KG groups of a workgroup's wavefronts take every KG th
+// stage through rings of their own and add their sums in group order at the end:
+// a lone tile's time is its chain of stages, not its bytes or products.
+//
+// PERSIST: as many workgroups as CUs, each with the next of its tiles. The first
+// stages of the next tile are loaded during the last products of this one, and
+// its stores drain during the next tile's products.
 //
 // The weights are the matrix instruction's first operand: a lane then holds four
 // consecutive outputs of one row of y, and the epilogue packs whole words.
 #include <type_traits>
+#include <utility>
 
 #include "mxfp4.hpp"
 
@@ -36,74 +46,94 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
+template <typename F, int... I>
+__device__ __forceinline__ void for_each_slot(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 // X: void (packed x), BF16, F16 or F32.
-template <typename X, int WM_, int WN_, int TM_, int TN_, int NS_, bool GATED_>
+template <typename X, int WM_, int WN_, int TM_, int TN_, int NS_, int KG_, bool PERSIST_, bool GATED_>
 struct MxTile {
-  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
-  static constexpr bool GATED = GATED_, PACKED = std::is_void_v<X>;
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_, KG = KG_;
+  static constexpr bool PERSIST = PERSIST_, GATED = GATED_, PACKED = std::is_void_v<X>;
   static constexpr bool XF32 = std::is_same_v<X, F32>;
   static constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN;
-  static constexpr int BNO = GATED ? BN / 2 : BN;          // outputs of the tile's rows
-  static constexpr int WC = GATED ? TN * 16 : TN * 32;     // a wavefront's
+  static constexpr int NG = GATED ? 2 : 1, BNO = BN / NG;        // matrices; outputs of the tile's rows
+  static constexpr int TO = TN / NG, WC = 32 * TO;               // output tiles and outputs of a wavefront
   static constexpr int BK = PACKED ? 128 : XF32 ? 32 : 64, SUB = PACKED || XF32 ? 2 : 4;
   static constexpr int XROW = PACKED ? 64 : 128, WROW = BK / 2;  // bytes of a row's stage
   static constexpr int XL = BM * XROW, WL = BN * WROW, XS = PACKED ? BM * 4 : 0, WS = BN * 4;
   static constexpr int STAGE = XL + WL + XS + WS;
-  static constexpr int XSEG = XL / 1024, WSEG = WL / 1024, SSEG = (XS + WS) / 256;  // direct loads of a stage
+  static constexpr int XSEG = XL / 1024, WSEG = WL / 1024, SSEG = (XS + WS) / 256, BSEG = BN / 64;  // direct loads
   static constexpr int SX = XSEG > NW ? XSEG / NW : 1, SW = WSEG > NW ? WSEG / NW : 1, SS = (SSEG + NW - 1) / NW;
-  static constexpr int OPS = SX + SW + SS;                 // of each wavefront
-  static constexpr int LDS = NS * STAGE;
+  static constexpr int SB = (BSEG + NW - 1) / NW;
+  static constexpr int OPS = SX + SW + SS;                       // of each wavefront and stage
+  static constexpr int OROW = 128 + 16, OUT = NW * 32 * OROW;    // the epilogue's rows: 128 bytes of 32 rows a wavefront
+  static constexpr int BIAS = NS * STAGE, OUT_AT = PERSIST ? BIAS + 2 * BN * 4 : 0;
+  static constexpr int RING = PERSIST ? OUT_AT + OUT : BIAS + BN * 4;  // of a group of wavefronts
+  static constexpr int PART = TM * TN * 16 * 64 * 4;             // a wavefront's sums
+  static constexpr int LDS = KG * RING;
   static_assert(XL % 1024 == 0 && WL % 1024 == 0 && BM % 64 == 0 && BNO % 64 == 0, "whole segments");
   static_assert((XSEG % NW == 0 || NW % XSEG == 0) && (WSEG % NW == 0 || NW % WSEG == 0), "even shares");
   static_assert(!GATED || TN % 2 == 0, "a gate tile beside every up tile");
-  static_assert(NW * 32 * (WC * 4 + 16) + BN * 4 <= LDS, "the epilogue's rows fit");
-  static_assert((NS - 2) * OPS < 64, "vmcnt");
+  static_assert(OUT_AT + OUT <= (PERSIST ? RING : BIAS) && LDS <= 160 * 1024, "the epilogue's rows fit");
+  static_assert(KG == 1 || (!PERSIST && NW * PART <= RING), "a group's sums fit its ring");
+  static_assert(NS >= 3 && (NS - 2) * OPS < 63, "stages");
 };
 
-template <typename X, int WM, int WN, int TM, int TN, int NS, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN, 1) void mx_gemm_kernel(MxLinearParams p, MxAct act, int tiles_m, int tiles_n) {
-  using T = MxTile<X, WM, WN, TM, TN, NS, GATED>;
+template <typename X, int WM, int WN, int TM, int TN, int NS, int KG, bool PERSIST, bool GATED>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearParams p, MxAct act, int tiles_m, int tiles_n) {
+  using T = MxTile<X, WM, WN, TM, TN, NS, KG, PERSIST, GATED>;
   constexpr int GM = 8;  // row tiles of a group
-  __shared__ __align__(16) char ring[T::LDS];
+  __shared__ __align__(16) char lds[T::LDS];
 
-  // XCD-contiguous ranges of tiles, groups of GM row tiles, as in q8_0_gemm_ring_kernel
-  const int G = tiles_m * tiles_n, bid = (int)blockIdx.x;
-  const int per = G / 8, rem = G % 8, xcd = bid % 8, pos = bid / 8;
-  const int lid = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + pos;
-  const int group = lid / (GM * tiles_n), first_m = group * GM;
-  const int gsize = tiles_m - first_m < GM ? tiles_m - first_m : GM;
-  const int in_group = lid - group * GM * tiles_n;
-  const int tm = first_m + in_group % gsize, tn = in_group / gsize;
-
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, l32 = lane & 31;
+  // group kg of the wavefronts takes every KG th stage through a ring of its own
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * T::NW)) : 0;
+  const int t = KG > 1 ? threadIdx.x - kg * 64 * T::NW : threadIdx.x;
+  const int lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, l32 = lane & 31;
+  char *const ring = lds + kg * T::RING;
   const int wm = wave / WN, wn = wave % WN;
-  const int64_t m0 = (int64_t)tm * T::BM, c0 = (int64_t)tn * T::BNO;
-  const int nblk = (int)(p.K / 32), nk = (int)((p.K + T::BK - 1) / T::BK);
-  const int rest = nblk % (T::BK / 32);  // blocks of a last stage that is not whole
+  const int nblk = (int)(p.K / 32), all = (int)((p.K + T::BK - 1) / T::BK), nk = (all + KG - 1) / KG;  // a group's stages
+  const int rest = nblk % (T::BK / 32);           // blocks of a last stage that is not whole
+  const bool tail = rest != 0 || all % KG != 0;   // the groups' last stages need zeros
 
-  // Direct loads. Rows past the matrix are clamped to its last: loaded, computed, never stored. A last stage that is not
-  // whole reads on into the next row, or past the descriptor's end (nothing): zero_tail clears x and the scales there, and
-  // any four bits are a finite weight. Descriptors span the tile's rows (of the scales, every group).
+  // Tiles: each XCD (workgroup id % 8) takes a contiguous range, in groups of GM row tiles, as in q8_0_gemm_ring_kernel; its
+  // workgroups take the range's tiles in turn.
+  const int G = tiles_m * tiles_n, xcd = (int)blockIdx.x % 8, per = G / 8, rem = G % 8;
+  const int first = xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per, end = first + per + (xcd < rem ? 1 : 0);
+  const int step = ((int)gridDim.x - xcd + 7) / 8;
+  int lid = first + (int)blockIdx.x / 8;
+  if (lid >= end) return;
+  int64_t m0 = 0, c0 = 0;  // of the tile that is computed
+  auto place = [&](int id, int64_t &m, int64_t &c) {
+    const int group = id / (GM * tiles_n), first_m = group * GM;
+    const int gsize = tiles_m - first_m < GM ? tiles_m - first_m : GM;
+    const int in_group = id - group * GM * tiles_n;
+    m = (int64_t)(first_m + in_group % gsize) * T::BM;
+    c = (int64_t)(in_group / gsize) * T::BNO;
+  };
+
+  // Direct loads. A lane's offsets are the same for every tile; the descriptors span the tile's rows (of the scales, every
+  // group). Rows past the matrix lie past the descriptor: they are not read, and what the LDS holds there reaches only
+  // outputs that are not stored. A last stage that is not whole reads on into the next row: zero_tail clears x and the
+  // scales there, and any four bits are a finite weight.
   constexpr int EB = T::PACKED ? 1 : T::XF32 ? 4 : 2;
   const int64_t xrow = T::PACKED ? p.K / 2 : p.ldx * EB, xk = T::PACKED ? p.K / 2 : p.K * EB, groups = (nblk + 3) / 4;
-  const int64_t last_m = p.M - 1 - m0 < T::BM - 1 ? p.M - 1 - m0 : T::BM - 1;
-  const int64_t ncols = p.N - c0 < T::BNO ? p.N - c0 : T::BNO;
-  const char *xbase = reinterpret_cast<const char *>(T::PACKED ? (const void *)p.xq : p.x) + m0 * xrow;
-  const i32x4_t xr = buffer_rsrc(xbase, last_m * xrow + xk);
-  uint32_t xoff[T::SX], xto[T::SX], woff[T::SW], wto[T::SW];
-  i32x4_t wsrc[T::SW];
+  const char *const xbase = reinterpret_cast<const char *>(T::PACKED ? (const void *)p.xq : p.x);
+  uint32_t xoff[T::SX], xto[T::SX], woff[T::SW], wto[T::SW], soff[T::SS], sto[T::SS];
+  bool wgate[T::SW], sgate[T::SS], sx[T::SS];  // uniform: the gate's weights, the gate's scales, x's scales
 #pragma unroll
   for (int i = 0; i < T::SX; ++i) {
     const int seg = (wave * T::SX + i) % T::XSEG;
     const int r = T::PACKED ? seg * 16 + (lane >> 2) : seg * 8 + (lane >> 3);
     const int c = T::PACKED ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ ((r >> 1) & 7);
-    xoff[i] = (uint32_t)((r <= last_m ? r : last_m) * xrow + 16 * c);
+    xoff[i] = (uint32_t)(r * xrow + 16 * c);
     xto[i] = seg * 1024;
   }
 #pragma unroll
   for (int i = 0; i < T::SW; ++i) {
-    const int seg = (wave * T::SW + i) % T::WSEG;
-    int r, c;  // row of the tile, 16-byte piece
+    const int seg = (wave * T::SW + i) % T::WSEG;  // lies in one matrix
+    int r, c;                                      // row of the tile, 16-byte piece
     if constexpr (T::PACKED) {
       r = seg * 16 + (lane >> 2);
       c = (lane & 3) ^ ((r >> 2) & 3);
@@ -114,284 +144,436 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_gemm_kernel(MxLinearParams
       r = seg * 32 + (lane >> 1);
       c = (lane & 1) ^ ((r >> 3) & 1);
     }
-    const bool second = GATED && __builtin_amdgcn_readfirstlane(r) >= T::BNO;  // a segment lies in one matrix
-    wsrc[i] = buffer_rsrc((second ? p.w[1] : p.w[0]) + c0 * (p.K / 2), ncols * (p.K / 2));
-    const int64_t col = second ? r - T::BNO : r;
-    woff[i] = (uint32_t)((col < ncols ? col : ncols - 1) * (p.K / 2) + 16 * c);
+    wgate[i] = GATED && seg >= T::WSEG / 2;
+    woff[i] = (uint32_t)((r - (wgate[i] ? T::BNO : 0)) * (p.K / 2) + 16 * c);
     wto[i] = T::XL + seg * 1024;
   }
-  // the scales: 64 rows' words a load
-  i32x4_t ssrc[T::SS];
-  uint32_t soff[T::SS], sto[T::SS], sstep[T::SS];
 #pragma unroll
-  for (int i = 0; i < T::SS; ++i) {
-    const int seg = (wave * T::SS + i) % T::SSEG, r = seg * 64 + lane;
+  for (int i = 0; i < T::SS; ++i) {  // 64 rows' words a load
+    const int seg = (wave * T::SS + i) % T::SSEG, r = seg * 64 - T::XS / 4;
+    sx[i] = r < 0;
+    sgate[i] = GATED && r >= T::BNO;
+    soff[i] = (uint32_t)((sx[i] ? seg * 64 : sgate[i] ? r - T::BNO : r) + lane) * 4;
     sto[i] = T::XL + T::WL + seg * 256;
-    const bool of_x = seg * 256 < T::XS;
-    const int rw = of_x ? r : r - T::XS / 4;
-    const bool second = GATED && !of_x && seg * 64 - T::XS / 4 >= T::BNO;
-    const int64_t line = second ? rw - T::BNO : rw, rows = of_x ? p.M : p.N, have = of_x ? last_m + 1 : ncols;
-    ssrc[i] = buffer_rsrc((of_x ? p.xs + m0 * 4 : (second ? p.ws[1] : p.ws[0]) + c0 * 4), ((groups - 1) * rows + have) * 4);
-    soff[i] = (uint32_t)((line < have ? line : have - 1) * 4);
-    sstep[i] = (uint32_t)(rows * 4);
   }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)ring;
-  auto issue = [&](int kt, int slot) {
-    const uint32_t st = lds0 + slot * T::STAGE;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + kg * T::RING;
+  // the tile that is loaded: its descriptors, and the stage that comes next
+  i32x4_t xr, wr[T::SW], sr[T::SS];  // one of each load, where it may be of either matrix
+  int load_lid = lid, load_kt = kg, bias_buf = 0;
 #pragma unroll
-    for (int i = 0; i < T::SX; ++i) lds_load16(xr, xoff[i], (uint32_t)kt * T::XROW, __builtin_amdgcn_readfirstlane(st + xto[i]));
+  for (int i = 0; i < T::SX; ++i) xto[i] = __builtin_amdgcn_readfirstlane(lds0 + xto[i]);
 #pragma unroll
-    for (int i = 0; i < T::SW; ++i) lds_load16(wsrc[i], woff[i], (uint32_t)kt * T::WROW, __builtin_amdgcn_readfirstlane(st + wto[i]));
+  for (int i = 0; i < T::SW; ++i) wto[i] = __builtin_amdgcn_readfirstlane(lds0 + wto[i]);
+#pragma unroll
+  for (int i = 0; i < T::SS; ++i) sto[i] = __builtin_amdgcn_readfirstlane(lds0 + sto[i]);
+  auto load_tile = [&]() {
+    int64_t m, c;
+    place(load_lid, m, c);
+    const int64_t rows = p.M - m < T::BM ? p.M - m : T::BM, cols = p.N - c < T::BNO ? p.N - c : T::BNO;
+    xr = buffer_rsrc(xbase + m * xrow, (rows - 1) * xrow + xk);
+#pragma unroll
+    for (int i = 0; i < T::SW; ++i) wr[i] = buffer_rsrc((wgate[i] ? p.w[1] : p.w[0]) + c * (p.K / 2), cols * (p.K / 2));
 #pragma unroll
     for (int i = 0; i < T::SS; ++i)
-      lds_load4(ssrc[i], soff[i], __builtin_amdgcn_readfirstlane((uint32_t)(kt / (128 / T::BK)) * sstep[i]),
-                __builtin_amdgcn_readfirstlane(st + sto[i]));
+      sr[i] = buffer_rsrc(sx[i] ? p.xs + m * 4 : (sgate[i] ? p.ws[1] : p.ws[0]) + c * 4,
+                          ((groups - 1) * (sx[i] ? p.xs_rows : p.N) + (sx[i] ? rows : cols)) * 4);
+    // biases, beside the tile's first stage (no bias, columns past the matrix: not read, not used)
+#pragma unroll
+    for (int i = 0; i < T::SB; ++i) {
+      const int seg = (wave * T::SB + i) % T::BSEG;
+      const bool gate = GATED && seg >= T::BSEG / 2;
+      const float *b = gate ? p.bias[1] : p.bias[0];
+      const i32x4_t br = buffer_rsrc(b ? b + c : b, b ? cols * 4 : 0);
+      lds_load4(br, (uint32_t)((seg - (gate ? T::BSEG / 2 : 0)) * 64 + lane) * 4, 0,
+                __builtin_amdgcn_readfirstlane(lds0 + T::BIAS + bias_buf * T::BN * 4 + seg * 256));
+    }
+    if constexpr (PERSIST) bias_buf ^= 1;
   };
-  // A last stage that is not whole: zeros for x past its end, and for the scales of the blocks that are not there.
+  auto issue = [&](int n, int to) {  // the n-th of OPS loads of the next stage, into slot `to`
+    if (n < T::SX) {
+      lds_load16(xr, xoff[n], (uint32_t)load_kt * T::XROW, __builtin_amdgcn_readfirstlane(xto[n] + to * T::STAGE));
+    } else if (n < T::SX + T::SW) {
+      const int i = n - T::SX;
+      lds_load16(wr[i], woff[i], (uint32_t)load_kt * T::WROW, __builtin_amdgcn_readfirstlane(wto[i] + to * T::STAGE));
+    } else {
+      const int i = n - T::SX - T::SW;
+      const uint32_t rows4 = (uint32_t)((sx[i] ? p.xs_rows : p.N) * 4);
+      lds_load4(sr[i], soff[i], __builtin_amdgcn_readfirstlane((uint32_t)(load_kt / (128 / T::BK)) * rows4),
+                __builtin_amdgcn_readfirstlane(sto[i] + to * T::STAGE));
+    }
+  };
+  // Behind the last load of a stage. Past the last stage of the last tile that stage is loaded again, into slots that are
+  // not read for data any more, so that the wait counts stay.
+  auto advance = [&]() {
+    if (load_kt + KG < all) {
+      load_kt += KG;
+    } else if (PERSIST && load_lid + step < end) {
+      load_lid += step;
+      load_kt = 0;
+      load_tile();
+    }
+  };
+  // A group's last stage where it is not whole, or not there (the stage before was loaded again): zeros for x past its end,
+  // and for the scales of the blocks that are not there.
   auto zero_tail = [&](int slot) {
     char *st = ring + slot * T::STAGE;
-    constexpr int CPR = T::XROW / 16, CPB = T::PACKED ? 1 : 4;  // pieces of a row, of a block
+    constexpr int CPR = T::XROW / 16, CPB = T::PACKED ? 1 : T::XF32 ? 8 : 4;  // pieces of a row, of a block
+    const int last = (nk - 1) * KG + kg, have = last >= all ? 0 : last + 1 == all && rest ? rest : T::BK / 32;
     for (int i = t; i < T::BM * CPR; i += 64 * T::NW) {
       const int r = i / CPR, c = i % CPR;
-      if (c < rest * CPB) continue;
+      if (c < have * CPB) continue;
       const int at = T::PACKED ? c ^ ((r >> 2) & 3) : c ^ ((r >> 1) & 7);
       *reinterpret_cast<uint4 *>(st + r * T::XROW + at * 16) = make_uint4(0, 0, 0, 0);
     }
-    const int keep = (nblk - 1) % 4 + 1;  // scale bytes of the last group
-    if (keep < 4)
+    const int keep = last >= all ? 0 : (nblk - 1) % 4 + 1;  // scale bytes of the last group of blocks
+    if (last + 1 >= all && keep < 4)
       for (int i = t; i < (T::XS + T::WS) / 4; i += 64 * T::NW)
         reinterpret_cast<uint32_t *>(st + T::XL + T::WL)[i] &= (1u << (8 * keep)) - 1;
     lds_barrier();
   };
 
-  // Fragments of a sub-step. Weight tile j lies in rows wrow(j) of the stage, x tile i in (wm TM + i) * 32.
-  auto wrow = [&](int j) {
-    if constexpr (GATED) return (j / (TN / 2)) * T::BNO + (wn * (TN / 2) + j % (TN / 2)) * 32;
-    else return (wn * TN + j) * 32;
-  };
-  constexpr int XT = T::XF32 ? 3 : 1;  // terms of x
-  struct XFrag { u32x4_t v[XT]; };
-  XFrag xf[2][TM];
-  u32x4_t wf[2][TN];
-  u32x4_t wraw[TN];                 // plain: the stage's codes of a lane (f32: half of it used)
-  uint32_t wsc[TN], xsc[TM];        // scales of the stage in use: packed two bytes, else one
-  uint32_t wsn[TN], xsn[TM];        // and of the next
-  auto read_stage = [&](int kt) {
-    const char *st = ring + (kt % NS) * T::STAGE;
-    const char *ws = st + T::XL + T::WL + T::XS;
+  // Fragments. Weight tile j lies in rows wrow(j) of the stage, x tile i in (wm TM + i) * 32.
+  auto wrow = [&](int j) { return (j / T::TO) * T::BNO + (wn * T::TO + j % T::TO) * 32; };
+  // a lane's place in a stage: of x for each 16-byte piece that it reads, of the weights, of the scales
+  constexpr int XPC = T::PACKED ? 2 : 4;             // pieces of a lane
+  int xat[XPC], wat[2], wsat, xsat = 0;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int r = wrow(j) + l32;
+  for (int c = 0; c < XPC; ++c)
+    xat[c] = (wm * TM * 32 + l32) * T::XROW + (T::PACKED ? ((2 * h + c) ^ ((l32 >> 2) & 3)) << 4 : ((4 * h + c) ^ ((l32 >> 1) & 7)) << 4);
+  const int w0 = wn * T::TO * 32 + l32;              // row of the first weight tile; tile j: wtile(j) further
+  auto wtile = [](int j) { return (j / T::TO) * T::BNO + j % T::TO * 32; };
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    wat[c] = T::XL + w0 * T::WROW + (T::PACKED ? ((2 * h + c) ^ ((l32 >> 2) & 3)) << 4 : T::XF32 ? h * 8 : (h ^ ((l32 >> 3) & 1)) << 4);
+  wsat = T::XL + T::WL + T::XS + w0 * 4 + (T::XF32 ? 0 : 2 * h);
+  if constexpr (T::PACKED) xsat = T::XL + T::WL + (wm * TM * 32 + l32) * 4 + 2 * h;
+  else if constexpr (!T::XF32) wsat -= h;            // one byte: h, and 2 more in every second stage
+  constexpr int XP = T::XF32 ? 2 : 1;                // 16-byte pieces of x's fragment
+  struct Frag { u32x4_t v[XP]; };
+  Frag xf[2][TM];
+  u32x4_t wf[2][TN];                                 // plain: converted
+  u32x4_t wraw[TN];                                  // plain: the stage's codes of a lane (f32: half of it used)
+  uint32_t wsc[2][TN], xsc[2][TM];                   // scales: packed two bytes, else one
+  // the n-th of NRS reads of a stage's scales, plain with its weights, into buffer b
+  constexpr int NRS = T::PACKED ? TN + TM : TN;
+  auto read_stage = [&](int slot, int kt, int n, int b) {
+    const char *st = ring + slot * T::STAGE;
+    if (n < TN) {
       if constexpr (T::PACKED) {
-        wsn[j] = *reinterpret_cast<const uint16_t *>(ws + r * 4 + 2 * h);
+        wsc[b][n] = *reinterpret_cast<const uint16_t *>(st + wsat + wtile(n) * 4);
       } else if constexpr (T::XF32) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(st + T::XL + r * 16 + h * 8);
-        wraw[j] = u32x4_t{u.x, u.y, 0, 0};
-        wsn[j] = *reinterpret_cast<const uint8_t *>(ws + r * 4 + (kt & 3));
+        const uint2 u = *reinterpret_cast<const uint2 *>(st + wat[0] + wtile(n) * T::WROW);
+        wraw[n] = u32x4_t{u.x, u.y, 0, 0};
+        wsc[b][n] = *reinterpret_cast<const uint8_t *>(st + wsat + wtile(n) * 4 + (kt & 3));
       } else {
-        wraw[j] = *reinterpret_cast<const u32x4_t *>(st + T::XL + r * 32 + ((h ^ ((l32 >> 3) & 1)) << 4));
-        wsn[j] = *reinterpret_cast<const uint8_t *>(ws + r * 4 + 2 * (kt & 1) + h);
+        wraw[n] = *reinterpret_cast<const u32x4_t *>(st + wat[0] + wtile(n) * T::WROW);
+        wsc[b][n] = *reinterpret_cast<const uint8_t *>(st + wsat + wtile(n) * 4 + 2 * (kt & 1));
       }
-    }
-    if constexpr (T::PACKED) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        xsn[i] = *reinterpret_cast<const uint16_t *>(st + T::XL + T::WL + ((wm * TM + i) * 32 + l32) * 4 + 2 * h);
+    } else if constexpr (T::PACKED) {
+      xsc[b][n - TN] = *reinterpret_cast<const uint16_t *>(st + xsat + (n - TN) * 128);
     }
   };
-  auto read_frags = [&](int kt, int s, int buf) {
-    const char *st = ring + (kt % NS) * T::STAGE;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      if constexpr (T::PACKED) {
-        const int r = wrow(j) + l32;
-        wf[buf][j] = *reinterpret_cast<const u32x4_t *>(st + T::XL + r * 64 + (((2 * h + s) ^ ((l32 >> 2) & 3)) << 4));
-      } else {
-        wf[buf][j] = mx_values8<std::conditional_t<std::is_same_v<X, F16>, F16, BF16>>(wraw[j][s], wsn[j]);
-      }
+  typedef std::conditional_t<std::is_same_v<X, F16>, F16, BF16> WT;  // the weights' type in the products
+  // the n-th of NRF fragments of sub-step s into buffer b: x's, then the weights'
+  constexpr int NRF = TM + TN;
+  auto read_frag = [&](int slot, int s, int b, int n) {
+    const char *st = ring + slot * T::STAGE;
+    if (n >= TM) {
+      const int j = n - TM;
+      if constexpr (T::PACKED) wf[b][j] = *reinterpret_cast<const u32x4_t *>(st + wat[s & 1] + wtile(j) * 64);
+      else wf[b][j] = mx_values8<WT>(wraw[j][s], wsc[0][j]);
+      return;
     }
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int r = (wm * TM + i) * 32 + l32;
-      const char *row = st + r * T::XROW;
-      if constexpr (T::PACKED) {
-        xf[buf][i].v[0] = *reinterpret_cast<const u32x4_t *>(row + (((2 * h + s) ^ ((l32 >> 2) & 3)) << 4));
-      } else if constexpr (T::XF32) {
-        const int sw = (l32 >> 1) & 7;
-        const float4 a = *reinterpret_cast<const float4 *>(row + (((4 * h + 2 * s) ^ sw) << 4));
-        const float4 b = *reinterpret_cast<const float4 *>(row + (((4 * h + 2 * s + 1) ^ sw) << 4));
-        const Split3 q[4] = {split3_bf16(a.x, a.y), split3_bf16(a.z, a.w), split3_bf16(b.x, b.y), split3_bf16(b.z, b.w)};
-        xf[buf][i].v[0] = u32x4_t{q[0].t1, q[1].t1, q[2].t1, q[3].t1};
-        xf[buf][i].v[XT / 2] = u32x4_t{q[0].t2, q[1].t2, q[2].t2, q[3].t2};
-        xf[buf][i].v[XT - 1] = u32x4_t{q[0].t3, q[1].t3, q[2].t3, q[3].t3};
-      } else {
-        xf[buf][i].v[0] = *reinterpret_cast<const u32x4_t *>(row + (((4 * h + s) ^ ((l32 >> 1) & 7)) << 4));
-      }
-    }
+    for (int e = 0; e < XP; ++e)
+      xf[b][n].v[e] = *reinterpret_cast<const u32x4_t *>(st + xat[(XP * s + e) % XPC] + n * 32 * T::XROW);
   };
   f32x16_t acc[TN][TM];
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int i = 0; i < TM; ++i) acc[j][i] = f32x16_t{};
-  auto products = [&](auto sub, int buf) {
+  // The products of sub-step s, from buffer b, in a fixed order, other(n) behind the n-th: LDS reads and direct loads go
+  // between them, so that neither the LDS nor the matrix core waits for a burst of the other. Each accumulator passes an
+  // empty statement that the compiler may not move: it would else sink a sub-step's products below the barrier, past the
+  // reads.
+  constexpr int NP = TM * TN;
+  auto products = [&](auto sub, int b, auto other) {
     constexpr int S = decltype(sub)::value;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      u32x4_t x[3];
+      if constexpr (T::XF32) {
+        const u32x4_t a = xf[b][i].v[0], c = xf[b][i].v[XP - 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Split3 q = e < 2 ? split3_bf16(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]))
+                                 : split3_bf16(__uint_as_float(c[2 * e - 4]), __uint_as_float(c[2 * e - 3]));
+          x[0][e] = q.t1;
+          x[1][e] = q.t2;
+          x[2][e] = q.t3;
+        }
+      } else {
+        x[0] = xf[b][i].v[0];
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const u32x4_t w = wf[b][j];
+        if constexpr (T::PACKED) {
+          const i32x8_t av = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+          const i32x8_t bv = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], 0, 0, 0, 0};
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[j][i], 4, 4, S, (int)wsc[0][j], S, (int)xsc[0][i]);
+        } else if constexpr (std::is_same_v<X, F16>) {
+          acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, x[0]),
+                                                             acc[j][i], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = T::XF32 ? 2 : 0; e >= 0; --e)  // smallest terms first
+            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x[e]),
+                                                                acc[j][i], 0, 0, 0);
+        }
+        asm volatile("" : "+v"(acc[j][i]));
+        other(i * TN + j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // the share of `count` operations that goes behind the n-th of `products`, two at a time at least
+  auto share = [&](int n, int products, int count, auto &&op) {
+    const int each = (count + products - 1) / products > 2 ? (count + products - 1) / products : 2;
+#pragma unroll
+    for (int o = 0; o < each; ++o)
+      if (n * each + o < count) op(n * each + o);
+  };
+  constexpr auto c_0 = std::integral_constant<int, 0>{};
+  constexpr auto c_1 = std::integral_constant<int, 1>{};
+  constexpr auto c_2 = std::integral_constant<int, 2>{};
+
+  int slot = 0, tile = 0;  // slot of the stage in use; tiles done
+  load_tile();
+#pragma unroll
+  for (int st = 0; st < NS - 1; ++st) {
+#pragma unroll
+    for (int n = 0; n < T::OPS; ++n) issue(n, st);
+    advance();
+  }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(PERSIST ? 0 : (NS - 2) * T::OPS));  // stage 0 landed (PERSIST: all)
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  if (tail && nk == 1) zero_tail(0);
+#pragma unroll
+  for (int n = 0; n < NRS; ++n) read_stage(0, kg, n, 0);
+#pragma unroll
+  for (int n = 0; n < NRF; ++n) read_frag(0, 0, 0, n);
+
+  // Stage kt of the tile, in slot SL: a constant, so that LDS addresses are a lane's base and an immediate. (With the slot
+  // in a register a stage took 60 instructions more, which bound the small tiles.)
+  auto stage = [&](int kt, auto sl) {
+    constexpr int SL = decltype(sl)::value, NX = (SL + 1) % NS, TO_SLOT = (SL + NS - 1) % NS;
+    const int next = kt + 1 < nk ? kt + 1 : 0;  // PERSIST: the next tile's first
+    // the slot refilled here was last read a stage ago, before that stage's barrier
+    products(c_0, 0, [&](int n) {
+      share(n, NP, NRF + T::OPS, [&](int o) {
+        if (o < NRF) read_frag(SL, 1, 1, o);
+        else issue(o - NRF, TO_SLOT);
+      });
+    });
+    advance();
+    if constexpr (T::SUB == 4) {
+      products(c_1, 1, [&](int n) { share(n, NP, NRF, [&](int o) { read_frag(SL, 2, 0, o); }); });
+      products(c_2, 0, [&](int n) { share(n, NP, NRF, [&](int o) { read_frag(SL, 3, 1, o); }); });
+    }
+    // The next stage landed (only those issued after it may be in flight), this wavefront's reads of this one are done;
+    // then every one's. PERSIST, first stage of a tile: what is older than its stores was waited for before them.
+    if (PERSIST && kt == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(63));
+    else __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((NS - 2) * T::OPS));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (tail && next + 1 == nk) zero_tail(NX);
+    // the scales of the stage in use stay until its last products
+    products(std::integral_constant<int, T::SUB - 1>{}, 1, [&](int n) {
+      share(n, NP, NRS + NRF, [&](int o) {
+        if (o < NRS) read_stage(NX, next * KG + kg, o, T::PACKED ? 1 : 0);
+        else read_frag(NX, 0, 0, o - NRS);
+      });
+    });
+    if constexpr (T::PACKED) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) wsc[0][j] = wsc[1][j];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) xsc[0][i] = xsc[1][i];
+    }
+  };
+
+  do {
+    place(lid, m0, c0);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        if constexpr (T::PACKED) {
-          const u32x4_t a = wf[buf][j], b = xf[buf][i].v[0];
-          const i32x8_t av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-          const i32x8_t bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[j][i], 4, 4, S, (int)wsc[j], S, (int)xsc[i]);
-        } else if constexpr (std::is_same_v<X, F16>) {
-          acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, wf[buf][j]),
-                                                             __builtin_bit_cast(f16x8_t, xf[buf][i].v[0]), acc[j][i], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int e = XT - 1; e >= 0; --e)  // smallest terms first
-            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, wf[buf][j]),
-                                                                __builtin_bit_cast(bf16x8_t, xf[buf][i].v[e]), acc[j][i], 0, 0, 0);
-        }
+      for (int i = 0; i < TM; ++i) acc[j][i] = f32x16_t{};
+
+    // the stages in turn; a tile may end, and the next begin, at any slot
+    int kt = 0;
+    auto turn = [&](auto sl) {
+      constexpr int SL = decltype(sl)::value;
+      if (kt < nk && slot == SL) {
+        stage(kt, sl);
+        ++kt;
+        slot = (SL + 1) % NS;
       }
-  };
-  auto next_scales = [&]() {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) wsc[j] = wsn[j];
-    if constexpr (T::PACKED) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) xsc[i] = xsn[i];
-    }
-  };
+    };
+    while (kt < nk) for_each_slot(turn, std::make_integer_sequence<int, NS>{});
 
-  // Past the last stage the loop reloads it into slots that are not read for data again, so that the wait counts stay.
-#pragma unroll
-  for (int st = 0; st < NS - 1; ++st) issue(st < nk ? st : nk - 1, st);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm((NS - 2) * T::OPS));  // stage 0 landed
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  if (rest && nk == 1) zero_tail(0);
-  read_stage(0);
-  read_frags(0, 0, 0);
-  for (int kt = 0; kt < nk; ++kt) {
-    next_scales();
-    // the slot refilled here was last read in step kt - 1, before its barrier
-    issue(kt + NS - 1 < nk ? kt + NS - 1 : nk - 1, (kt + NS - 1) % NS);
-    __builtin_amdgcn_sched_barrier(0);
-    read_frags(kt, 1, 1);
-    products(std::integral_constant<int, 0>{}, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (T::SUB == 4) {
-      read_frags(kt, 2, 0);
-      products(std::integral_constant<int, 1>{}, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      read_frags(kt, 3, 1);
-      products(std::integral_constant<int, 2>{}, 0);
-      __builtin_amdgcn_sched_barrier(0);
+    // Epilogue. Lane holds outputs 8 q + 4 h .. + 3 of weight tile j for row l32 of x tile i: bias, activation and product in
+    // f32, one rounding, 32 rows x 128 bytes of the wavefront's outputs at a time through LDS (rows padded by 16 bytes),
+    // 16-byte pieces out, 8 lanes a row's line. y is written once: not kept in the caches (16392 x 2048 -> 8192: 220 -> 197 us).
+    if constexpr (!PERSIST) {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads and reads
+      __builtin_amdgcn_s_barrier();                     // every wavefront is done with the ring
     }
-    // stage kt + 1 landed (only those issued after it may be in flight), this wavefront's reads of stage kt are done; then
-    // every one's
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((NS - 2) * T::OPS));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (rest && kt + 2 == nk) zero_tail((kt + 1) % NS);
-    read_stage(kt + 1);
-    read_frags(kt + 1, 0, 0);
-    products(std::integral_constant<int, T::SUB - 1>{}, 1);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads and reads
-  __builtin_amdgcn_s_barrier();                     // every wavefront is done with the ring
-
-  // Epilogue. Lane holds outputs 8 q + 4 h .. + 3 of weight tile j for row l32 of x tile i: bias, activation and product in
-  // f32, one rounding, 32 rows of the wavefront's outputs at a time through LDS (rows padded by 16 bytes), whole 16-byte
-  // pieces of y's rows out.
-  float *const bias = reinterpret_cast<float *>(ring + T::LDS - T::BN * 4);
-  for (int i = t; i < T::BN; i += 64 * T::NW) {
-    const bool second = GATED && i >= T::BNO;
-    const float *b = second ? p.bias[1] : p.bias[0];
-    const int64_t col = c0 + (second ? i - T::BNO : i);
-    bias[i] = b && col < p.N ? b[col] : 0.f;
-  }
-  lds_barrier();
-  constexpr int TO = GATED ? TN / 2 : TN;  // output tiles of a wavefront
-  auto write = [&](auto bytes) {
-    constexpr int B = decltype(bytes)::value, ROW = T::WC * B + 16, CPR = T::WC * B / 16, EPC = 16 / B;
-    char *const reg = ring + wave * 32 * ROW;
-    const int64_t cw = c0 + wn * T::WC;
-    const bool whole = (uintptr_t)p.y % 16 == 0 && p.ldy * B % 16 == 0;
+    if constexpr (KG > 1) {
+      // the groups' sums in group order, through their rings
+      float *const part = reinterpret_cast<float *>(ring) + wave * (T::PART / 4);
+      if (kg > 0) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int j = 0; j < TO; ++j)
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 b0 = *reinterpret_cast<const float4 *>(bias + wrow(j) + 8 * q + 4 * h);
-          float v[4] = {acc[j][i][4 * q] + b0.x, acc[j][i][4 * q + 1] + b0.y, acc[j][i][4 * q + 2] + b0.z, acc[j][i][4 * q + 3] + b0.w};
-          if constexpr (GATED) {
-            const float4 b1 = *reinterpret_cast<const float4 *>(bias + wrow(j + TO) + 8 * q + 4 * h);
-            const float g[4] = {b1.x, b1.y, b1.z, b1.w};
+            for (int e = 0; e < 16; ++e) part[((j * TM + i) * 16 + e) * 64 + lane] = acc[j][i][e];
+      }
+      lds_barrier();
+      if (kg > 0) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= mx_activate(act, acc[j + TO][i][4 * q + e] + g[e]);
-          }
-          char *to = reg + l32 * ROW + (j * 32 + 8 * q + 4 * h) * B;
-          if constexpr (B == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-          else if (p.y_dt == LUX3D_BF16) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-          else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
-        }
-      // the wavefront's own memory: its LDS operations keep their order, only the compiler has to know
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      for (int it = 0; it < 32 * CPR / 64; ++it) {
-        const int n = it * 64 + lane, r = n / CPR, part = n % CPR;
-        const int64_t row = m0 + (wm * TM + i) * 32 + r, col = cw + part * EPC;
-        if (row >= p.M || col >= p.N) continue;
-        const uint4 v = *reinterpret_cast<const uint4 *>(reg + r * ROW + part * 16);
-        char *dst = reinterpret_cast<char *>(p.y) + (row * p.ldy + col) * B;
-        if (whole && col + EPC <= p.N) {
-          *reinterpret_cast<uint4 *>(dst) = v;
-        } else {
-          const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+      for (int g = 1; g < KG; ++g)
 #pragma unroll
-          for (int e = 0; e < EPC; ++e)
-            if (col + e < p.N) {
-              if constexpr (B == 4) reinterpret_cast<uint32_t *>(dst)[e] = w4[e];
-              else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w4[e >> 1] >> (16 * (e & 1)));
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][i][e] += part[g * (T::RING / 4) + ((j * TM + i) * 16 + e) * 64 + lane];
+    }
+    const float *const bias = reinterpret_cast<const float *>(ring + T::BIAS + (PERSIST ? (tile & 1) * T::BN * 4 : 0));
+    char *const reg = ring + T::OUT_AT + wave * 32 * T::OROW;
+    auto write = [&](auto bytes) {
+      constexpr int B = decltype(bytes)::value, JP = 4 / B, EPC = 16 / B;  // output tiles a pass; values of a piece
+      const bool whole = (uintptr_t)p.y % 16 == 0 && p.ldy * B % 16 == 0;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j0 = 0; j0 < T::TO; j0 += JP) {
+#pragma unroll
+          for (int jj = 0; jj < JP; ++jj) {
+            const int j = j0 + jj;
+            if (j >= T::TO) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e];
+              if (p.bias[0]) {
+                const float4 b = *reinterpret_cast<const float4 *>(bias + wrow(j) + 8 * q + 4 * h);
+                v[0] += b.x;
+                v[1] += b.y;
+                v[2] += b.z;
+                v[3] += b.w;
+              }
+              if constexpr (GATED) {
+                float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.bias[1]) b = *reinterpret_cast<const float4 *>(bias + wrow(j + T::TO) + 8 * q + 4 * h);
+                const float g[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= mx_activate(act, acc[j + T::TO][i][4 * q + e] + g[e]);
+              }
+              char *to = reg + l32 * T::OROW + (jj * 32 + 8 * q + 4 * h) * B;
+              if constexpr (B == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+              else if (p.y_dt == LUX3D_BF16) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+              else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
             }
+          }
+          // the wavefront's own memory: its LDS operations keep their order, only the compiler has to know
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          // the next tile's stages on their way, before the first store
+          if (PERSIST && i == 0 && j0 == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+          const int64_t cw = c0 + wn * T::WC + j0 * 32;
+          constexpr int WIDTH = T::TO * 32 < JP * 32 ? T::TO * 32 : JP * 32;  // of a pass
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const int r = it * 8 + (lane >> 3), part = lane & 7;
+            const int64_t row = m0 + (wm * TM + i) * 32 + r, col = cw + part * EPC;
+            if (row >= p.M || col >= p.N || part * EPC >= WIDTH) continue;
+            const uint4 v = *reinterpret_cast<const uint4 *>(reg + r * T::OROW + part * 16);
+            char *dst = reinterpret_cast<char *>(p.y) + (row * p.ldy + col) * B;
+            if (whole && col + EPC <= p.N) {
+              st16(dst, v);
+            } else {
+              const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < EPC; ++e)
+                if (col + e < p.N) {
+                  if constexpr (B == 4) reinterpret_cast<uint32_t *>(dst)[e] = w4[e];
+                  else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w4[e >> 1] >> (16 * (e & 1)));
+                }
+            }
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
         }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  };
-  if (p.y_dt == LUX3D_F32) write(std::integral_constant<int, 4>{});
-  else write(std::integral_constant<int, 2>{});
+    };
+    if (p.y_dt == LUX3D_F32) write(std::integral_constant<int, 4>{});
+    else write(std::integral_constant<int, 2>{});
+    ++tile;
+    lid += step;
+  } while (PERSIST && lid < end);
+  if constexpr (PERSIST) __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads
 }
 
-template <typename X, int WM, int WN, int TM, int TN, int NS, bool GATED>
+template <typename X, int WM, int WN, int TM, int TN, int NS, int KG, bool PERSIST, bool GATED>
 hipError_t launch_tile(const MxLinearParams &p, hipStream_t s) {
-  using T = MxTile<X, WM, WN, TM, TN, NS, GATED>;
+  using T = MxTile<X, WM, WN, TM, TN, NS, KG, PERSIST, GATED>;
   const int64_t tiles_m = (p.M + T::BM - 1) / T::BM, tiles_n = (p.N + T::BNO - 1) / T::BNO;
   if (tiles_m * tiles_n > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((mx_gemm_kernel<X, WM, WN, TM, TN, NS, GATED>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * T::NW), 0, s, p,
+  const int64_t tiles = tiles_m * tiles_n, cus = PERSIST ? cu_count(s) : tiles;
+  hipLaunchKernelGGL((mx_gemm_kernel<X, WM, WN, TM, TN, NS, KG, PERSIST, GATED>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(64 * T::NW * KG), 0, s, p,
                      mx_act(p.act), (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
 template <typename X, bool GATED>
-hipError_t launch_gemm(const MxLinearParams &p, int tile, hipStream_t s) {
+hipError_t launch_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s) {
+  const auto is = [&](int rows, int cols, int groups) { return t.rows == rows && t.cols == cols && t.groups == groups; };
   if constexpr (std::is_void_v<X>) {
-    if (tile == 256) return launch_tile<X, 2, 2, 4, 4, 4, GATED>(p, s);
+    if constexpr (!GATED) {
+      if (is(64, 64, 1)) return launch_tile<X, 2, 2, 1, 1, 4, 1, false, GATED>(p, s);
+      if (is(64, 64, 2)) return launch_tile<X, 2, 2, 1, 1, 4, 2, false, GATED>(p, s);
+    }
+    if (is(64, 128, 1)) return launch_tile<X, 2, 2, 1, 2, 4, 1, false, GATED>(p, s);
+    if (is(128, 128, 1)) return launch_tile<X, 2, 2, 2, 2, 4, 1, false, GATED>(p, s);
+    // its bias buffers and waits need four stages a tile
+    if (is(256, 256, 1) && p.K > 384) return launch_tile<X, 4, 2, 2, 4, 3, 1, true, GATED>(p, s);
   } else if constexpr (!std::is_same_v<X, F32>) {
-    if (tile == 256) return launch_tile<X, 2, 4, 4, 2, 3, GATED>(p, s);
+    if constexpr (!GATED) {
+      if (is(64, 64, 1)) return launch_tile<X, 2, 2, 1, 1, 4, 1, false, GATED>(p, s);
+      if (is(64, 64, 2)) return launch_tile<X, 2, 2, 1, 1, 4, 2, false, GATED>(p, s);
+      if (is(64, 64, 4)) return launch_tile<X, 2, 2, 1, 1, 3, 4, false, GATED>(p, s);
+    }
+    if (is(64, 128, 1)) return launch_tile<X, 2, 2, 1, 2, 4, 1, false, GATED>(p, s);
+    if (is(64, 128, 2)) return launch_tile<X, 2, 2, 1, 2, 4, 2, false, GATED>(p, s);
+    if (is(64, 128, 4)) return launch_tile<X, 2, 2, 1, 2, 3, 4, false, GATED>(p, s);
+    if (is(128, 128, 1)) return launch_tile<X, 2, 2, 2, 2, 3, 1, false, GATED>(p, s);
+    if (is(128, 256, 1)) return launch_tile<X, 2, 2, 2, 4, 3, 1, false, GATED>(p, s);
+    if (is(256, 256, 1)) return launch_tile<X, 2, 4, 4, 2, 3, 1, false, GATED>(p, s);
+  } else {
+    // a wavefront's 32 rows of x meet 128 weight rows, so that each value is split into its three terms once a workgroup
+    // (64 x 64 a wavefront, 4100 rows of 8192 -> 2048: 472 us against 397)
+    if constexpr (!GATED)
+      if (is(64, 64, 4)) return launch_tile<X, 2, 2, 1, 1, 4, 4, false, GATED>(p, s);
+    if (is(64, 128, 2)) return launch_tile<X, 2, 1, 1, 4, 3, 2, false, GATED>(p, s);
+    if (is(64, 128, 4)) return launch_tile<X, 2, 1, 1, 4, 3, 4, false, GATED>(p, s);
   }
-  return launch_tile<X, 2, 2, 2, 2, std::is_void_v<X> ? 4 : 3, GATED>(p, s);
+  return hipErrorInvalidValue;
 }
 
 template <typename X>
-hipError_t launch_gemm(const MxLinearParams &p, int tile, hipStream_t s) {
-  return p.act >= 0 ? launch_gemm<X, true>(p, tile, s) : launch_gemm<X, false>(p, tile, s);
+hipError_t launch_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s) {
+  return p.act >= 0 ? launch_gemm<X, true>(p, t, s) : launch_gemm<X, false>(p, t, s);
 }
 
 }  // namespace
@@ -401,15 +583,15 @@ hipError_t launch_gemm(const MxLinearParams &p, int tile, hipStream_t s) {
 bool mx_gemm_fits(const MxLinearParams &p) {
   const int64_t lim = 0x7FFFFFFF, eb = p.x_dt == LUX3D_F32 ? 4 : 2;
   return 256 * (p.x ? p.ldx * eb + 64 : p.K / 2) <= lim && 256 * p.K <= lim && (p.K + 127) / 32 * p.N <= lim &&
-         (p.K + 127) / 32 * p.M <= lim;
+         (p.x || (p.K + 127) / 32 * p.xs_rows <= lim);
 }
 
-hipError_t launch_mx_gemm(const MxLinearParams &p, int tile, hipStream_t s) {
-  if (!p.x) return launch_gemm<void>(p, tile, s);
+hipError_t launch_mx_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s) {
+  if (!p.x) return launch_gemm<void>(p, t, s);
   switch (p.x_dt) {
-    case LUX3D_F32: return launch_gemm<F32>(p, tile, s);
-    case LUX3D_BF16: return launch_gemm<BF16>(p, tile, s);
-    case LUX3D_F16: return launch_gemm<F16>(p, tile, s);
+    case LUX3D_F32: return launch_gemm<F32>(p, t, s);
+    case LUX3D_BF16: return launch_gemm<BF16>(p, t, s);
+    case LUX3D_F16: return launch_gemm<F16>(p, t, s);
   }
   return hipErrorInvalidValue;
 }

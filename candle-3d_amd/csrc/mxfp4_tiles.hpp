@@ -1,0 +1,112 @@
+// mxfp4_tiles.hpp -- which kernel and tile a linear on microscaled 4-bit weights
+// takes: the measured costs and the choice among them, host code without HIP.
+#pragma once
+#include <cmath>
+#include <cstdint>
+
+namespace lux3d {
+
+// How x enters: packed (on the scaled matrix instructions), 2-byte values, f32.
+enum MxKind : int { MX_PACKED = 0, MX_2BYTE = 1, MX_F32 = 2 };
+
+// rows x cols of y and of the weights' rows (gated: half of cols outputs), the
+// stages of k shared by `groups` groups of wavefronts. 256 x 256 of packed x:
+// workgroups that stay for several tiles.
+struct MxTileId {
+  int rows, cols, groups;
+};
+
+// The rows below `rows` in tiles of `tile`, the rest (16 at most; all of them
+// where rows is 0) by the few-rows kernel.
+struct MxChoice {
+  MxTileId tile;
+  int64_t rows;
+};
+
+inline double mx_up(int64_t a, int64_t b) { return (double)((a + b - 1) / b); }
+
+// Us of the few-rows kernel: a launch, the chain of a wavefront's groups of 128
+// of k, and the workgroups' loads of weights and of x, by the rows of their tile.
+// Fitted to 48, 24 and 24 sizes of up to 16 rows and 150 to 168 of more, within
+// 8 to 16% (root mean square).
+inline double mx_few_cost(MxKind kind, int64_t m, int64_t n, int64_t k, bool gated) {
+  constexpr double f[3][2][5] = {
+      // launch, chain, weights, x's rows, workgroup: up to 16 rows; more
+      {{1.5, 1.12, 0.019, 0.0081, 0.0}, {2.0, 0.64, 0.048, 0.0003, 0.51}},
+      {{1.5, 1.12, 0.036, 0.0076, 0.0}, {1.7, 1.39, 0.043, 0.0038, 0.46}},
+      {{1.2, 1.99, 0.028, 0.0139, 0.0}, {1.2, 2.53, 0.0, 0.0111, 0.84}}};
+  const bool few = m <= 16;
+  const double *c = f[kind][few ? 0 : 1];
+  const int64_t t = few ? 16 : 32;
+  const double g = mx_up(k, 128), w = mx_up(n, 16) * mx_up(m, t) / 256, rows = (double)(m < t ? m : t);
+  return c[0] + c[1] * std::ceil(g / (few && k >= 6144 ? 16 : 8)) * (gated ? 1.41 : 1) + w * (g * (c[2] * (gated ? 2 : 1) + c[3] * rows) + c[4]);
+}
+
+// Us of the tiles: c + r (a stages + b). A workgroup alone on its CU takes a
+// stages + b; w tiles a CU take r = s (th ceil(w) + (1 - th) w) times that, 1 at
+// least: s below 1 where several share a CU, th what of a last round is idle.
+// Fitted to 70 to 320 sizes each (k 128 to 8192, 17 to 16392 rows), within 4 to
+// 16% where a tile is near the best (the 256 x 256 tile of packed x 22%). Of 1180
+// sizes timed with every tile, the tile so chosen takes 1.0% (packed), 1.6% (2
+// bytes) and 0.3% (f32) longer than the shortest on average; most of what is
+// left are 100 to 160 rows of long k (8192 -> 2048 of 100 rows 16.7 against 11.5
+// us, few rows against 64 x 64) and 128 x 256 tiles of short k (256 -> 5000 of
+// 4098 rows 35 against 27).
+struct MxCost {
+  MxTileId tile;
+  double c, a, b, s, th;
+};
+
+inline MxChoice mx_choose(MxKind kind, int64_t m, int64_t n, int64_t k, bool gated) {
+  constexpr MxCost packed[] = {{{64, 64, 1}, 2.76, 0.142, 0.92, 0.88, 0.72},
+                               {{64, 64, 2}, 1.99, 0.240, 2.16, 0.90, 1.00},
+                               {{64, 128, 1}, 3.10, 0.190, 1.17, 1.04, 0.69},
+                               {{128, 128, 1}, 2.97, 0.286, 2.82, 0.98, 0.80},
+                               {{256, 256, 1}, 6.78, 0.595, 4.75, 1.35, 0.69}};
+  constexpr MxCost two[] = {{{64, 64, 1}, 2.88, 0.257, 1.19, 0.68, 0.95},
+                            {{64, 64, 2}, 1.71, 0.333, 3.00, 1.09, 0.89},
+                            {{64, 64, 4}, 3.38, 0.576, 2.55, 1.24, 0.78},
+                            {{64, 128, 1}, 3.34, 0.297, 1.33, 0.87, 0.64},
+                            {{64, 128, 2}, 2.12, 0.453, 3.57, 1.07, 0.97},
+                            {{64, 128, 4}, 4.14, 0.764, 3.58, 1.27, 0.75},
+                            {{128, 128, 1}, 3.13, 0.419, 2.75, 0.98, 0.59},
+                            {{128, 256, 1}, 5.45, 0.705, 3.89, 1.03, 0.65},
+                            {{256, 256, 1}, 2.42, 1.070, 9.59, 1.21, 0.77}};
+  constexpr MxCost f32[] = {{{64, 64, 4}, 2.83, 1.011, 3.83, 1.08, 0.92},
+                            {{64, 128, 2}, 3.77, 0.666, 3.00, 0.91, 0.72},
+                            {{64, 128, 4}, 3.78, 1.083, 5.16, 1.17, 0.86}};
+  const MxCost *costs = kind == MX_PACKED ? packed : kind == MX_2BYTE ? two : f32;
+  const int count = kind == MX_PACKED ? 5 : kind == MX_2BYTE ? 9 : 3;
+  const int64_t depth = kind == MX_PACKED ? 128 : kind == MX_2BYTE ? 64 : 32;
+  MxChoice best = {{16, 16, 1}, 0};
+  if (m <= 16) return best;
+  double least = mx_few_cost(kind, m, n, k, gated);
+  for (int i = 0; i < count; ++i) {
+    const MxCost &t = costs[i];
+    if (gated && t.tile.cols == 64) continue;                                   // a gate's half of 32 columns
+    if (kind == MX_PACKED && t.tile.rows == 256 && k < 512) continue;           // four stages a tile at least
+    const double one = t.a * std::ceil(mx_up(k, depth) / t.tile.groups) + t.b;
+    const double cols = mx_up(n, gated ? t.tile.cols / 2 : t.tile.cols);
+    auto cost = [&](int64_t rows) {
+      const double w = mx_up(rows, t.tile.rows) * cols / 256;
+      return t.c + (w <= 1 ? 1 : std::fmax(1, t.s * (t.th * std::ceil(w) + (1 - t.th) * w))) * one;
+    };
+    const double whole = cost(m);
+    if (whole < least) {
+      least = whole;
+      best = {t.tile, m};
+    }
+    // few rows past the last whole tile: a launch of their own where that saves a row of tiles (2 x 2049 tokens)
+    const int64_t rest = m % t.tile.rows;
+    if (rest >= 1 && rest <= 16 && m > t.tile.rows) {
+      const double split = cost(m - rest) + mx_few_cost(kind, rest, n, k, gated);
+      if (split < least) {
+        least = split;
+        best = {t.tile, m - rest};
+      }
+    }
+  }
+  return best;
+}
+
+}  // namespace lux3d
