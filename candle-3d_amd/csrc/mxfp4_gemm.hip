@@ -177,13 +177,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
     for (int i = 0; i < T::SS; ++i)
       sr[i] = buffer_rsrc(sx[i] ? p.xs + m * 4 : (sgate[i] ? p.ws[1] : p.ws[0]) + c * 4,
                           ((groups - 1) * (sx[i] ? p.xs_rows : p.N) + (sx[i] ? rows : cols)) * 4);
-    // biases, beside the tile's first stage (no bias, columns past the matrix: not read, not used)
+    // biases, ahead of the tile's first stage (columns past the matrix: not read, not used; no bias: the zeros stay)
 #pragma unroll
     for (int i = 0; i < T::SB; ++i) {
       const int seg = (wave * T::SB + i) % T::BSEG;
       const bool gate = GATED && seg >= T::BSEG / 2;
       const float *b = gate ? p.bias[1] : p.bias[0];
-      const i32x4_t br = buffer_rsrc(b ? b + c : b, b ? cols * 4 : 0);
+      if (!b || kg > 0) continue;  // uniform
+      const i32x4_t br = buffer_rsrc(b + c, cols * 4);
       lds_load4(br, (uint32_t)((seg - (gate ? T::BSEG / 2 : 0)) * 64 + lane) * 4, 0,
                 __builtin_amdgcn_readfirstlane(lds0 + T::BIAS + bias_buf * T::BN * 4 + seg * 256));
     }
@@ -346,6 +347,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
   constexpr auto c_2 = std::integral_constant<int, 2>{};
 
   int slot = 0, tile = 0;  // slot of the stage in use; tiles done
+  for (int i = t; i < (PERSIST ? 2 : 1) * T::BN; i += 64 * T::NW) reinterpret_cast<float *>(ring + T::BIAS)[i] = 0.f;
+  lds_barrier();
   load_tile();
 #pragma unroll
   for (int st = 0; st < NS - 1; ++st) {
@@ -403,10 +406,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
 
   do {
     place(lid, m0, c0);
+    // the sums start as the biases (zeros where there are none, and in the groups of wavefronts that add theirs to group 0's)
+    const float *const bias = reinterpret_cast<const float *>(ring + T::BIAS + (PERSIST ? (tile & 1) * T::BN * 4 : 0)) + wn * T::TO * 32 + 4 * h;
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) acc[j][i] = f32x16_t{};
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 b = *reinterpret_cast<const float4 *>(bias + wtile(j) + 8 * q);
+          acc[j][i][4 * q] = b.x;
+          acc[j][i][4 * q + 1] = b.y;
+          acc[j][i][4 * q + 2] = b.z;
+          acc[j][i][4 * q + 3] = b.w;
+        }
 
     // the stages in turn; a tile may end, and the next begin, at any slot
     int kt = 0;
@@ -420,9 +433,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
     };
     while (kt < nk) for_each_slot(turn, std::make_integer_sequence<int, NS>{});
 
-    // Epilogue. Lane holds outputs 8 q + 4 h .. + 3 of weight tile j for row l32 of x tile i: bias, activation and product in
-    // f32, one rounding, 32 rows x 128 bytes of the wavefront's outputs at a time through LDS (rows padded by 16 bytes),
-    // 16-byte pieces out, 8 lanes a row's line. y is written once: not kept in the caches (16392 x 2048 -> 8192: 220 -> 197 us).
+    // Epilogue. Lane holds outputs 8 q + 4 h .. + 3 of weight tile j for row l32 of x tile i: activation and product in f32,
+    // one rounding, 32 rows x 128 bytes of the wavefront's outputs at a time through LDS (rows padded by 16 bytes), 16-byte
+    // pieces out, 8 lanes a row's line. y is written once: not kept in the caches (16392 x 2048 -> 8192: 220 -> 197 us).
     if constexpr (!PERSIST) {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));  // the trailing reloads and reads
       __builtin_amdgcn_s_barrier();                     // every wavefront is done with the ring
@@ -449,11 +462,15 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] += part[g * (T::RING / 4) + ((j * TM + i) * 16 + e) * 64 + lane];
     }
-    const float *const bias = reinterpret_cast<const float *>(ring + T::BIAS + (PERSIST ? (tile & 1) * T::BN * 4 : 0));
     char *const reg = ring + T::OUT_AT + wave * 32 * T::OROW;
     auto write = [&](auto bytes) {
       constexpr int B = decltype(bytes)::value, JP = 4 / B, EPC = 16 / B;  // output tiles a pass; values of a piece
+      constexpr int WIDTH = T::TO < JP ? T::TO * 32 : JP * 32;            // outputs of a pass
       const bool whole = (uintptr_t)p.y % 16 == 0 && p.ldy * B % 16 == 0;
+      const bool inside = whole && m0 + T::BM <= p.M && c0 + T::BNO <= p.N;  // uniform: every piece is stored
+      char *const ytile = reinterpret_cast<char *>(p.y) + (m0 * p.ldy + c0) * B;
+      const uint32_t row8 = (uint32_t)(8 * p.ldy * B);                    // 8 rows of y; a tile spans less than 2^31 bytes
+      const uint32_t yoff = (uint32_t)(((wm * TM * 32 + (lane >> 3)) * p.ldy + wn * T::WC + (lane & 7) * EPC) * B);
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -466,20 +483,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
             for (int q = 0; q < 4; ++q) {
               float v[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e];
-              if (p.bias[0]) {
-                const float4 b = *reinterpret_cast<const float4 *>(bias + wrow(j) + 8 * q + 4 * h);
-                v[0] += b.x;
-                v[1] += b.y;
-                v[2] += b.z;
-                v[3] += b.w;
-              }
-              if constexpr (GATED) {
-                float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (p.bias[1]) b = *reinterpret_cast<const float4 *>(bias + wrow(j + T::TO) + 8 * q + 4 * h);
-                const float g[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= mx_activate(act, acc[j + T::TO][i][4 * q + e] + g[e]);
+              for (int e = 0; e < 4; ++e) {
+                v[e] = acc[j][i][4 * q + e];
+                if constexpr (GATED) v[e] *= mx_activate(act, acc[j + T::TO][i][4 * q + e]);
               }
               char *to = reg + l32 * T::OROW + (jj * 32 + 8 * q + 4 * h) * B;
               if constexpr (B == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
@@ -492,25 +498,40 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
           __builtin_amdgcn_wave_barrier();
           // the next tile's stages on their way, before the first store
           if (PERSIST && i == 0 && j0 == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-          const int64_t cw = c0 + wn * T::WC + j0 * 32;
-          constexpr int WIDTH = T::TO * 32 < JP * 32 ? T::TO * 32 : JP * 32;  // of a pass
+          const bool mine = WIDTH * B == 128 || (lane & 7) * 16 < WIDTH * B;
+          if (inside) {
 #pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            const int r = it * 8 + (lane >> 3), part = lane & 7;
-            const int64_t row = m0 + (wm * TM + i) * 32 + r, col = cw + part * EPC;
-            if (row >= p.M || col >= p.N || part * EPC >= WIDTH) continue;
-            const uint4 v = *reinterpret_cast<const uint4 *>(reg + r * T::OROW + part * 16);
-            char *dst = reinterpret_cast<char *>(p.y) + (row * p.ldy + col) * B;
-            if (whole && col + EPC <= p.N) {
-              st16(dst, v);
-            } else {
-              const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+            for (int it = 0; it < 4; ++it)
+              if (mine) st16(ytile + (i * 4 + it) * (uint64_t)row8 + j0 * 32 * B + yoff,
+                             *reinterpret_cast<const uint4 *>(reg + (it * 8 + (lane >> 3)) * T::OROW + (lane & 7) * 16));
+          } else if (whole) {
 #pragma unroll
-              for (int e = 0; e < EPC; ++e)
-                if (col + e < p.N) {
-                  if constexpr (B == 4) reinterpret_cast<uint32_t *>(dst)[e] = w4[e];
-                  else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w4[e >> 1] >> (16 * (e & 1)));
-                }
+            for (int it = 0; it < 4; ++it) {
+              const int64_t row = m0 + (wm * TM + i) * 32 + it * 8 + (lane >> 3), col = c0 + wn * T::WC + j0 * 32 + (lane & 7) * EPC;
+              if (row >= p.M || col >= p.N || !mine) continue;
+              const uint4 v = *reinterpret_cast<const uint4 *>(reg + (it * 8 + (lane >> 3)) * T::OROW + (lane & 7) * 16);
+              char *dst = ytile + (i * 4 + it) * (uint64_t)row8 + j0 * 32 * B + yoff;
+              if (col + EPC <= p.N) {
+                st16(dst, v);
+              } else {
+                const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < EPC; ++e)
+                  if (col + e < p.N) {
+                    if constexpr (B == 4) reinterpret_cast<uint32_t *>(dst)[e] = w4[e];
+                    else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w4[e >> 1] >> (16 * (e & 1)));
+                  }
+              }
+            }
+          } else {
+            // rows of y that are not 16-byte aligned: an element a lane, neighbouring lanes in a row
+            constexpr int L = WIDTH < 64 ? WIDTH : 64;
+            for (int r = lane / L; r < 32; r += 64 / L) {
+              const int64_t row = m0 + (wm * TM + i) * 32 + r, col = c0 + wn * T::WC + j0 * 32 + lane % L;
+              if (row >= p.M || col >= p.N) continue;
+              const char *from = reg + r * T::OROW + (lane % L) * B;
+              if constexpr (B == 4) reinterpret_cast<uint32_t *>(p.y)[row * p.ldy + col] = *reinterpret_cast<const uint32_t *>(from);
+              else reinterpret_cast<uint16_t *>(p.y)[row * p.ldy + col] = *reinterpret_cast<const uint16_t *>(from);
             }
           }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -578,11 +599,11 @@ hipError_t launch_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s
 
 }  // namespace
 
-// The kernel's descriptors span 256 rows of x and of the weights, and the scales of the whole matrix; its offsets have 32
-// bits.
+// The kernel's descriptors span 256 rows of x and of the weights, and the scales of the whole matrix; its offsets, also into
+// a tile of y, have 32 bits.
 bool mx_gemm_fits(const MxLinearParams &p) {
   const int64_t lim = 0x7FFFFFFF, eb = p.x_dt == LUX3D_F32 ? 4 : 2;
-  return 256 * (p.x ? p.ldx * eb + 64 : p.K / 2) <= lim && 256 * p.K <= lim && (p.K + 127) / 32 * p.N <= lim &&
+  return 256 * (p.x ? p.ldx * eb + 64 : p.K / 2) <= lim && 256 * p.K <= lim && 256 * 4 * p.ldy <= lim && (p.K + 127) / 32 * p.N <= lim &&
          (p.x || (p.K + 127) / 32 * p.xs_rows <= lim);
 }
 

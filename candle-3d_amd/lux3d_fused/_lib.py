@@ -133,6 +133,16 @@ def _load() -> ctypes.CDLL:
 
 
 LIB = _load()
+
+
+def with_bytes(name: str):
+    """The entry as a function that takes each tensor's descriptor as packed bytes or None."""
+    fn = LIB[name]  # a function object of its own: LIB's keeps its argument types
+    fn.argtypes = [ctypes.c_void_p if t is TP else t for t in SIGNATURES[name]]
+    fn.restype = ctypes.c_int
+    return fn
+
+
 ABI_VERSION = LIB.lux3d_abi_version()
 
 

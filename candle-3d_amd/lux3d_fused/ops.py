@@ -530,10 +530,34 @@ _MX_FEW_ROWS = 16  # LUX3D_MXFP4_FEW_ROWS: up to here a linear quantizes x as it
 _ACTS = {"gelu_erf": 0, "gelu_tanh": 1, "silu": 2}
 
 
-def _mx_packed(rows: int, lead, k: int, device):
-    """Empty packed storage of [rows, k] values: codes u8 [*lead, k / 2], scales u8 [ceil(k / 128), rows, 4]."""
-    return (torch.empty((*lead, k // 2), dtype=torch.uint8, device=device),
-            torch.empty(((k + 127) // 128, rows, 4), dtype=torch.uint8, device=device))
+def _b(t: Optional[torch.Tensor]):
+    """A tensor's lux3d_tensor_t as bytes, for the functions of _MX (None -> NULL): 0.4 us against _d's 0.7. Calls of a few
+    rows are as long as their host time."""
+    if t is None:
+        return None
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    shape = t.shape
+    if not shape:
+        return _PACK[1](t.data_ptr(), code, 1, 1, 1)
+    return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape, *t.stride())
+
+
+_MX = {fn: _lib.with_bytes(fn) for fn in ("lux3d_mxfp4_quantize", "lux3d_mxfp4_dequantize", "lux3d_mxfp4_linear",
+                                          "lux3d_mxfp4_linear_fp4", "lux3d_mxfp4_linear_gated")}
+
+
+def _mx_call(fn: str, lead: torch.Tensor, *args):
+    """The entry with lead's current stream, on its GPU."""
+    dev = lead.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = _MX[fn](*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = _MX[fn](*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != _lib.OK:
+        raise _lib.Lux3dError(fn, rc, _lib.LIB.lux3d_last_error().decode())
 
 
 def mxfp4_quantize(x: torch.Tensor):
@@ -541,11 +565,13 @@ def mxfp4_quantize(x: torch.Tensor):
     one exponent byte per 32 values, by groups of four blocks, u8 [ceil(k / 128), rows, 4]."""
     fn = "lux3d_mxfp4_quantize"
     _one_device(fn, x)
-    if x.dim() < 2 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) < 2 or shape[-1] == 0:
         raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "x must be [..., k]")
-    with _device_of(x):
-        q, scales = _mx_packed(x.numel() // x.shape[-1], x.shape[:-1], x.shape[-1], x.device)
-        _lib.call(fn, _d(x), _d(q), _d(scales), _stream(x))
+    k = shape[-1]
+    q = x.new_empty((*shape[:-1], k // 2), dtype=torch.uint8)
+    scales = x.new_empty(((k + 127) // 128, x.numel() // k, 4), dtype=torch.uint8)
+    _mx_call(fn, x, _b(x), _b(q), _b(scales))
     return q, scales
 
 
@@ -555,9 +581,8 @@ def mxfp4_dequantize(q: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16
     _one_device(fn, q, scales)
     if q.dim() < 2:
         raise _lib.Lux3dError(fn, _lib.ERR_SHAPE, "q must be [..., k / 2]")
-    with _device_of(q):
-        y = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=dtype, device=q.device)
-        _lib.call(fn, _d(q), _d(scales), _d(y), _stream(q))
+    y = q.new_empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=dtype)
+    _mx_call(fn, q, _b(q), _b(scales), _b(y))
     return y
 
 
@@ -577,23 +602,25 @@ def mxfp4_linear(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, bias: O
     x @ W^T (+ bias) -> [..., n] in out_dtype (default: x's)."""
     fn = "lux3d_mxfp4_linear"
     _one_device(fn, x, q, scales, bias)
-    with _device_of(x):
-        y = x.new_empty((*x.shape[:-1], q.shape[0]), dtype=out_dtype or x.dtype)
-        _lib.call(fn, _d(x), _d(q), _d(scales), _d(bias), _d(y), _stream(x))
+    y = x.new_empty((*x.shape[:-1], q.shape[0]), dtype=out_dtype)
+    _mx_call(fn, x, _b(x), _b(q), _b(scales), _b(bias), _b(y))
     return y
 
 
-def _mx_x(fn: str, x):
+def _mx_x(x):
     """(plain x or None, xq, xs, the tensor that leads) of an x that enters in 4 bits: a tensor, or the pair that
     mxfp4_quantize gave. More rows than few take a workspace for x's packed form."""
     if not isinstance(x, torch.Tensor):
         return None, x[0], x[1], x[0]
-    if x.dim() < 1 or x.shape[-1] == 0 or not x.is_cuda:
+    shape = x.shape
+    if not shape or shape[-1] == 0 or not x.is_cuda:
         return x, None, None, x
-    rows = x.numel() // x.shape[-1]
+    k = shape[-1]
+    rows = x.numel() // k
     if rows <= _MX_FEW_ROWS:
         return x, None, None, x
-    return (x, *_mx_packed(rows, (rows,), x.shape[-1], x.device), x)
+    return (x, x.new_empty((rows, k // 2), dtype=torch.uint8),
+            x.new_empty(((k + 127) // 128, rows, 4), dtype=torch.uint8), x)
 
 
 def mxfp4_linear_fp4(x, q: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -601,30 +628,32 @@ def mxfp4_linear_fp4(x, q: torch.Tensor, scales: torch.Tensor, bias: Optional[to
     """mxfp4_linear with x in 4 bits too: quantized here (x a tensor), or the pair that mxfp4_quantize gave (one
     quantization for several projections). out_dtype defaults to x's type, bf16 for a pair."""
     fn = "lux3d_mxfp4_linear_fp4"
-    plain, xq, xs, lead = _mx_x(fn, x)
+    plain, xq, xs, lead = _mx_x(x)
     _one_device(fn, lead, xs, q, scales, bias)
-    with _device_of(lead):
-        dt = out_dtype or (torch.bfloat16 if plain is None else plain.dtype)
-        y = torch.empty((*lead.shape[:-1], q.shape[0]), dtype=dt, device=lead.device)
-        _lib.call(fn, _d(plain), _d(xq), _d(xs), _d(q), _d(scales), _d(bias), _d(y), _stream(lead))
+    if plain is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    y = lead.new_empty((*lead.shape[:-1], q.shape[0]), dtype=out_dtype)
+    _mx_call(fn, lead, _b(plain), _b(xq), _b(xs), _b(q), _b(scales), _b(bias), _b(y))
     return y
 
 
 def mxfp4_linear_gated(x, gate, up, act: str = "silu", *, gate_bias: Optional[torch.Tensor] = None,
                        up_bias: Optional[torch.Tensor] = None, fp4: bool = False, out_dtype=None) -> torch.Tensor:
-    """act(x @ Wg^T + gate_bias) * (x @ Wu^T + up_bias) in one kernel, the first half of a gated feed-forward block
+    """act(x @ Wg^T + gate_bias) * (x @ Wu^T + up_bias) in one pass, the first half of a gated feed-forward block
     (GeGlu::forward, runtime/nn_blocks.rs:238-254, and its kin). gate, up: (q, scales) of packed weights [n, k]; act
     "silu", "gelu_erf" or "gelu_tanh". fp4: x enters in 4 bits, as in mxfp4_linear_fp4 (a pair is possible then)."""
     fn = "lux3d_mxfp4_linear_gated"
-    if act not in _ACTS:
+    code = _ACTS.get(act)
+    if code is None:
         raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"act must be one of {sorted(_ACTS)}, not {act!r}")
-    plain, xq, xs, lead = _mx_x(fn, x) if fp4 else (x, None, None, x)
-    _one_device(fn, lead, xs, *gate, gate_bias, *up, up_bias)
-    with _device_of(lead):
-        dt = out_dtype or (torch.bfloat16 if plain is None else plain.dtype)
-        y = torch.empty((*lead.shape[:-1], up[0].shape[0]), dtype=dt, device=lead.device)
-        _lib.call(fn, _d(plain), _d(xq), _d(xs), _d(gate[0]), _d(gate[1]), _d(gate_bias), _d(up[0]), _d(up[1]), _d(up_bias),
-                  _ACTS[act], 1 if fp4 else 0, _d(y), _stream(lead))
+    plain, xq, xs, lead = _mx_x(x) if fp4 else (x, None, None, x)
+    (gq, gs), (uq, us) = gate, up
+    _one_device(fn, lead, xs, gq, gs, gate_bias, uq, us, up_bias)
+    if plain is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    y = lead.new_empty((*lead.shape[:-1], uq.shape[0]), dtype=out_dtype)
+    _mx_call(fn, lead, _b(plain), _b(xq), _b(xs), _b(gq), _b(gs), _b(gate_bias), _b(uq), _b(us), _b(up_bias), code,
+             1 if fp4 else 0, _b(y))
     return y
 
 
