@@ -107,23 +107,22 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
 
 // ---- linear, few rows -----------------------------------------------------------
 //
-// A workgroup owns 16 weight rows (of each matrix) and MT tiles of 16 rows of
-// x; its NW wavefronts take groups of 128 of k in turn and add their sums in
+// A workgroup owns NT tiles of 16 weight rows (of each matrix) and MT tiles of
+// 16 rows of x; its NW wavefronts take groups of 128 of k in turn and add their sums in
 // wavefront order through LDS. Lane l holds row l % 16 and block l / 16 of the
 // group of either operand: 16 bytes of a packed row, 32 values of a plain one.
 //   fp4    one v_mfma_scale_f32_16x16x128_f8f6f4 a group, each lane's scale its
 //          own block's; plain x is quantised in the lane that holds the block
 //   plain  four v_mfma_f32_16x16x32 on the block's four eighths; the weights'
 //          values are exact in bf16; f32 x in three exact bf16 terms
-template <typename X, bool FP4, bool GATED, int MT, int NW>
+template <typename X, bool FP4, bool GATED, int MT, int NT, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAct act) {
   constexpr bool PACKED = std::is_void_v<X>;
-  constexpr int NM = GATED ? 2 : 1;
+  constexpr int NM = GATED ? 2 * NT : NT;  // weight tiles: the gate's behind the others
   __shared__ float part[NW][NM][MT][256];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, l16 = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 16 * MT;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NT, m0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 16 * MT;
   if (m0 >= p.M) return;  // uniform
-  const int64_t n = n0 + l16 < p.N ? n0 + l16 : p.N - 1;  // past N: clamped, never stored
   const int64_t nb = p.K / 32, groups = (nb + 3) / 4;
   f32x4_t acc[NM][MT];
 #pragma unroll
@@ -141,8 +140,9 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
     const bool live = b < nb;  // a last group may have fewer than four blocks: the others count as 0
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
-      q.w[j] = ld16<false>(p.w[j] + n * (p.K / 2) + (live ? b : nb - 1) * 16);
-      q.sw[j] = live ? p.ws[j][(c * p.N + n) * 4 + g] : 0;
+      const int64_t at = n0 + 16 * (j % NT) + l16, n = at < p.N ? at : p.N - 1;  // past N: clamped, never stored
+      q.w[j] = ld16<false>(p.w[j / NT] + n * (p.K / 2) + (live ? b : nb - 1) * 16);
+      q.sw[j] = live ? p.ws[j / NT][(c * p.N + n) * 4 + g] : 0;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -241,30 +241,31 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
 #pragma unroll
       for (int e = 0; e < 4; ++e) part[wave][j][i][e * 64 + lane] = acc[j][i][e];
   __syncthreads();
-  for (int o = t; o < MT * 256; o += 64 * NW) {
-    const int c = o & 15, r = (o >> 4) & 15, i = o >> 8, at = (c & 3) * 64 + (c >> 2) * 16 + r;
-    const int64_t row = m0 + 16 * i + r, col = n0 + c;
+  for (int o = t; o < MT * NT * 256; o += 64 * NW) {
+    const int c16 = o % (16 * NT), tile = c16 >> 4, c = c16 & 15, r = o / (16 * NT) & 15, i = o / (256 * NT);
+    const int at = (c & 3) * 64 + (c >> 2) * 16 + r;
+    const int64_t row = m0 + 16 * i + r, col = n0 + c16;
     if (row >= p.M || col >= p.N) continue;
-    float v[NM];
+    float v[2];
 #pragma unroll
-    for (int j = 0; j < NM; ++j) {
-      v[j] = part[0][j][i][at];
+    for (int j = 0; j < NM / NT; ++j) {
+      v[j] = part[0][j * NT + tile][i][at];
 #pragma unroll
-      for (int k = 1; k < NW; ++k) v[j] += part[k][j][i][at];
+      for (int k = 1; k < NW; ++k) v[j] += part[k][j * NT + tile][i][at];
       if (p.bias[j]) v[j] += p.bias[j][col];
     }
     float y = v[0];
-    if constexpr (GATED) y *= mx_activate(act, v[NM - 1]);
+    if constexpr (GATED) y *= mx_activate(act, v[1]);
     mx_store(p.y, p.y_dt, row * p.ldy + col, y);
   }
 }
 
-template <typename X, bool FP4, bool GATED, int MT, int NW>
+template <typename X, bool FP4, bool GATED, int MT, int NT, int NW>
 hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
-  const int64_t tn = (p.N + 15) / 16, tm = (p.M + 16 * MT - 1) / (16 * MT), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
+  const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
   if (tn > INT32_MAX || z > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tn, (unsigned)((tm + z - 1) / z), (unsigned)z);
-  hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, MT, NW>), grid, dim3(64 * NW), 0, s, p, mx_act(p.act));
+  hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, MT, NT, NW>), grid, dim3(64 * NW), 0, s, p, mx_act(p.act));
   return hipGetLastError();
 }
 
@@ -275,8 +276,13 @@ hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
 // 35.6, 2048 -> 8192 19.9 -> 19.6. Two groups in flight a wavefront: within 8%.
 template <typename X, bool FP4, bool GATED>
 hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
-  if (p.M > 16) return launch_rows_kernel<X, FP4, GATED, 2, 8>(p, s);
-  return p.K >= 6144 ? launch_rows_kernel<X, FP4, GATED, 1, 16>(p, s) : launch_rows_kernel<X, FP4, GATED, 1, 8>(p, s);
+  if (p.M > 16) return launch_rows_kernel<X, FP4, GATED, 2, 1, 8>(p, s);
+  constexpr bool two_byte = !FP4 && std::conditional_t<FP4, F32, X>::bytes == 2;
+  const int nt = mx_few_tiles(two_byte, p.N, p.K, GATED);
+  if constexpr (!GATED)
+    if (nt == 4) return launch_rows_kernel<X, FP4, GATED, 1, 4, 8>(p, s);
+  if (nt == 2) return launch_rows_kernel<X, FP4, GATED, 1, 2, 8>(p, s);
+  return p.K >= 6144 ? launch_rows_kernel<X, FP4, GATED, 1, 1, 16>(p, s) : launch_rows_kernel<X, FP4, GATED, 1, 1, 8>(p, s);
 }
 
 template <typename X, bool FP4>

@@ -25,8 +25,26 @@ struct MxChoice {
 
 inline double mx_up(int64_t a, int64_t b) { return (double)((a + b - 1) / b); }
 
+// Weight tiles of 16 rows that a workgroup of the few-rows kernel takes for up to
+// 16 rows of x, which is read, and quantised or split into its terms, once for all
+// of them: more than one where enough workgroups are left. us with 1 / 2 / 4, 1
+// and 16 rows:
+//   bf16 2048 -> 8192    4.4 / 4.2 / 7.0 and 7.7 / 6.6 / 9.5
+//        4096 -> 16384  12.2 / 10.2 / 11.6 and 22.3 / 15.9 / 14.5
+//        4096 -> 32000  20.1 / 16.9 / 15.7 and 40.4 / 27.4 / 22.1
+//   f32  4096 -> 16384  19.1 / 14.8 / 14.6 and 37.1 / 23.6 / 19.2
+//   x in 4 bits, bf16 4096 -> 16384  11.8 / 10.6 / 9.3 and 21.9 / 15.6 / 13.1
+//   bf16 8192 -> 2048    6.9 / 9.2 / 13.3 and 12.6 / 16.2 / 21.6
+//   gated bf16 1536 -> 9216   7.1 / 8.4 / 10.5 and 10.5 / 12.5 / 13.7
+//              4096 -> 16384 17.2 / 15.4 / 19.2 and 27.1 / 21.9 / 22.7
+inline int mx_few_tiles(bool plain_2byte, int64_t n, int64_t k, bool gated) {
+  if (gated) return n >= 16384 && k >= 1024 ? 2 : 1;
+  if (n < 8192 || k < 512) return 1;
+  return k >= 1024 && n >= (plain_2byte ? 24576 : 16384) ? 4 : 2;
+}
+
 // Us of the few-rows kernel: a launch, the chain of a wavefront's groups of 128
-// of k, and the workgroups' loads of weights and of x, by the rows of their tile.
+// of k, and the loads of weights and of x, by the rows of a workgroup's tile.
 // Fitted to 48, 24 and 24 sizes of up to 16 rows and 150 to 168 of more, within
 // 8 to 16% (root mean square).
 inline double mx_few_cost(MxKind kind, int64_t m, int64_t n, int64_t k, bool gated) {
@@ -38,7 +56,8 @@ inline double mx_few_cost(MxKind kind, int64_t m, int64_t n, int64_t k, bool gat
   const bool few = m <= 16;
   const double *c = f[kind][few ? 0 : 1];
   const int64_t t = few ? 16 : 32;
-  const double g = mx_up(k, 128), w = mx_up(n, 16) * mx_up(m, t) / 256, rows = (double)(m < t ? m : t);
+  const double g = mx_up(k, 128), w = mx_up(n, 16) * mx_up(m, t) / 256;
+  const double rows = (double)(m < t ? m : t) / (few ? mx_few_tiles(kind == MX_2BYTE, n, k, gated) : 1);
   return c[0] + c[1] * std::ceil(g / (few && k >= 6144 ? 16 : 8)) * (gated ? 1.41 : 1) + w * (g * (c[2] * (gated ? 2 : 1) + c[3] * rows) + c[4]);
 }
 
