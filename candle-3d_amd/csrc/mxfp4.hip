@@ -15,20 +15,25 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 // ---- quantisation ---------------------------------------------------------------
 //
-// A stream: x read once, 17 / 32 byte a value written. A workgroup takes 32
-// rows x 512 values; a wavefront reads a row's 512 with 8 values a lane (4
-// lanes a block, the block's maximum by two DPP steps), 8 rows in flight, and
-// writes 256 contiguous bytes of codes a row. The scales go through LDS: a
-// group's bytes of 32 rows are one 128-byte line.
-constexpr int kQuantRows = 32, kQuantCols = 512;
+// A stream: x read once, 17 / 32 byte a value written. A workgroup takes 4 R rows
+// x 512 values; a wavefront reads a row's 512 with 8 values a lane (4 lanes a
+// block, the block's maximum by two DPP steps), R rows in flight, and writes 256
+// contiguous bytes of codes a row. The scales go through LDS: a group's bytes of
+// 4 R rows are adjacent. R is 4, and 2 where that leaves fewer than two workgroups
+// a CU (us with R of 8 / 4 / 2: 777 x 1120 bf16 3.4 / 2.8 / 2.5, 1029 x 1024 f32
+// 4.8 / 3.0 / 2.6, 4098 x 2048 bf16 5.8 / 5.0 / 5.0, 9001 x 1536 8.2 / 7.4 / 7.9,
+// 64000 x 1536 41.1 / 40.4 / 43.9, 8192 x 2048 f32 17.0 / 14.8 / 14.7: 5.1 to 6.2
+// TB/s where the launch does not count).
+constexpr int kQuantCols = 512;
+inline int64_t mx_quant_tiles(int64_t rows, int64_t k, int r) { return (k + kQuantCols - 1) / kQuantCols * ((rows + 4 * r - 1) / (4 * r)); }
 
-template <typename T>
+template <typename T, int R>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
-  constexpr int NV = T::bytes == 4 ? 2 : 1, R = kQuantRows / 4;  // 16-byte loads a lane and row; rows a wavefront
-  __shared__ uint32_t sc[4][kQuantRows];
+  constexpr int NV = T::bytes == 4 ? 2 : 1;  // 16-byte loads a lane and row
+  __shared__ uint32_t sc[4][4 * R];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
-  const int64_t r0 = rt * kQuantRows, k = kt * kQuantCols + lane * 8;
+  const int64_t r0 = rt * (4 * R), k = kt * kQuantCols + lane * 8;
   const bool live = k < p.K;
   uint32_t v[R][4 * NV];
 #pragma unroll
@@ -60,22 +65,22 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
     if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(&sc[lane >> 4][wave * R + i])[(lane >> 2) & 3] = (uint8_t)s;
   }
   __syncthreads();
-  const int64_t g = kt * 4 + (t >> 5), r = r0 + (t & 31);
-  if (t < 128 && g * 128 < p.K && r < p.M) reinterpret_cast<uint32_t *>(p.s)[g * p.M + r] = sc[t >> 5][t & 31];
+  const int64_t g = kt * 4 + t / (4 * R), r = r0 + t % (4 * R);
+  if (t < 16 * R && g * 128 < p.K && r < p.M) reinterpret_cast<uint32_t *>(p.s)[g * p.M + r] = sc[t / (4 * R)][t % (4 * R)];
 }
 
 // ---- and back -------------------------------------------------------------------
 //
-// The same tiles of 32 rows x 512 values, 8 rows of a wavefront in flight. A
-// lane writes 16 bytes and the next lane the 16 behind them: 8 values of a
-// 2-byte type, 4 of f32, which takes the row's half in two steps (16 values a
-// lane and four stores 64 bytes apart instead: 8192 x 2048 f32 50 us).
-template <typename T>
+// The same tiles, R rows of a wavefront in flight. A lane writes 16 bytes and the
+// next lane the 16 behind them: 8 values of a 2-byte type, 4 of f32, which takes
+// the row's half in two steps (16 values a lane and four stores 64 bytes apart
+// instead: 8192 x 2048 f32 50 us against 12).
+template <typename T, int R>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
-  constexpr int V = 16 / T::bytes, STEPS = 8 / V, R = kQuantRows / 4;  // values a lane and step
+  constexpr int V = 16 / T::bytes, STEPS = 8 / V;  // values a lane and step
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
-  const int64_t r0 = rt * kQuantRows + wave * R;
+  const int64_t r0 = rt * (4 * R) + wave * R;
 #pragma unroll
   for (int step = 0; step < STEPS; ++step) {
     const int64_t k = kt * kQuantCols + step * (kQuantCols / STEPS) + lane * V;
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(MxLinearParams p, MxAc
 template <typename X, bool FP4, bool GATED, int MT, int NT, int NW>
 hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
   const int64_t tn = (p.N + 16 * NT - 1) / (16 * NT), tm = (p.M + 16 * MT - 1) / (16 * MT), z = (tm + 65534) / 65535;  // a grid's y and z end at 65535
-  if (tn > INT32_MAX || z > 65535) return hipErrorInvalidValue;
+  if (tn * 64 * NW > UINT32_MAX || z > 65535) return hipErrorInvalidValue;  // a launch's work-items along x
   const dim3 grid((unsigned)tn, (unsigned)((tm + z - 1) / z), (unsigned)z);
   hipLaunchKernelGGL((mx_rows_kernel<X, FP4, GATED, MT, NT, NW>), grid, dim3(64 * NW), 0, s, p, mx_act(p.act));
   return hipGetLastError();
@@ -298,30 +303,40 @@ template <typename X> hipError_t launch_rows_x(const MxLinearParams &p, hipStrea
 
 hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s) {
   if (p.M <= 0) return hipSuccess;
-  const int64_t tiles = (p.K + kQuantCols - 1) / kQuantCols * ((p.M + kQuantRows - 1) / kQuantRows);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)tiles);
+  const bool two = mx_quant_tiles(p.M, p.K, 4) < 512;
+  const int64_t tiles = mx_quant_tiles(p.M, p.K, two ? 2 : 4);
+  if (tiles * 256 > UINT32_MAX) return hipErrorInvalidValue;  // a launch's work-items
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (two) hipLaunchKernelGGL((mx_quantize_kernel<T, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((mx_quantize_kernel<T, 4>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    return hipGetLastError();
+  };
   switch (p.x_dt) {
-    case LUX3D_F32: hipLaunchKernelGGL(mx_quantize_kernel<F32>, grid, dim3(256), 0, s, p); break;
-    case LUX3D_BF16: hipLaunchKernelGGL(mx_quantize_kernel<BF16>, grid, dim3(256), 0, s, p); break;
-    case LUX3D_F16: hipLaunchKernelGGL(mx_quantize_kernel<F16>, grid, dim3(256), 0, s, p); break;
-    default: return hipErrorInvalidValue;
+    case LUX3D_F32: return launch(F32{});
+    case LUX3D_BF16: return launch(BF16{});
+    case LUX3D_F16: return launch(F16{});
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s) {
   if (p.M <= 0) return hipSuccess;
-  const int64_t tiles = (p.K + kQuantCols - 1) / kQuantCols * ((p.M + kQuantRows - 1) / kQuantRows);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)tiles);
+  const bool two = mx_quant_tiles(p.M, p.K, 4) < 512;
+  const int64_t tiles = mx_quant_tiles(p.M, p.K, two ? 2 : 4);
+  if (tiles * 256 > UINT32_MAX) return hipErrorInvalidValue;  // a launch's work-items
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (two) hipLaunchKernelGGL((mx_dequantize_kernel<T, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((mx_dequantize_kernel<T, 4>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    return hipGetLastError();
+  };
   switch (p.y_dt) {
-    case LUX3D_F32: hipLaunchKernelGGL(mx_dequantize_kernel<F32>, grid, dim3(256), 0, s, p); break;
-    case LUX3D_BF16: hipLaunchKernelGGL(mx_dequantize_kernel<BF16>, grid, dim3(256), 0, s, p); break;
-    case LUX3D_F16: hipLaunchKernelGGL(mx_dequantize_kernel<F16>, grid, dim3(256), 0, s, p); break;
-    default: return hipErrorInvalidValue;
+    case LUX3D_F32: return launch(F32{});
+    case LUX3D_BF16: return launch(BF16{});
+    case LUX3D_F16: return launch(F16{});
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 namespace {

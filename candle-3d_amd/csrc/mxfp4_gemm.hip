@@ -233,9 +233,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
     lds_barrier();
   };
 
-  // Fragments. Weight tile j lies in rows wrow(j) of the stage, x tile i in (wm TM + i) * 32.
-  auto wrow = [&](int j) { return (j / T::TO) * T::BNO + (wn * T::TO + j % T::TO) * 32; };
-  // a lane's place in a stage: of x for each 16-byte piece that it reads, of the weights, of the scales
+  // Fragments. Weight tile j lies in rows (j / TO) BNO + (wn TO + j % TO) 32 of the stage, x tile i in (wm TM + i) 32. A lane's
+  // place in a stage: of x for each 16-byte piece that it reads, of the weights, of the scales
   constexpr int XPC = T::PACKED ? 2 : 4;             // pieces of a lane
   int xat[XPC], wat[2], wsat, xsat = 0;
 #pragma unroll
@@ -550,8 +549,8 @@ template <typename X, int WM, int WN, int TM, int TN, int NS, int KG, bool PERSI
 hipError_t launch_tile(const MxLinearParams &p, hipStream_t s) {
   using T = MxTile<X, WM, WN, TM, TN, NS, KG, PERSIST, GATED>;
   const int64_t tiles_m = (p.M + T::BM - 1) / T::BM, tiles_n = (p.N + T::BNO - 1) / T::BNO;
-  if (tiles_m * tiles_n > INT32_MAX) return hipErrorInvalidValue;
   const int64_t tiles = tiles_m * tiles_n, cus = PERSIST ? cu_count(s) : tiles;
+  if (tiles > INT32_MAX || (tiles < cus ? tiles : cus) * 64 * T::NW * KG > UINT32_MAX) return hipErrorInvalidValue;
   hipLaunchKernelGGL((mx_gemm_kernel<X, WM, WN, TM, TN, NS, KG, PERSIST, GATED>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(64 * T::NW * KG), 0, s, p,
                      mx_act(p.act), (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
@@ -579,7 +578,8 @@ hipError_t launch_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s
     if (is(64, 128, 2)) return launch_tile<X, 2, 2, 1, 2, 4, 2, false, GATED>(p, s);
     if (is(64, 128, 4)) return launch_tile<X, 2, 2, 1, 2, 3, 4, false, GATED>(p, s);
     if (is(128, 128, 1)) return launch_tile<X, 2, 2, 2, 2, 3, 1, false, GATED>(p, s);
-    if (is(128, 256, 1)) return launch_tile<X, 2, 2, 2, 4, 3, 1, false, GATED>(p, s);
+    // two wavefronts a SIMD (four of 64 x 128 in all: 4096 rows of 8192 -> 2048 122 us against 118)
+    if (is(128, 256, 1)) return launch_tile<X, 2, 4, 2, 2, 3, 1, false, GATED>(p, s);
     if (is(256, 256, 1)) return launch_tile<X, 2, 4, 4, 2, 3, 1, false, GATED>(p, s);
   } else {
     // a wavefront's 32 rows of x meet 128 weight rows, so that each value is split into its three terms once a workgroup

@@ -63,13 +63,13 @@ def dense(q, scales):
 
 def product(x, w, bias, e_x=0.0):
     """(x W^T + bias, a bound on the error of its f32 sum). A sum of K products is formed in f32 from pieces of 16 products
-    at least, so it is off by at most (K / 16 + 64) u of its terms' magnitudes; f32 x enters as three bf16 terms, each
-    product within 2 u."""
+    at least, so it is off by at most (K / 16 + 64) u of its terms' magnitudes, the bias among them (tiles: the sum starts
+    at it, and it passes every one of the K / 16 + 64 additions); f32 x enters as three bf16 terms, each product within 2 u."""
     xd, wd = x.double(), w.double()
     y = torch.mm(xd, wd.t().contiguous())
     err = torch.mm(xd.abs(), wd.abs().t().contiguous()) * ((x.shape[1] / 16 + 64) * U + e_x)
     if bias is not None:
-        y, err = y + bias.double(), err + U * bias.double().abs()
+        y, err = y + bias.double(), err + (x.shape[1] / 16 + 64) * U * bias.double().abs()
     return y, err + U * y.abs()
 
 
