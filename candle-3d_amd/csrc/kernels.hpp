@@ -215,6 +215,7 @@ struct MxLinearParams {
   int act = -1;                                             // Act; -1: no gate
   void *y = nullptr; int64_t ldy = 0; int y_dt = 0;         // [M, N] rows
   int64_t M = 0, N = 0, K = 0;
+  int64_t rest = 0;                                         // kernel for many rows: rows behind M, 16 at most, as few rows
 };
 hipError_t launch_mx_linear(const MxLinearParams &p, hipStream_t s);
 // Its kernel for many rows (mxfp4_gemm.hip): whether a call's sizes fit it; with packed x (p.x null) or plain, not fp4.

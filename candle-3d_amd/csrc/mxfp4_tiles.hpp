@@ -16,8 +16,8 @@ struct MxTileId {
   int rows, cols, groups;
 };
 
-// The rows below `rows` in tiles of `tile`, the rest (16 at most; all of them
-// where rows is 0) by the few-rows kernel.
+// The rows below `rows` in tiles of `tile`, the rest (16 at most) as few rows in
+// the same launch; rows 0: the few-rows kernel takes all.
 struct MxChoice {
   MxTileId tile;
   int64_t rows;
@@ -74,26 +74,27 @@ inline double mx_few_cost(MxKind kind, int64_t m, int64_t n, int64_t k, bool gat
 struct MxCost {
   MxTileId tile;
   double c, a, b, s, th;
+  bool beside;  // two workgroups fit a CU's LDS
 };
 
 inline MxChoice mx_choose(MxKind kind, int64_t m, int64_t n, int64_t k, bool gated) {
-  constexpr MxCost packed[] = {{{64, 64, 1}, 2.76, 0.142, 0.92, 0.88, 0.72},
-                               {{64, 64, 2}, 1.99, 0.240, 2.16, 0.90, 1.00},
-                               {{64, 128, 1}, 3.10, 0.190, 1.17, 1.04, 0.69},
-                               {{128, 128, 1}, 2.97, 0.286, 2.82, 0.98, 0.80},
-                               {{256, 256, 1}, 6.78, 0.595, 4.75, 1.35, 0.69}};
-  constexpr MxCost two[] = {{{64, 64, 1}, 2.88, 0.257, 1.19, 0.68, 0.95},
-                            {{64, 64, 2}, 1.71, 0.333, 3.00, 1.09, 0.89},
-                            {{64, 64, 4}, 3.38, 0.576, 2.55, 1.24, 0.78},
-                            {{64, 128, 1}, 3.34, 0.297, 1.33, 0.87, 0.64},
-                            {{64, 128, 2}, 2.12, 0.453, 3.57, 1.07, 0.97},
-                            {{64, 128, 4}, 4.14, 0.764, 3.58, 1.27, 0.75},
-                            {{128, 128, 1}, 3.13, 0.419, 2.75, 0.98, 0.59},
-                            {{128, 256, 1}, 5.45, 0.705, 3.89, 1.03, 0.65},
-                            {{256, 256, 1}, 2.42, 1.070, 9.59, 1.21, 0.77}};
-  constexpr MxCost f32[] = {{{64, 64, 4}, 2.83, 1.011, 3.83, 1.08, 0.92},
-                            {{64, 128, 2}, 3.77, 0.666, 3.00, 0.91, 0.72},
-                            {{64, 128, 4}, 3.78, 1.083, 5.16, 1.17, 0.86}};
+  constexpr MxCost packed[] = {{{64, 64, 1}, 2.76, 0.142, 0.92, 0.88, 0.72, true},
+                               {{64, 64, 2}, 1.99, 0.240, 2.16, 0.90, 1.00, true},
+                               {{64, 128, 1}, 3.10, 0.190, 1.17, 1.04, 0.69, true},
+                               {{128, 128, 1}, 2.97, 0.286, 2.82, 0.98, 0.80, true},
+                               {{256, 256, 1}, 6.78, 0.595, 4.75, 1.35, 0.69, false}};
+  constexpr MxCost two[] = {{{64, 64, 1}, 2.88, 0.257, 1.19, 0.68, 0.95, true},
+                            {{64, 64, 2}, 1.71, 0.333, 3.00, 1.09, 0.89, false},
+                            {{64, 64, 4}, 3.38, 0.576, 2.55, 1.24, 0.78, false},
+                            {{64, 128, 1}, 3.34, 0.297, 1.33, 0.87, 0.64, true},
+                            {{64, 128, 2}, 2.12, 0.453, 3.57, 1.07, 0.97, false},
+                            {{64, 128, 4}, 4.14, 0.764, 3.58, 1.27, 0.75, false},
+                            {{128, 128, 1}, 3.13, 0.419, 2.75, 0.98, 0.59, true},
+                            {{128, 256, 1}, 5.45, 0.705, 3.89, 1.03, 0.65, true},
+                            {{256, 256, 1}, 2.42, 1.070, 9.59, 1.21, 0.77, false}};
+  constexpr MxCost f32[] = {{{64, 64, 4}, 2.83, 1.011, 3.83, 1.08, 0.92, false},
+                            {{64, 128, 2}, 3.77, 0.666, 3.00, 0.91, 0.72, true},
+                            {{64, 128, 4}, 3.78, 1.083, 5.16, 1.17, 0.86, false}};
   const MxCost *costs = kind == MX_PACKED ? packed : kind == MX_2BYTE ? two : f32;
   const int count = kind == MX_PACKED ? 5 : kind == MX_2BYTE ? 9 : 3;
   const int64_t depth = kind == MX_PACKED ? 128 : kind == MX_2BYTE ? 64 : 32;
@@ -115,10 +116,12 @@ inline MxChoice mx_choose(MxKind kind, int64_t m, int64_t n, int64_t k, bool gat
       least = whole;
       best = {t.tile, m};
     }
-    // few rows past the last whole tile: a launch of their own where that saves a row of tiles (2 x 2049 tokens)
+    // Few rows past the last whole tile (2 x 2049 tokens) as few rows, where that saves a row of tiles. Beside the tiles they
+    // cost a tenth to two thirds of their own launch (1029 rows against 1024, us: f32 1024 -> 4096 28.4 / 27.5, gated f16
+    // 23.8 / 21.0, 4098 against 4096, 1024 -> 4096 bf16 35.0 / 33.4), behind them, where no second workgroup fits a CU, all of it.
     const int64_t rest = m % t.tile.rows;
     if (rest >= 1 && rest <= 16 && m > t.tile.rows) {
-      const double split = cost(m - rest) + mx_few_cost(kind, rest, n, k, gated);
+      const double split = cost(m - rest) + (t.beside ? 0.4 : 1) * mx_few_cost(kind, rest, n, k, gated);
       if (split < least) {
         least = split;
         best = {t.tile, m - rest};

@@ -468,8 +468,7 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  *      k]; bias: f32 [n] or NULL; y: [..., n] rows, f32 / bf16 / f16.
  * Weights enter as x's type holds them (exact in bf16 and f32; f16: exact for
  * block scales 2^-23 to 2^13, rounded beyond), products and sums are f32, f32 x
- * in three exact bf16 terms; y is rounded once. One kernel, or two: up to 16 rows
- * past the last whole tile go to the kernel of few rows where that is shorter.
+ * in three exact bf16 terms; y is rounded once. One kernel.
  *
  * lux3d_mxfp4_linear_fp4: x is quantized as by lux3d_mxfp4_quantize first, and
  * the products of 4-bit values run on the scaled matrix instructions, four times
@@ -481,7 +480,7 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  *      between calls; no two calls that may overlap share them.
  *   x NULL: xq and xs hold the packed x already (one quantization for several
  *      projections); its bits are those that the quantization of x would give.
- * One kernel for few rows, else lux3d_mxfp4_linear's behind one that quantizes x.
+ * One kernel for few rows or packed x, else two.
  *
  * lux3d_mxfp4_linear_gated: act(x Wg^T + bg) * (x Wu^T + bu), the first half of
  * a gated feed-forward block, in one pass: GeGlu::forward (runtime/nn_blocks.rs:

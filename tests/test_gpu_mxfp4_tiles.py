@@ -5,116 +5,132 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import mxfp4_reference as ref  # noqa: E402
-from test_gpu_mxfp4 import DT, as_products_see, call, dev, ops, rnd, run_gated, run_linear, same_as_defined, tokens, weight  # noqa: E402,F401
+from test_gpu_mxfp4 import DT, dev, ops, rnd, run_gated, run_linear, same_as_defined, tokens, weight  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
 # how x enters, gated, tile rows, columns, groups that share k, few rows past the last tile apart, m, k, n: the choice of
 # csrc/mxfp4_tiles.hpp, which test_mxfp4_tiles_cpu.py holds to this list
 TILES = [
-    ("fp4", False, 64, 64, 1, False, 456, 32, 562),
-    ("fp4", False, 64, 64, 1, False, 455, 128, 561),
-    ("fp4", False, 64, 64, 2, False, 455, 2784, 433),
-    ("fp4", False, 64, 64, 2, False, 452, 2816, 435),
-    ("fp4", False, 64, 128, 1, False, 1345, 32, 965),
-    ("fp4", False, 64, 128, 1, False, 1217, 128, 1089),
-    ("fp4", False, 128, 128, 1, False, 2305, 288, 1567),
-    ("fp4", False, 128, 128, 1, False, 1987, 384, 1847),
-    ("fp4", False, 128, 128, 1, True, 2569, 960, 3125),
-    ("fp4", False, 128, 128, 1, True, 4102, 896, 2025),
-    ("fp4", False, 256, 256, 1, False, 2492, 544, 4154),
-    ("fp4", False, 256, 256, 1, False, 3400, 512, 2949),
-    ("fp4", False, 256, 256, 1, True, 4612, 608, 3420),
-    ("fp4", False, 256, 256, 1, True, 3329, 512, 4663),
-    ("fp4", True, 64, 128, 1, False, 549, 32, 567),
-    ("fp4", True, 64, 128, 1, False, 645, 128, 481),
-    ("fp4", True, 128, 128, 1, False, 1239, 288, 1473),
-    ("fp4", True, 128, 128, 1, False, 1418, 384, 1282),
-    ("fp4", True, 128, 128, 1, True, 3587, 2976, 560),
-    ("fp4", True, 128, 128, 1, True, 2945, 1792, 2776),
-    ("fp4", True, 256, 256, 1, False, 1966, 544, 2633),
-    ("fp4", True, 256, 256, 1, False, 1734, 512, 2891),
-    ("fp4", True, 256, 256, 1, True, 1293, 576, 5695),
-    ("fp4", True, 256, 256, 1, True, 2064, 512, 3731),
-    ("2byte", False, 64, 64, 1, False, 514, 32, 468),
-    ("2byte", False, 64, 64, 1, False, 513, 128, 577),
-    ("2byte", False, 64, 64, 2, False, 614, 480, 533),
-    ("2byte", False, 64, 64, 2, False, 577, 512, 561),
-    ("2byte", False, 64, 64, 4, False, 376, 3552, 472),
-    ("2byte", False, 64, 64, 4, False, 322, 3584, 482),
-    ("2byte", False, 64, 128, 1, False, 1615, 32, 1217),
-    ("2byte", False, 64, 128, 1, False, 1166, 128, 1665),
-    ("2byte", False, 64, 128, 1, True, 2510, 992, 1558),
-    ("2byte", False, 64, 128, 1, True, 1601, 896, 2512),
-    ("2byte", False, 64, 128, 2, False, 779, 992, 1267),
-    ("2byte", False, 64, 128, 2, False, 1092, 1024, 925),
-    ("2byte", False, 64, 128, 2, True, 1159, 1632, 1709),
-    ("2byte", False, 64, 128, 2, True, 1474, 1024, 1359),
-    ("2byte", False, 64, 128, 4, False, 864, 3744, 1185),
-    ("2byte", False, 64, 128, 4, False, 907, 3840, 1127),
-    ("2byte", False, 64, 128, 4, True, 1098, 4000, 1899),
-    ("2byte", False, 64, 128, 4, True, 1164, 4096, 1685),
-    ("2byte", False, 128, 128, 1, False, 2191, 160, 1683),
-    ("2byte", False, 128, 128, 1, False, 1799, 256, 1923),
-    ("2byte", False, 128, 128, 1, True, 2955, 576, 1361),
-    ("2byte", False, 128, 128, 1, True, 1668, 640, 2347),
-    ("2byte", False, 128, 256, 1, False, 5833, 32, 3853),
-    ("2byte", False, 128, 256, 1, False, 3083, 128, 4886),
-    ("2byte", False, 128, 256, 1, True, 4225, 160, 5809),
-    ("2byte", False, 128, 256, 1, True, 6150, 128, 4085),
-    ("2byte", False, 256, 256, 1, False, 3845, 32, 3471),
-    ("2byte", False, 256, 256, 1, False, 3588, 128, 3371),
-    ("2byte", False, 256, 256, 1, True, 5391, 160, 2819),
-    ("2byte", False, 256, 256, 1, True, 4109, 128, 3972),
-    ("2byte", True, 64, 128, 1, False, 551, 32, 437),
-    ("2byte", True, 64, 128, 1, False, 577, 128, 515),
-    ("2byte", True, 64, 128, 1, True, 4677, 992, 391),
-    ("2byte", True, 64, 128, 1, True, 1483, 1024, 1379),
-    ("2byte", True, 64, 128, 2, False, 569, 1120, 405),
-    ("2byte", True, 64, 128, 2, False, 365, 1152, 596),
-    ("2byte", True, 64, 128, 2, True, 1031, 1824, 967),
-    ("2byte", True, 64, 128, 2, True, 972, 1792, 1042),
-    ("2byte", True, 64, 128, 4, False, 458, 3808, 389),
-    ("2byte", True, 64, 128, 4, False, 455, 3840, 413),
-    ("2byte", True, 64, 128, 4, True, 582, 3744, 1684),
-    ("2byte", True, 64, 128, 4, True, 1097, 3840, 921),
-    ("2byte", True, 128, 128, 1, False, 1634, 160, 1154),
-    ("2byte", True, 128, 128, 1, False, 1415, 256, 1222),
-    ("2byte", True, 128, 128, 1, True, 901, 672, 2199),
-    ("2byte", True, 128, 128, 1, True, 2305, 640, 843),
-    ("2byte", True, 128, 256, 1, False, 4172, 32, 2691),
-    ("2byte", True, 128, 256, 1, False, 2319, 128, 3207),
-    ("2byte", True, 128, 256, 1, True, 4492, 32, 5398),
-    ("2byte", True, 128, 256, 1, True, 3843, 128, 4301),
-    ("2byte", True, 256, 256, 1, False, 2692, 32, 2500),
-    ("2byte", True, 256, 256, 1, False, 2754, 128, 2191),
-    ("2byte", True, 256, 256, 1, True, 2051, 96, 4001),
-    ("2byte", True, 256, 256, 1, True, 3592, 128, 2265),
-    ("f32", False, 64, 64, 4, False, 582, 96, 716),
-    ("f32", False, 64, 64, 4, False, 706, 128, 578),
-    ("f32", False, 64, 128, 2, False, 515, 32, 745),
-    ("f32", False, 64, 128, 2, False, 771, 128, 1217),
-    ("f32", False, 64, 128, 2, True, 1476, 224, 1303),
-    ("f32", False, 64, 128, 2, True, 1601, 256, 1210),
-    ("f32", False, 64, 128, 4, False, 844, 1120, 1177),
-    ("f32", False, 64, 128, 4, False, 1102, 1152, 904),
-    ("f32", False, 64, 128, 4, True, 1154, 1120, 1787),
-    ("f32", False, 64, 128, 4, True, 1795, 1152, 1032),
-    ("f32", True, 64, 128, 2, False, 483, 32, 561),
-    ("f32", True, 64, 128, 2, False, 584, 128, 595),
-    ("f32", True, 64, 128, 2, True, 972, 416, 1033),
-    ("f32", True, 64, 128, 2, True, 577, 384, 1745),
-    ("f32", True, 64, 128, 4, False, 478, 1120, 731),
-    ("f32", True, 64, 128, 4, False, 591, 1152, 548),
-    ("f32", True, 64, 128, 4, True, 1607, 1120, 581),
-    ("f32", True, 64, 128, 4, True, 769, 1152, 1229),
+    ("fp4", False, 64, 64, 1, False, 517, 32, 501),
+    ("fp4", False, 64, 64, 1, False, 449, 128, 562),
+    ("fp4", False, 64, 64, 1, True, 1418, 736, 1409),
+    ("fp4", False, 64, 64, 1, True, 833, 640, 2449),
+    ("fp4", False, 64, 64, 2, False, 522, 2720, 399),
+    ("fp4", False, 64, 64, 2, False, 396, 2816, 506),
+    ("fp4", False, 64, 64, 2, True, 16388, 3616, 31),
+    ("fp4", False, 64, 64, 2, True, 8195, 5120, 79),
+    ("fp4", False, 64, 128, 1, False, 973, 32, 1347),
+    ("fp4", False, 64, 128, 1, False, 1345, 128, 964),
+    ("fp4", False, 64, 128, 1, True, 514, 32, 7596),
+    ("fp4", False, 64, 128, 1, True, 577, 128, 6907),
+    ("fp4", False, 128, 128, 1, False, 2323, 288, 1537),
+    ("fp4", False, 128, 128, 1, False, 2004, 384, 1827),
+    ("fp4", False, 128, 128, 1, True, 1936, 288, 2120),
+    ("fp4", False, 128, 128, 1, True, 1665, 384, 2381),
+    ("fp4", False, 256, 256, 1, False, 2891, 544, 3495),
+    ("fp4", False, 256, 256, 1, False, 2891, 512, 3458),
+    ("fp4", False, 256, 256, 1, True, 5902, 576, 2724),
+    ("fp4", False, 256, 256, 1, True, 3085, 512, 4922),
+    ("fp4", True, 64, 128, 1, False, 563, 32, 565),
+    ("fp4", True, 64, 128, 1, False, 547, 128, 575),
+    ("fp4", True, 64, 128, 1, True, 835, 288, 1167),
+    ("fp4", True, 64, 128, 1, True, 1224, 384, 784),
+    ("fp4", True, 128, 128, 1, False, 1228, 288, 1491),
+    ("fp4", True, 128, 128, 1, False, 1414, 384, 1289),
+    ("fp4", True, 128, 128, 1, True, 1800, 288, 1115),
+    ("fp4", True, 128, 128, 1, True, 1161, 384, 1675),
+    ("fp4", True, 256, 256, 1, False, 1922, 544, 2650),
+    ("fp4", True, 256, 256, 1, False, 2055, 512, 2439),
+    ("fp4", True, 256, 256, 1, True, 1545, 544, 4978),
+    ("fp4", True, 256, 256, 1, True, 2562, 512, 2948),
+    ("2byte", False, 64, 64, 1, False, 457, 32, 531),
+    ("2byte", False, 64, 64, 1, False, 450, 128, 644),
+    ("2byte", False, 64, 64, 1, True, 1415, 224, 1467),
+    ("2byte", False, 64, 64, 1, True, 1671, 256, 1159),
+    ("2byte", False, 64, 64, 2, False, 518, 480, 663),
+    ("2byte", False, 64, 64, 2, False, 609, 512, 545),
+    ("2byte", False, 64, 64, 2, True, 16390, 3264, 17),
+    ("2byte", False, 64, 64, 2, True, 16385, 2560, 22),
+    ("2byte", False, 64, 64, 4, False, 392, 3520, 439),
+    ("2byte", False, 64, 64, 4, False, 452, 3584, 367),
+    ("2byte", False, 64, 64, 4, True, 16400, 3840, 33),
+    ("2byte", False, 64, 128, 1, False, 1672, 32, 1155),
+    ("2byte", False, 64, 128, 1, False, 1154, 128, 1675),
+    ("2byte", False, 64, 128, 1, True, 1537, 96, 2607),
+    ("2byte", False, 64, 128, 1, True, 1543, 128, 2563),
+    ("2byte", False, 64, 128, 2, False, 908, 992, 1145),
+    ("2byte", False, 64, 128, 2, False, 1175, 1024, 839),
+    ("2byte", False, 64, 128, 4, False, 1155, 3776, 845),
+    ("2byte", False, 64, 128, 4, False, 1221, 3840, 794),
+    ("2byte", False, 64, 128, 4, True, 1219, 5312, 1659),
+    ("2byte", False, 64, 128, 4, True, 1604, 4992, 1186),
+    ("2byte", False, 128, 128, 1, False, 2575, 160, 1411),
+    ("2byte", False, 128, 128, 1, False, 2250, 256, 1540),
+    ("2byte", False, 128, 128, 1, True, 1537, 160, 2563),
+    ("2byte", False, 128, 128, 1, True, 2057, 256, 1965),
+    ("2byte", False, 128, 256, 1, False, 4884, 32, 4611),
+    ("2byte", False, 128, 256, 1, False, 4889, 128, 3111),
+    ("2byte", False, 128, 256, 1, True, 5126, 32, 4757),
+    ("2byte", False, 128, 256, 1, True, 2954, 128, 5528),
+    ("2byte", False, 256, 256, 1, False, 3595, 32, 3730),
+    ("2byte", False, 256, 256, 1, False, 3337, 128, 3587),
+    ("2byte", False, 256, 256, 1, True, 3076, 96, 5258),
+    ("2byte", False, 256, 256, 1, True, 3592, 128, 4526),
+    ("2byte", True, 64, 128, 1, False, 513, 32, 465),
+    ("2byte", True, 64, 128, 1, False, 483, 128, 611),
+    ("2byte", True, 64, 128, 1, True, 321, 96, 5662),
+    ("2byte", True, 64, 128, 1, True, 321, 128, 5584),
+    ("2byte", True, 64, 128, 2, False, 527, 1120, 437),
+    ("2byte", True, 64, 128, 2, False, 484, 1152, 456),
+    ("2byte", True, 64, 128, 4, False, 528, 3744, 356),
+    ("2byte", True, 64, 128, 4, False, 452, 3840, 391),
+    ("2byte", True, 128, 128, 1, False, 1927, 160, 965),
+    ("2byte", True, 128, 128, 1, False, 1417, 256, 1221),
+    ("2byte", True, 128, 128, 1, True, 1156, 160, 1748),
+    ("2byte", True, 128, 128, 1, True, 1155, 256, 1683),
+    ("2byte", True, 128, 256, 1, False, 2959, 32, 3815),
+    ("2byte", True, 128, 256, 1, False, 2338, 128, 3210),
+    ("2byte", True, 128, 256, 1, True, 4236, 32, 2905),
+    ("2byte", True, 128, 256, 1, True, 2694, 128, 3036),
+    ("2byte", True, 256, 256, 1, False, 2453, 32, 2769),
+    ("2byte", True, 256, 256, 1, False, 2758, 128, 2193),
+    ("2byte", True, 256, 256, 1, True, 1032, 96, 7700),
+    ("2byte", True, 256, 256, 1, True, 2576, 128, 3163),
+    ("f32", False, 64, 64, 4, False, 713, 96, 585),
+    ("f32", False, 64, 64, 4, False, 549, 128, 739),
+    ("f32", False, 64, 64, 4, True, 16386, 992, 20),
+    ("f32", False, 64, 64, 4, True, 16400, 1024, 54),
+    ("f32", False, 64, 128, 2, False, 581, 32, 659),
+    ("f32", False, 64, 128, 2, False, 1219, 128, 773),
+    ("f32", False, 64, 128, 2, True, 1802, 32, 1033),
+    ("f32", False, 64, 128, 2, True, 1611, 128, 1163),
+    ("f32", False, 64, 128, 4, False, 974, 1120, 1051),
+    ("f32", False, 64, 128, 4, False, 1155, 1152, 839),
+    ("f32", False, 64, 128, 4, True, 2306, 4704, 783),
+    ("f32", False, 64, 128, 4, True, 1793, 4096, 1045),
+    ("f32", True, 64, 128, 2, False, 513, 32, 533),
+    ("f32", True, 64, 128, 2, False, 613, 128, 561),
+    ("f32", True, 64, 128, 2, True, 773, 32, 1219),
+    ("f32", True, 64, 128, 2, True, 777, 128, 1223),
+    ("f32", True, 64, 128, 4, False, 587, 1120, 589),
+    ("f32", True, 64, 128, 4, False, 527, 1152, 609),
+    ("2byte", True, 64, 128, 4, True, 16392, 8192, 1),
+    ("f32", True, 64, 128, 4, True, 16392, 8192, 17),
 ]
-# workgroups that stay for a second and third tile: more 256 x 256 tiles than CUs
-STAY = [(False, 8656, 512, 2308), (False, 8657, 1056, 2309), (False, 4111, 640, 8237), (True, 5121, 544, 2001), (True, 5121, 512, 2000)]
+# workgroups that stay for a second and third tile: more 256 x 256 tiles than CUs, twice with rows past the last one
+STAY = [(False, 8656, 512, 2309), (False, 9985, 1056, 3079), (False, 4123, 640, 8238), (True, 2817, 544, 5389), (True, 3808, 512, 2694)]
 # weight tiles a workgroup of few rows: tiles, 2-byte x as it is, gated, n, k
 WIDE = [(1, True, False, 8191, 512), (2, True, False, 8199, 544), (2, False, False, 8192, 512), (2, True, False, 16401, 1024),
         (4, False, False, 16390, 1056), (4, True, False, 24583, 1024), (1, False, True, 16383, 1024), (2, False, True, 16391, 1024),
         (2, True, True, 16391, 1120), (1, True, True, 16391, 992), (2, True, False, 24583, 992)]
+# rows past the last tile: x as it is, and packed
+PLAIN_REST = [("bf16", 1537, 96, 2607), ("bf16", 16390, 3264, 17), ("bf16", 5126, 32, 4757),
+              ("bf16", 3076, 96, 5258), ("f32", 1802, 32, 1033), ("f32", 2306, 4704, 783)]
+PACKED_REST = [(False, 1418, 736, 1409), (False, 833, 640, 2449), (False, 16388, 3616, 31), (False, 8195, 5120, 79),
+               (False, 514, 32, 7596), (False, 577, 128, 6907), (False, 1936, 288, 2120), (False, 1665, 384, 2381),
+               (False, 5902, 576, 2724), (False, 3085, 512, 4922), (True, 835, 288, 1167), (True, 1224, 384, 784),
+               (True, 1800, 288, 1115), (True, 1161, 384, 1675), (True, 1545, 544, 4978), (True, 2562, 512, 2948)]
 ACTS = {"64": "silu", "128": "gelu_erf", "256": "gelu_tanh"}
 
 
@@ -122,7 +138,8 @@ ACTS = {"64": "silu", "128": "gelu_erf", "256": "gelu_tanh"}
 def test_tile(ops, dev, kind, gated, rows, cols, groups, split, m, k, n):
     arith = "fp4" if kind == "fp4" else "plain"
     for dt in {"fp4": ["bf16"], "2byte": ["bf16", "f16"], "f32": ["f32"]}[kind]:
-        for out, bias in (("same", True), ("f32" if dt != "f32" else "f16", False)):
+        for out, bias in (("same", True),
+              ("f32" if dt != "f32" else "f16", False)):
             if gated:
                 run_gated(ops, dev, m, k, n, dt, arith, ACTS[str(rows)], out, use_bias=bias)
             else:
@@ -131,7 +148,8 @@ def test_tile(ops, dev, kind, gated, rows, cols, groups, split, m, k, n):
 
 @pytest.mark.parametrize("gated,m,k,n", STAY)
 def test_workgroups_that_stay(ops, dev, gated, m, k, n):
-    for out, bias in (("same", True), ("f32", False)):
+    for out, bias in (("same", True),
+              ("f32", False)):
         if gated:
             run_gated(ops, dev, m, k, n, "bf16", "fp4", "gelu_tanh", out, use_bias=bias)
         else:
@@ -141,7 +159,8 @@ def test_workgroups_that_stay(ops, dev, gated, m, k, n):
 @pytest.mark.parametrize("m", [1, 5, 16])
 @pytest.mark.parametrize("tiles,plain_2byte,gated,n,k", WIDE)
 def test_wide_weights(ops, dev, m, tiles, plain_2byte, gated, n, k):
-    for dt, arith in (("bf16", "plain"), ("f16", "plain")) if plain_2byte else (("f32", "plain"), ("bf16", "fp4"), ("f32", "fp4")):
+    for dt, arith in (("bf16", "plain"), ("f16", "plain")) if plain_2byte else (("f32", "plain"), ("bf16", "fp4"),
+              ("f32", "fp4")):
         if gated:
             run_gated(ops, dev, m, k, n, dt, arith, "silu")
         else:
@@ -155,7 +174,7 @@ def test_packed_few_rows_of_wide_weights(ops, dev, m):
     assert torch.equal(ops.mxfp4_linear_fp4(ops.mxfp4_quantize(x), *w), ops.mxfp4_linear_fp4(x, *w))
 
 
-@pytest.mark.parametrize("dt,m,k,n", [("bf16", 4677, 992, 391), ("f32", 1476, 224, 1303), ("bf16", 4097, 1024, 464)])
+@pytest.mark.parametrize("dt,m,k,n", PLAIN_REST)
 def test_rows_past_the_last_tile_in_views(ops, dev, dt, m, k, n):
     """A slice of wider rows in, a slice of a wider tensor out: what lies beside and behind stays."""
     from lux3d_fused import _lib
@@ -171,7 +190,7 @@ def test_rows_past_the_last_tile_in_views(ops, dev, dt, m, k, n):
         assert bool((big == 5.0).all())
 
 
-@pytest.mark.parametrize("gated,m,k,n", [(False, 2569, 960, 3125), (False, 4612, 608, 3420), (True, 2064, 512, 3731)])
+@pytest.mark.parametrize("gated,m,k,n", PACKED_REST)
 def test_packed_rows_past_the_last_tile(ops, dev, gated, m, k, n):
     x, w, v = tokens(dev, m, k, "bf16"), weight(dev, n, k), weight(dev, n, k, 1)
     pair = ops.mxfp4_quantize(x)

@@ -43,13 +43,15 @@ def test_tile_tests_reach_the_tiles_they_name(lib):
     for gated, m, k, n in gpu.STAY:
         r, c, g, below = choose(lib, "fp4", gated, m, k, n)
         assert (r, c) == (256, 256) and -(-below // 256) * -(-n // (128 if gated else 256)) > 256, (gated, m, k, n, r, c, below)
+    for kind, gated, m, k, n in [("f32" if t[0] == "f32" else "2byte", False, *t[1:]) for t in gpu.PLAIN_REST] + [("fp4", *t) for t in gpu.PACKED_REST]:
+        assert 0 < choose(lib, kind, gated, m, k, n)[3] < m, (kind, gated, m, k, n)
     for tiles, two, gated, n, k in gpu.WIDE:
         assert lib.few_tiles(int(two), n, k, int(gated)) == tiles, (tiles, two, gated, n, k)
 
 
 def test_every_choice_is_named(lib):
     """Over the whole range no tile comes up that the GPU tests do not name, and what a tile leaves over is a few rows."""
-    named = {t[:5] for t in gpu.TILES}
+    named = {t[:6] for t in gpu.TILES}
     sizes = [17, 31, 33, 64, 65, 100, 129, 250, 257, 400, 515, 777, 1029, 1500, 2049, 2500, 4098, 6000, 9001, 16392, 40000]
     for kind, gated, m, k, n in itertools.product(KIND, (False, True), sizes, [32, 64, 96, 128, 352, 384, 416, 512, 1024, 1536, 2048, 4096, 8192],
                                                   [1, 17, 64, 130, 300, 777, 1536, 2048, 3001, 4096, 8192, 9216, 20000]):
@@ -57,7 +59,7 @@ def test_every_choice_is_named(lib):
         if below == 0:
             assert (r, c) == (16, 16)
             continue
-        assert (kind, gated, r, c, g) in named, (kind, gated, m, k, n, r, c, g, below)
+        assert (kind, gated, r, c, g, below != m) in named, (kind, gated, m, k, n, r, c, g, below)
         assert below == m or (below % r == 0 and 1 <= m - below <= 16)
         assert not (kind == "fp4" and r == 256 and k < 512)
 
