@@ -30,6 +30,11 @@
 // stages of the next tile are loaded during the last products of this one, and
 // its stores drain during the next tile's products.
 //
+// 16384 x 8192 -> 8192 of packed x 539 us (4.08 PFLOP/s), of bf16 1519 (1.45): the
+// chip's power bounds both. With zeros for data the first takes 395 (2.35 GHz
+// instead of 1.58), 4096 x 8192 -> 2048 of bf16 81 instead of 114. y's stores, in
+// bursts at the tiles' ends, take 30 of 170 us of 16384 x 2048 -> 8192 packed.
+//
 // The weights are the matrix instruction's first operand: a lane then holds four
 // consecutive outputs of one row of y, and the epilogue packs whole words.
 #include <utility>
