@@ -17,21 +17,30 @@ namespace {
 // 4.8 / 3.0 / 2.6, 4098 x 2048 bf16 5.8 / 5.0 / 5.0, 9001 x 1536 8.2 / 7.4 / 7.9,
 // 64000 x 1536 41.1 / 40.4 / 43.9, 8192 x 2048 f32 17.0 / 14.8 / 14.7: 5.1 to 6.2
 // TB/s where the launch does not count).
-constexpr int kQuantCols = 512;
-inline int64_t mx_quant_tiles(int64_t rows, int64_t k, int r) { return (k + kQuantCols - 1) / kQuantCols * ((rows + 4 * r - 1) / (4 * r)); }
+//
+// COLS: rows of up to 128 and 256 values share a wavefront's 512, 4 and 2 at a time
+// (100000 rows, us, a row a wavefront / shared: 128 bf16 12.1 / 7.7, 64 f32 12.5 /
+// 8.2, 256 bf16 14.7 / 13.6; back 7.1 / 5.5, 7.0 / 5.5, 11.1 / 11.0).
+inline int mx_quant_cols(int64_t k) { return k <= 128 ? 128 : k <= 256 ? 256 : 512; }
+inline int64_t mx_quant_tiles(int64_t rows, int64_t k, int r) {
+  const int64_t cols = mx_quant_cols(k), tile = 4 * r * 512 / cols;
+  return (k + cols - 1) / cols * ((rows + tile - 1) / tile);
+}
 
-template <typename T, int R>
+template <typename T, int R, int COLS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
   constexpr int NV = T::bytes == 4 ? 2 : 1;  // 16-byte loads a lane and row
-  __shared__ uint32_t sc[4][4 * R];
+  constexpr int L = COLS / 8, RL = 64 / L, ROWS = 4 * R * RL;  // lanes of a row; rows of a load, of the workgroup
+  __shared__ uint32_t sc[COLS / 128][ROWS];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
-  const int64_t r0 = rt * (4 * R), k = kt * kQuantCols + lane * 8;
+  const int64_t tk = (p.K + COLS - 1) / COLS, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
+  const int64_t r0 = rt * ROWS, k = kt * COLS + lane % L * 8;
+  const int lr = wave * R * RL + lane / L;  // row of the workgroup, of the lane's first
   const bool live = k < p.K;
   uint32_t v[R][4 * NV];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int64_t r = r0 + wave * R + i;
+    const int64_t r = r0 + lr + i * RL;
 #pragma unroll
     for (int j = 0; j < 4 * NV; ++j) v[i][j] = 0;
     if (live && r < p.M) {
@@ -48,18 +57,18 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int64_t r = r0 + wave * R + i;
+    const int64_t r = r0 + lr + i * RL;
     uint32_t top = mx_top<T>(v[i]);
     top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, DPP_XOR1, 0xF, 0xF, false));
     top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, DPP_XOR2, 0xF, 0xF, false));
     const uint32_t s = mx_scale(top);  // values past K count as 0: so do the scales that fill up the last group
     const uint32_t codes = mx_codes<T>(v[i], s);
     if (live && r < p.M) *reinterpret_cast<uint32_t *>(p.q + (r * p.K + k) / 2) = codes;
-    if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(&sc[lane >> 4][wave * R + i])[(lane >> 2) & 3] = (uint8_t)s;
+    if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(&sc[lane % L >> 4][lr + i * RL])[(lane >> 2) & 3] = (uint8_t)s;
   }
   __syncthreads();
-  const int64_t g = kt * 4 + t / (4 * R), r = r0 + t % (4 * R);
-  if (t < 16 * R && g * 128 < p.K && r < p.M) reinterpret_cast<uint32_t *>(p.s)[g * p.M + r] = sc[t / (4 * R)][t % (4 * R)];
+  const int64_t g = kt * (COLS / 128) + t / ROWS, r = r0 + t % ROWS;
+  if (t < 16 * R && g * 128 < p.K && r < p.M) reinterpret_cast<uint32_t *>(p.s)[g * p.M + r] = sc[t / ROWS][t % ROWS];
 }
 
 // ---- and back -------------------------------------------------------------------
@@ -68,20 +77,20 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantParams p) {
 // next lane the 16 behind them: 8 values of a 2-byte type, 4 of f32, which takes
 // the row's half in two steps (16 values a lane and four stores 64 bytes apart
 // instead: 8192 x 2048 f32 50 us against 12).
-template <typename T, int R>
+template <typename T, int R, int COLS>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
-  constexpr int V = 16 / T::bytes, STEPS = 8 / V;  // values a lane and step
+  constexpr int V = 16 / T::bytes, STEPS = 8 / V, L = COLS / 8, RL = 64 / L;  // values a lane and step; lanes of a row; rows of a store
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int64_t tk = (p.K + kQuantCols - 1) / kQuantCols, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
-  const int64_t r0 = rt * (4 * R) + wave * R;
+  const int64_t tk = (p.K + COLS - 1) / COLS, rt = (int64_t)blockIdx.x / tk, kt = blockIdx.x - rt * tk;
+  const int64_t r0 = rt * (4 * R * RL) + wave * R * RL + lane / L;
 #pragma unroll
   for (int step = 0; step < STEPS; ++step) {
-    const int64_t k = kt * kQuantCols + step * (kQuantCols / STEPS) + lane * V;
+    const int64_t k = kt * COLS + step * (COLS / STEPS) + lane % L * V;
     if (k >= p.K) return;
     uint32_t c[R], s[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int64_t r = r0 + i < p.M ? r0 + i : p.M - 1;
+      const int64_t r = r0 + i * RL < p.M ? r0 + i * RL : p.M - 1;
       const uint8_t *src = p.q + (r * p.K + k) / 2;
       if constexpr (V == 8) c[i] = *reinterpret_cast<const uint32_t *>(src);
       else c[i] = *reinterpret_cast<const uint16_t *>(src);
@@ -89,8 +98,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantParams p) {
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (r0 + i >= p.M) break;
-      void *dst = reinterpret_cast<char *>(p.y) + ((r0 + i) * p.ldy + k) * T::bytes;
+      if (r0 + i * RL >= p.M) break;
+      void *dst = reinterpret_cast<char *>(p.y) + ((r0 + i * RL) * p.ldy + k) * T::bytes;
       if constexpr (V == 8) {
         const u32x4_t v = mx_values8<T>(c[i], s[i]);
         st16(dst, make_uint4(v[0], v[1], v[2], v[3]));
@@ -148,6 +157,17 @@ template <typename X> hipError_t launch_rows_x(const MxLinearParams &p, hipStrea
 
 }  // namespace
 
+namespace {
+template <int I> using int_t = std::integral_constant<int, I>;
+template <typename F> hipError_t mx_quant_variant(bool two, int64_t k, F with) {
+  switch (mx_quant_cols(k)) {
+    case 128: return two ? with(int_t<2>{}, int_t<128>{}) : with(int_t<4>{}, int_t<128>{});
+    case 256: return two ? with(int_t<2>{}, int_t<256>{}) : with(int_t<4>{}, int_t<256>{});
+  }
+  return two ? with(int_t<2>{}, int_t<512>{}) : with(int_t<4>{}, int_t<512>{});
+}
+}  // namespace
+
 hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s) {
   if (p.M <= 0) return hipSuccess;
   const bool two = mx_quant_tiles(p.M, p.K, 4) < 512;
@@ -155,9 +175,11 @@ hipError_t launch_mx_quantize(const MxQuantParams &p, hipStream_t s) {
   if (tiles * 256 > UINT32_MAX) return hipErrorInvalidValue;  // a launch's work-items
   auto launch = [&](auto type) {
     using T = decltype(type);
-    if (two) hipLaunchKernelGGL((mx_quantize_kernel<T, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((mx_quantize_kernel<T, 4>), dim3((unsigned)tiles), dim3(256), 0, s, p);
-    return hipGetLastError();
+    auto with = [&](auto rows, auto cols) {
+      hipLaunchKernelGGL((mx_quantize_kernel<T, decltype(rows)::value, decltype(cols)::value>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+      return hipGetLastError();
+    };
+    return mx_quant_variant(two, p.K, with);
   };
   switch (p.x_dt) {
     case LUX3D_F32: return launch(F32{});
@@ -174,9 +196,11 @@ hipError_t launch_mx_dequantize(const MxDequantParams &p, hipStream_t s) {
   if (tiles * 256 > UINT32_MAX) return hipErrorInvalidValue;  // a launch's work-items
   auto launch = [&](auto type) {
     using T = decltype(type);
-    if (two) hipLaunchKernelGGL((mx_dequantize_kernel<T, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((mx_dequantize_kernel<T, 4>), dim3((unsigned)tiles), dim3(256), 0, s, p);
-    return hipGetLastError();
+    auto with = [&](auto rows, auto cols) {
+      hipLaunchKernelGGL((mx_dequantize_kernel<T, decltype(rows)::value, decltype(cols)::value>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+      return hipGetLastError();
+    };
+    return mx_quant_variant(two, p.K, with);
   };
   switch (p.y_dt) {
     case LUX3D_F32: return launch(F32{});

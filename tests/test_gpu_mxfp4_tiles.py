@@ -201,7 +201,8 @@ def test_packed_rows_past_the_last_tile(ops, dev, gated, m, k, n):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("m,k", [(8200, 64), (3001, 1632), (8191, 512), (20000, 32)])
+@pytest.mark.parametrize("m,k", [(8200, 64), (3001, 1632), (8191, 512), (70000, 32), (33001, 128), (17003, 160), (16390, 256),
+                                 (900, 96), (901, 224), (5001, 288)])
 def test_quantize_many_rows(ops, dev, m, k, dt):
     x = tokens(dev, m, k, dt)
     q, s = ops.mxfp4_quantize(x)
