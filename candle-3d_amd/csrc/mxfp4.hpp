@@ -90,12 +90,16 @@ template <typename T> __device__ __forceinline__ u32x4_t mx_values8(uint32_t w, 
 // tanh GELU v / (1 + exp(-2 sqrt(2 / pi) (v + 0.044715 v^3))) exactly, and the
 // erf GELU v / (1 + exp(-v l(v^2))) with v l(v^2) = log(Phi(v) / Phi(-v)), l an
 // even function's smooth series in v^2. So all three are v / (1 + exp2(v P(v^2)))
-// with a polynomial P of their own, one code path for the three. erf: P is
-// fitted here, degree 8 over |v| <= 5.5, by iteratively reweighted least squares
-// on 20,001 Chebyshev nodes of v^2 against log2(Phi(-v) / Phi(v)) / v: evaluated
-// in f32 its result is off by 1.7e-7 at most, and by 1.4e-5 of itself up to
-// |v| = 5.5 (half a step of f16 is 4.9e-4, of bf16 3.9e-3); past that P stays at
-// its last value (|v| Phi(-|v|) is below 1.1e-7 there).
+// with a polynomial P of their own, one code path for the three. SiLU and tanh
+// GELU: 6 u for exp2, the sum, the reciprocal and the product, and the exponent's
+// roundings, which are those of a v at most 4 u off (u = 2^-24): v is an f32 sum
+// that is further off itself. (An exponent in two parts leaves 10 u in all and
+// takes 7% of 1029 f32 rows of 1024 -> 4096.) erf: P is fitted here, degree 8
+// over |v| <= 5.5, by iteratively reweighted least squares on 20,001 Chebyshev
+// nodes of v^2 against log2(Phi(-v) / Phi(v)) / v: evaluated in f32 its result is
+// off by 1.8e-5 of itself up to |v| = 5.5 (half a step of f16 is 4.9e-4, of bf16
+// 3.9e-3); past that P stays at its last value, off by 2.4e-8. For 2-byte results;
+// f32 results take mx_gelu_erf.
 inline MxAct mx_act(int act) {
   switch (act) {
     case ACT_SILU: return {{-1.44269504f, 0, 0, 0, 0, 0, 0, 0, 0}, 0.f};
@@ -111,6 +115,28 @@ __device__ __forceinline__ float mx_activate(const MxAct &a, float v) {
 #pragma unroll
   for (int i = 7; i >= 0; --i) q = __builtin_fmaf(q, t, a.p[i]);
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * q));
+}
+
+// The erf GELU of f32 results: v (1 - q) or v q with q = Phi(-|v|) = erfc(z) / 2, z =
+// |v| / sqrt(2), in the form of Press, Teukolsky, Vetterling & Flannery, "Numerical
+// Recipes in C" (2nd ed., section 6.2): t exp(P(t) - z^2), t = 1 / (1 + z / 2), whose
+// fit is off by 2 u. 12 u in all, and the exponent's roundings as above. (P of degree
+// 8 over |v| <= 5.5: 300 u, most of it cancellation among its terms.)
+__device__ __forceinline__ float mx_gelu_erf(float v) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(v), 0.353553391f, 1.0f));
+  float p = 0.17087277f;
+  p = __builtin_fmaf(p, t, -0.82215223f);
+  p = __builtin_fmaf(p, t, 1.48851587f);
+  p = __builtin_fmaf(p, t, -1.13520398f);
+  p = __builtin_fmaf(p, t, 0.27886807f);
+  p = __builtin_fmaf(p, t, -0.18628806f);
+  p = __builtin_fmaf(p, t, 0.09678418f);
+  p = __builtin_fmaf(p, t, 0.37409196f);
+  p = __builtin_fmaf(p, t, 1.00002368f);
+  p = __builtin_fmaf(p, t, -1.26551223f);
+  const float w = __builtin_fmaf(__builtin_fmaf(-0.5f, v * v, p), 1.44269504f, -1.0f);
+  const float q = t * __builtin_amdgcn_exp2f(w);
+  return v * (v < 0 ? q : 1.0f - q);
 }
 
 // One result, rounded once to the output's type (uniform over the call).

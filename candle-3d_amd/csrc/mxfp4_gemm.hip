@@ -474,7 +474,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
             for (int e = 0; e < 16; ++e) acc[j][i][e] += part[g * (T::RING / 4) + ((j * TM + i) * 16 + e) * 64 + lane];
     }
     char *const reg = ring + T::OUT_AT + wave * 32 * T::OROW;
-    auto write = [&](auto bytes) {
+    auto write = [&](auto bytes, auto erf) {
+      constexpr bool ERF = decltype(erf)::value;
       constexpr int B = decltype(bytes)::value, JP = 4 / B, EPC = 16 / B;  // output tiles a pass; values of a piece
       constexpr int WIDTH = T::TO < JP ? T::TO * 32 : JP * 32;            // outputs of a pass
       const bool whole = (uintptr_t)p.y % 16 == 0 && p.ldy * B % 16 == 0;
@@ -496,7 +497,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 v[e] = acc[j][i][4 * q + e];
-                if constexpr (GATED) v[e] *= mx_activate(act, acc[j + T::TO][i][4 * q + e]);
+                if constexpr (ERF) v[e] *= mx_gelu_erf(acc[j + T::TO][i][4 * q + e]);
+                else if constexpr (GATED) v[e] *= mx_activate(act, acc[j + T::TO][i][4 * q + e]);
               }
               char *to = reg + l32 * T::OROW + (jj * 32 + 8 * q + 4 * h) * B;
               if constexpr (B == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
@@ -549,8 +551,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx_gemm_kernel(MxLinearP
           __builtin_amdgcn_wave_barrier();
         }
     };
-    if (p.y_dt == LUX3D_F32) write(std::integral_constant<int, 4>{});
-    else write(std::integral_constant<int, 2>{});
+    // f32 erf GELU's form costs 1 to 3% of a call (1029 x 1024 -> 4096 f32 51.1 -> 52.4 us, 4098 x 2048 -> 8192 in 4 bits 107.1 ->
+    // 110.5); chosen here, not in the loop (100 x 1024 -> 4096 17.2 us against 18.2).
+    if (p.y_dt != LUX3D_F32) write(std::integral_constant<int, 2>{}, std::false_type{});
+    else if (GATED && p.act == ACT_GELU_ERF) write(std::integral_constant<int, 4>{}, std::bool_constant<GATED>{});
+    else write(std::integral_constant<int, 4>{}, std::false_type{});
     ++tile;
     lid += step;
   } while (PERSIST && lid < end);

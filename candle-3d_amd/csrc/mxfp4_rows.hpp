@@ -166,7 +166,7 @@ __device__ __forceinline__ void mx_rows_tile(const MxLinearParams &p, const MxAc
       if (p.bias[j]) v[j] += p.bias[j][col];
     }
     float y = v[0];
-    if constexpr (GATED) y *= mx_activate(act, v[1]);
+    if constexpr (GATED) y *= p.y_dt == LUX3D_F32 && p.act == ACT_GELU_ERF ? mx_gelu_erf(v[1]) : mx_activate(act, v[1]);
     mx_store(p.y, p.y_dt, row * p.ldy + col, y);
   }
 }

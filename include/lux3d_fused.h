@@ -487,8 +487,12 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  * 238-254: Linear, chunk, gelu_erf, product) and its kin. fp4 0: the arithmetic
  * of lux3d_mxfp4_linear (xq, xs NULL); fp4 1: of lux3d_mxfp4_linear_fp4 (x, xq,
  * xs as there). gate, up: packed [n, k] of one shape; biases f32 [n] or NULL.
- * The activation is taken of the f32 sum (SiLU and tanh GELU to a few f32 ulp,
- * erf GELU to 1.7e-7 absolute), the product rounded once.
+ * The activation is taken of the f32 sum v, the product rounded once. u = 2^-24:
+ *   y f32: within 12 u of the activation of a value within 4 u of v;
+ *   y of 2 bytes: the same of SiLU and tanh GELU, 1e-5 of the result at most; erf
+ *      GELU within 2e-5 of it (half a step of f16 is 4.9e-4) down to -5.5, and
+ *      2.4e-8 below;
+ *   results below |v| 2^-126 may be 0; of -inf it is NaN, as v * sigmoid(v) is.
  *
  * In all three the order of the f32 sums depends on the shape, the number of
  * rows among it; the same shape gives the same bits. y must not overlap an
