@@ -676,7 +676,8 @@ class Mxfp4MatMul:
 
 class Mxfp4GatedMlp:
     """A gated feed-forward block: down(act(gate(x)) * up(x)), three packed weights (GeGlu, runtime/nn_blocks.rs:238-254,
-    and the Linear after it). fp4: x and the hidden values enter their products in 4 bits."""
+    and the Linear after it). fp4: x and the hidden values enter their products in 4 bits. The hidden values have x's type
+    (bf16 for a pair); out_dtype is the result's."""
 
     def __init__(self, gate: Mxfp4MatMul, up: Mxfp4MatMul, down: Mxfp4MatMul, act: str = "silu", *, gate_bias=None,
                  up_bias=None, down_bias=None, fp4: bool = False):
@@ -685,7 +686,7 @@ class Mxfp4GatedMlp:
 
     def forward(self, xs, out_dtype=None) -> torch.Tensor:
         h = mxfp4_linear_gated(xs, (self.gate.q, self.gate.scales), (self.up.q, self.up.scales), self.act,
-                               gate_bias=self.gate_bias, up_bias=self.up_bias, fp4=self.fp4, out_dtype=out_dtype)
+                               gate_bias=self.gate_bias, up_bias=self.up_bias, fp4=self.fp4)
         return self.down.forward(h, self.down_bias, out_dtype, self.fp4)
 
 

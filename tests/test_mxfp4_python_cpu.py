@@ -1,0 +1,32 @@
+"""What the Python entries of the linears on 4-bit weights pass on and refuse, without a GPU."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from lux3d_fused import _lib, ops  # noqa: E402,F401
+
+
+def packed(n, k):
+    return torch.zeros((n, k // 2), dtype=torch.uint8), torch.zeros(((k + 127) // 128, n, 4), dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("out", [None, torch.float16, torch.float32])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_feed_forward_types(monkeypatch, fp4, out):
+    """The result's type is the down-projection's alone; the hidden values have x's."""
+    seen = {}
+
+    def gated(x, gate, up, act="silu", *, gate_bias=None, up_bias=None, fp4=False, out_dtype=None):
+        seen["hidden"] = out_dtype
+        return x
+
+    def linear(x, q, scales, bias=None, out_dtype=None):
+        seen["result"] = out_dtype
+        return x
+
+    monkeypatch.setattr(ops, "mxfp4_linear_gated", gated)
+    monkeypatch.setattr(ops, "mxfp4_linear", linear)
+    monkeypatch.setattr(ops, "mxfp4_linear_fp4", linear)
+    w = ops.Mxfp4MatMul(*packed(64, 64))
+    ops.Mxfp4GatedMlp(w, w, w, fp4=fp4).forward(torch.zeros((2, 64), dtype=torch.bfloat16), out_dtype=out)
+    assert seen == {"hidden": None, "result": out}
