@@ -596,21 +596,30 @@ def mxfp4_scales(exponents: torch.Tensor) -> torch.Tensor:
     return padded.view(rows, groups, 4).transpose(0, 1).contiguous()
 
 
+def _mx_as_it_is(fn: str, x) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor):
+        raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"x must be a tensor where it is taken as it is, not {type(x).__name__}")
+    return x
+
+
 def mxfp4_linear(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
                  out_dtype=None) -> torch.Tensor:
     """`Linear::forward` (runtime/nn_blocks.rs:83-93) on a packed weight [n, k], x as it is (f32, bf16 or f16 [..., k]):
     x @ W^T (+ bias) -> [..., n] in out_dtype (default: x's)."""
     fn = "lux3d_mxfp4_linear"
+    _mx_as_it_is(fn, x)
     _one_device(fn, x, q, scales, bias)
     y = x.new_empty((*x.shape[:-1], q.shape[0]), dtype=out_dtype)
     _mx_call(fn, x, _b(x), _b(q), _b(scales), _b(bias), _b(y))
     return y
 
 
-def _mx_x(x):
+def _mx_x(fn: str, x):
     """(plain x or None, xq, xs, the tensor that leads) of an x that enters in 4 bits: a tensor, or the pair that
     mxfp4_quantize gave. More rows than few take a workspace for x's packed form."""
     if not isinstance(x, torch.Tensor):
+        if len(x) != 2 or not all(isinstance(t, torch.Tensor) for t in x):
+            raise _lib.Lux3dError(fn, _lib.ERR_VALUE, "x must be a tensor or the pair (q, scales) of a packed one")
         return None, x[0], x[1], x[0]
     shape = x.shape
     if not shape or shape[-1] == 0 or not x.is_cuda:
@@ -628,7 +637,7 @@ def mxfp4_linear_fp4(x, q: torch.Tensor, scales: torch.Tensor, bias: Optional[to
     """mxfp4_linear with x in 4 bits too: quantized here (x a tensor), or the pair that mxfp4_quantize gave (one
     quantization for several projections). out_dtype defaults to x's type, bf16 for a pair."""
     fn = "lux3d_mxfp4_linear_fp4"
-    plain, xq, xs, lead = _mx_x(x)
+    plain, xq, xs, lead = _mx_x(fn, x)
     _one_device(fn, lead, xs, q, scales, bias)
     if plain is None and out_dtype is None:
         out_dtype = torch.bfloat16
@@ -646,7 +655,7 @@ def mxfp4_linear_gated(x, gate, up, act: str = "silu", *, gate_bias: Optional[to
     code = _ACTS.get(act)
     if code is None:
         raise _lib.Lux3dError(fn, _lib.ERR_VALUE, f"act must be one of {sorted(_ACTS)}, not {act!r}")
-    plain, xq, xs, lead = _mx_x(x) if fp4 else (x, None, None, x)
+    plain, xq, xs, lead = _mx_x(fn, x) if fp4 else (x, None, None, _mx_as_it_is(fn, x))
     (gq, gs), (uq, us) = gate, up
     _one_device(fn, lead, xs, gq, gs, gate_bias, uq, us, up_bias)
     if plain is None and out_dtype is None:

@@ -30,3 +30,20 @@ def test_feed_forward_types(monkeypatch, fp4, out):
     w = ops.Mxfp4MatMul(*packed(64, 64))
     ops.Mxfp4GatedMlp(w, w, w, fp4=fp4).forward(torch.zeros((2, 64), dtype=torch.bfloat16), out_dtype=out)
     assert seen == {"hidden": None, "result": out}
+
+
+def test_a_pair_where_x_is_taken_as_it_is():
+    """A packed x belongs to the forms that take x in 4 bits."""
+    w = packed(64, 64)
+    x = packed(4, 64)
+    for call in (lambda: ops.mxfp4_linear(x, *w), lambda: ops.mxfp4_linear_gated(x, w, w),
+                 lambda: ops.mxfp4_linear_gated(list(x), w, w, fp4=False), lambda: ops.Mxfp4MatMul(*w).forward(x),
+                 lambda: ops.Mxfp4GatedMlp(*[ops.Mxfp4MatMul(*w)] * 3).forward(x)):
+        with pytest.raises(_lib.Lux3dError, match="x must be a tensor") as e:
+            call()
+        assert e.value.code == _lib.ERR_VALUE
+    for call in (lambda: ops.mxfp4_linear_fp4((x[0],), *w), lambda: ops.mxfp4_linear_gated((*x, x[0]), w, w, fp4=True),
+                 lambda: ops.mxfp4_linear_fp4((None, x[1]), *w)):
+        with pytest.raises(_lib.Lux3dError, match="pair") as e:
+            call()
+        assert e.value.code == _lib.ERR_VALUE
