@@ -589,6 +589,9 @@ def mxfp4_dequantize(q: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16
 def mxfp4_scales(exponents: torch.Tensor) -> torch.Tensor:
     """Exponent bytes u8 [rows, k / 32], as checkpoints hold them, to the grouped layout [ceil(k / 128), rows, 4] that the
     operators take (once, at load)."""
+    if exponents.dim() != 2 or exponents.dtype != torch.uint8:
+        raise _lib.Lux3dError("mxfp4_scales", _lib.ERR_DTYPE if exponents.dim() == 2 else _lib.ERR_SHAPE,
+                              f"exponents must be u8 [rows, k / 32], not {exponents.dtype} {list(exponents.shape)}")
     rows, blocks = exponents.shape
     groups = (blocks + 3) // 4
     padded = exponents.new_zeros((rows, 4 * groups))

@@ -47,3 +47,12 @@ def test_a_pair_where_x_is_taken_as_it_is():
         with pytest.raises(_lib.Lux3dError, match="pair") as e:
             call()
         assert e.value.code == _lib.ERR_VALUE
+
+
+@pytest.mark.parametrize("exponents,code", [
+    (torch.zeros(8, dtype=torch.uint8), _lib.ERR_SHAPE), (torch.zeros((2, 3, 4), dtype=torch.uint8), _lib.ERR_SHAPE),
+    (torch.zeros((4, 8), dtype=torch.int32), _lib.ERR_DTYPE), (torch.zeros((4, 8)), _lib.ERR_DTYPE)])
+def test_scales_of_another_form(exponents, code):
+    with pytest.raises(_lib.Lux3dError, match="u8 \\[rows, k / 32\\]") as e:
+        ops.mxfp4_scales(exponents)
+    assert e.value.code == code
