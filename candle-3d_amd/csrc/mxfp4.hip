@@ -130,20 +130,18 @@ hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
   return hipGetLastError();
 }
 
-// us with 4 / 8 / 16 wavefronts: 1 row, 8192 -> 2048 bf16 12.9 / 8.9 / 7.4, f32
-// 19.3 / 13.8 / 11.0; 2048 -> 8192 4.5 / 4.5 / 4.5, f32 6.8 / 6.4 / 6.9; 1536 ->
-// 9216 5.1 / 4.8 / 5.3; 33 rows, 8192 -> 2048 23.6 / 20.4 / 20.2, 1536 -> 9216
-// 13.6 / 13.0 / 14.1. Four row tiles instead of two: 64 rows, 8192 -> 2048 20.7 ->
-// 35.6, 2048 -> 8192 19.9 -> 19.6. Two groups in flight a wavefront: within 8%.
 template <typename X, bool FP4, bool GATED>
 hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
-  if (p.M > 16) return launch_rows_kernel<X, FP4, GATED, 2, 1, 8>(p, s);
   constexpr bool two_byte = !FP4 && std::conditional_t<FP4, F32, X>::bytes == 2;
-  const int nt = mx_few_tiles(two_byte, p.N, p.K, GATED);
+  const MxFewTile f = mx_few_tile(two_byte, p.M, p.N, p.K, GATED);
+  const auto is = [&](int rows, int cols, int waves) { return f.rows == rows && f.cols == cols && f.waves == waves; };
+  if (is(2, 1, 8)) return launch_rows_kernel<X, FP4, GATED, 2, 1, 8>(p, s);
+  if (is(1, 1, 8)) return launch_rows_kernel<X, FP4, GATED, 1, 1, 8>(p, s);
+  if (is(1, 1, 16)) return launch_rows_kernel<X, FP4, GATED, 1, 1, 16>(p, s);
+  if (is(1, 2, 8)) return launch_rows_kernel<X, FP4, GATED, 1, 2, 8>(p, s);
   if constexpr (!GATED)
-    if (nt == 4) return launch_rows_kernel<X, FP4, GATED, 1, 4, 8>(p, s);
-  if (nt == 2) return launch_rows_kernel<X, FP4, GATED, 1, 2, 8>(p, s);
-  return p.K >= 6144 ? launch_rows_kernel<X, FP4, GATED, 1, 1, 16>(p, s) : launch_rows_kernel<X, FP4, GATED, 1, 1, 8>(p, s);
+    if (is(1, 4, 8)) return launch_rows_kernel<X, FP4, GATED, 1, 4, 8>(p, s);
+  return hipErrorInvalidValue;
 }
 
 template <typename X, bool FP4>

@@ -43,6 +43,21 @@ inline int mx_few_tiles(bool plain_2byte, int64_t n, int64_t k, bool gated) {
   return k >= 1024 && n >= (plain_2byte ? 24576 : 16384) ? 4 : 2;
 }
 
+// The few-rows kernel's workgroup: row tiles of x and weight tiles of 16 rows each, wavefronts that share k.
+struct MxFewTile {
+  int rows, cols, waves;
+};
+
+// us with 4 / 8 / 16 wavefronts: 1 row, 8192 -> 2048 bf16 12.9 / 8.9 / 7.4, f32 19.3 / 13.8 / 11.0; 2048 -> 8192 4.5 / 4.5 /
+// 4.5, f32 6.8 / 6.4 / 6.9; 1536 -> 9216 5.1 / 4.8 / 5.3; 33 rows, 8192 -> 2048 23.6 / 20.4 / 20.2, 1536 -> 9216 13.6 / 13.0 /
+// 14.1. Four row tiles instead of two: 64 rows, 8192 -> 2048 20.7 -> 35.6, 2048 -> 8192 19.9 -> 19.6. Two groups in flight a
+// wavefront: within 8%.
+inline MxFewTile mx_few_tile(bool plain_2byte, int64_t m, int64_t n, int64_t k, bool gated) {
+  if (m > 16) return {2, 1, 8};
+  const int tiles = mx_few_tiles(plain_2byte, n, k, gated);
+  return {1, tiles, tiles == 1 && k >= 6144 ? 16 : 8};
+}
+
 // Us of the few-rows kernel: a launch, the chain of a wavefront's groups of 128
 // of k, and the loads of weights and of x, by the rows of a workgroup's tile.
 // Fitted to 48, 24 and 24 sizes of up to 16 rows and 150 to 168 of more, within
