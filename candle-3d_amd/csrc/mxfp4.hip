@@ -135,7 +135,8 @@ hipError_t launch_rows_kernel(const MxLinearParams &p, hipStream_t s) {
   constexpr bool two_byte = !FP4 && std::conditional_t<FP4, F32, X>::bytes == 2;
   const MxFewTile f = mx_few_tile(two_byte, p.M, p.N, p.K, GATED);
   const auto is = [&](int rows, int cols, int waves) { return f.rows == rows && f.cols == cols && f.waves == waves; };
-  if (is(2, 1, 8)) return launch_rows_kernel<X, FP4, GATED, 2, 1, 8>(p, s);
+  if constexpr (!FP4 || std::is_void_v<X>)  // more rows that enter in 4 bits are packed before
+    if (is(2, 1, 8)) return launch_rows_kernel<X, FP4, GATED, 2, 1, 8>(p, s);
   if (is(1, 1, 8)) return launch_rows_kernel<X, FP4, GATED, 1, 1, 8>(p, s);
   if (is(1, 1, 16)) return launch_rows_kernel<X, FP4, GATED, 1, 1, 16>(p, s);
   if (is(1, 2, 8)) return launch_rows_kernel<X, FP4, GATED, 1, 2, 8>(p, s);

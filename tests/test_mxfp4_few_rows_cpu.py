@@ -1,12 +1,15 @@
-"""Which form of the few-rows kernel each size takes (csrc/mxfp4_tiles.hpp, compiled here): the GPU tests name every form."""
+"""Which form of the few-rows kernel each size takes (csrc/mxfp4_tiles.hpp, compiled here): the GPU tests name every form, and
+no form is built that no call takes."""
 import ctypes
 import itertools
 import os
+import re
 import subprocess
 
 import pytest
 
 import test_gpu_mxfp4_few_rows as gpu
+from lux3d_fused import _lib
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "candle-3d_amd", "csrc")
 KIND = {"fp4": 0, "2byte": 1, "f32": 2}
@@ -56,3 +59,18 @@ def test_few_rows_tests_reach_the_forms_they_name(lib):
 @pytest.mark.parametrize("two", [False, True])
 def test_every_form_is_named(lib, two, gated):
     assert forms(lib, two, gated, 100) == {t[:3] for t in gpu.FEW if t[3:5] == (two, gated)}
+
+
+def test_every_built_form_is_taken(lib):
+    """The names of the kernels in the library, by their template arguments: x's type (void: packed), x in 4 bits, gated, the
+    form. Plain x of more than 16 rows that enters in 4 bits is packed first."""
+    with open(_lib.LIB_PATH, "rb") as f:
+        names = set(re.findall(rb"mx_rows_kernelI(?:NS_\d+(\w+?)E|(v))Lb([01])ELb([01])ELi(\d+)ELi(\d+)ELi(\d+)E", f.read()))
+    built = {((x or v).decode(), int(fp4), int(gated), int(mt), int(nt), int(nw)) for x, v, fp4, gated, mt, nt, nw in names}
+    taken = set()
+    for x, fp4, gated in itertools.product(("BF16", "F16", "F32", "v"), (0, 1), (0, 1)):
+        if x == "v" and not fp4:
+            continue
+        for f in forms(lib, x in ("BF16", "F16") and not fp4, gated, 16 if fp4 and x != "v" else 100):
+            taken.add((x, fp4, gated, *f))
+    assert built == taken, (built - taken, taken - built)
