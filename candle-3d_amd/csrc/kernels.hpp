@@ -218,8 +218,7 @@ struct MxLinearParams {
   int64_t rest = 0;                                         // kernel for many rows: rows behind M, 16 at most, as few rows
 };
 hipError_t launch_mx_linear(const MxLinearParams &p, hipStream_t s);
-// Its kernel for many rows (mxfp4_gemm.hip): whether a call's sizes fit it; with packed x (p.x null) or plain, not fp4.
-bool mx_gemm_fits(const MxLinearParams &p);
+// Its kernel for many rows (mxfp4_gemm.hip); with packed x (p.x null) or plain, not fp4.
 hipError_t launch_mx_gemm(const MxLinearParams &p, const MxTileId &tile, hipStream_t s);
 
 // Scaled dot-product attention over [B, H, L, D] views (element strides per

@@ -231,7 +231,7 @@ hipError_t launch_mx_linear(const MxLinearParams &given, hipStream_t s) {
   }
   const MxKind kind = !p.x ? MX_PACKED : p.x_dt == LUX3D_F32 ? MX_F32 : MX_2BYTE;
   const MxChoice c = mx_choose(kind, p.M, p.N, p.K, p.act >= 0);
-  if (c.rows == 0 || !mx_gemm_fits(p)) return launch_rows(p, s);
+  if (c.rows == 0 || !mx_gemm_fits(kind, p.ldx, p.xs_rows, p.N, p.K, p.ldy)) return launch_rows(p, s);
   p.rest = p.M - c.rows;
   p.M = c.rows;
   return launch_mx_gemm(p, c.tile, s);

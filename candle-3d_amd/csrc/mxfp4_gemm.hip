@@ -624,14 +624,6 @@ hipError_t launch_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s
 
 }  // namespace
 
-// The kernel's descriptors span 256 rows of x and of the weights, and the scales of the whole matrix; its offsets, also into
-// a tile of y, have 32 bits.
-bool mx_gemm_fits(const MxLinearParams &p) {
-  const int64_t lim = 0x7FFFFFFF, eb = p.x_dt == LUX3D_F32 ? 4 : 2;
-  return 256 * (p.x ? p.ldx * eb + 64 : p.K / 2) <= lim && 256 * p.K <= lim && 256 * 4 * p.ldy <= lim && (p.K + 127) / 32 * p.N <= lim &&
-         (p.x || (p.K + 127) / 32 * p.xs_rows <= lim);
-}
-
 hipError_t launch_mx_gemm(const MxLinearParams &p, const MxTileId &t, hipStream_t s) {
   if (!p.x) return launch_gemm<void>(p, t, s);
   switch (p.x_dt) {

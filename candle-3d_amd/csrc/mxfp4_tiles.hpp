@@ -146,4 +146,13 @@ inline MxChoice mx_choose(MxKind kind, int64_t m, int64_t n, int64_t k, bool gat
   return best;
 }
 
+// Whether a call's rows lie close enough for the kernel of many rows: its descriptors span 256 rows of x and of the weights,
+// and the scales of the whole matrix; its offsets, also into a tile of y, have 32 bits. ldx: elements between plain x's rows;
+// xs_rows: rows of packed x's scales.
+inline bool mx_gemm_fits(MxKind kind, int64_t ldx, int64_t xs_rows, int64_t n, int64_t k, int64_t ldy) {
+  const int64_t lim = 0x7FFFFFFF, s = (k + 127) / 32;  // s: a row's scales, at most
+  const int64_t xrow = kind == MX_PACKED ? k / 2 : ldx * (kind == MX_F32 ? 4 : 2) + 64;
+  return 256 * xrow <= lim && 256 * k <= lim && 256 * 4 * ldy <= lim && s * n <= lim && (kind != MX_PACKED || s * xs_rows <= lim);
+}
+
 }  // namespace lux3d
