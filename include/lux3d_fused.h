@@ -466,9 +466,11 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  * 83-93) on a packed weight, x as it is:
  *   x: f32, bf16 or f16 rows [..., k], 16-byte aligned; w, w_scales: packed [n,
  *      k]; bias: f32 [n] or NULL; y: [..., n] rows, f32 / bf16 / f16.
- * Weights enter as x's type holds them (exact in bf16 and f32; f16: exact for
- * block scales 2^-23 to 2^13, rounded beyond), products and sums are f32, f32 x
- * in three exact bf16 terms; y is rounded once. One kernel.
+ * Weights enter as x's type holds them, exact in bf16 and f32. f16 holds block
+ * scales 2^-23 to 2^13 exactly; smaller ones are rounded to its subnormals, and
+ * of larger ones the weights past 65504 are infinite (4 and 6 times 2^14, 2 to 6
+ * times 2^15): bf16 or f32 x, or x in 4 bits, takes those. Products and sums are
+ * f32, f32 x in three exact bf16 terms; y is rounded once. One kernel.
  *
  * lux3d_mxfp4_linear_fp4: x is quantized as by lux3d_mxfp4_quantize first, and
  * the products of 4-bit values run on the scaled matrix instructions, four times
