@@ -470,7 +470,8 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  * scales 2^-23 to 2^13 exactly; smaller ones are rounded to its subnormals, and
  * of larger ones the weights past 65504 are infinite (4 and 6 times 2^14, 2 to 6
  * times 2^15): bf16 or f32 x, or x in 4 bits, takes those. Products and sums are
- * f32, f32 x in three exact bf16 terms; y is rounded once. One kernel.
+ * f32, f32 x in three exact bf16 terms (below 2^-110 off by up to 2^-126; above
+ * 3.396e38, where bf16 ends, a row of NaN); y is rounded once. One kernel.
  *
  * lux3d_mxfp4_linear_fp4: x is quantized as by lux3d_mxfp4_quantize first, and
  * the products of 4-bit values run on the scaled matrix instructions, four times
