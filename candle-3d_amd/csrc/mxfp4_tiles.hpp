@@ -82,10 +82,15 @@ inline double mx_few_cost(MxKind kind, int64_t m, int64_t n, int64_t k, bool gat
 // Fitted to 70 to 320 sizes each (k 128 to 8192, 17 to 16392 rows), within 4 to
 // 16% where a tile is near the best (the 256 x 256 tile of packed x 22%). Of 1180
 // sizes timed with every tile, the tile so chosen takes 1.0% (packed), 1.6% (2
-// bytes) and 0.3% (f32) longer than the shortest on average; most of what is
-// left are 100 to 160 rows of long k (8192 -> 2048 of 100 rows 16.7 against 11.5
-// us, few rows against 64 x 64) and 128 x 256 tiles of short k (256 -> 5000 of
-// 4098 rows 35 against 27).
+// bytes) and 0.3% (f32) longer than the shortest on average. Of 624 sizes of 17 to
+// 600 rows, few rows among the forms, it takes 0.9% longer, and 20 to 43% in eight:
+// few rows where a tile is shorter (us; 160 rows of 4096 -> 1024 packed 9.5 against
+// 6.7, bf16 19.4 against 13.6, gated 22.3 against 17.1; gated, 64 rows of 256 -> 5000
+// bf16 7.3 against 5.6, of 1024 -> 4096 packed 6.2 against 5.0, 100 of 1536 -> 1536
+// packed 7.1 against 5.9), and two rows past a tile apart (130 of 4096 -> 16384 packed
+// 16.5 against 13.6, gated 32.5 against 24.2). Beside those: gated packed x of 48 rows
+// of 8192 -> 2048 (with its quantisation 19.0 against few rows' 15.6), and 128 x 256
+// tiles of short k (256 -> 5000 of 4098 rows 29.8 against 64 x 128's 25.8).
 struct MxCost {
   MxTileId tile;
   double c, a, b, s, th;

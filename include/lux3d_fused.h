@@ -498,8 +498,8 @@ int lux3d_mxfp4_dequantize(const lux3d_tensor_t *q, const lux3d_tensor_t *scales
  *   results below |v| 2^-126 may be 0; of -inf it is NaN, as v * sigmoid(v) is.
  *
  * In all three the order of the f32 sums depends on the shape, the number of
- * rows among it; the same shape gives the same bits. y must not overlap an
- * input. An infinity or NaN in x reaches its own row of y alone.             */
+ * rows among it, and on whether rows of x or y lie 4 MiB and more apart; the same
+ * shape gives the same bits. y must not overlap an input. An infinity or NaN in x reaches its own row of y alone.             */
 #define LUX3D_MXFP4_FEW_ROWS 16
 typedef enum { LUX3D_GELU_ERF = 0, LUX3D_GELU_TANH = 1, LUX3D_SILU = 2 } lux3d_act;
 int lux3d_mxfp4_linear(const lux3d_tensor_t *x, const lux3d_tensor_t *w,
